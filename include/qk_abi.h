@@ -31,7 +31,13 @@ enum qk_status {
 };
 
 /* GGUF on-disk tensor type ids (the values of ggml_type). */
-enum qk_type { QK_TYPE_F32 = 0, QK_TYPE_F16 = 1, QK_TYPE_Q4_K = 12, QK_TYPE_Q6_K = 14 };
+enum qk_type {
+    QK_TYPE_F32 = 0,
+    QK_TYPE_F16 = 1,
+    QK_TYPE_Q4_K = 12,
+    QK_TYPE_Q6_K = 14,
+    QK_TYPE_BF16 = 30 /* caches and attention rows only */
+};
 
 typedef void *qk_stream_t; /* a hipStream_t; NULL is the null stream */
 typedef void *qk_event_t;  /* a hipEvent_t */
@@ -263,6 +269,149 @@ int qk_argmax(const float *logits, int64_t count, uint32_t *result, void *worksp
 int qk_matmul_argmax(const float *x, const void *w, int type, int64_t K, int64_t N, float *logits,
                      uint32_t *result, void *workspace, size_t workspace_bytes,
                      qk_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Between the projections: a paged key/value cache, attention over it, and the
+ * choice of the next token. No counterpart with these interfaces in the
+ * reference (its cache is one fp32 array per layer, its attention and rope are
+ * src/cuda/attention.cu and src/cuda/rope.cu, its decoding is argmax).
+ * ------------------------------------------------------------------------- */
+
+/* One layer's cache: `pages` pages of `page_size` tokens (any size from 1 to
+ * 65536), keys in k and values in v, both F16 or BF16 (`type`) and laid out
+ * alike: the head_dim values of token slot t of page p and head h start at
+ * p*page_stride + t*token_stride + h*head_stride (elements; multiples of 8, so
+ * that every row is 16-byte aligned; tokens outside heads or heads outside
+ * tokens). head_dim is 64 or 128.
+ * fault: NULL, or a device word that the calls on this cache OR bits into (the
+ * caller clears it once): QK_KV_FAULT_PAGE, a page id outside [0, pages) or a
+ * position beyond the sequence's page table was met; QK_KV_FAULT_LENGTH,
+ * token_start or context did not fit together. qk_kv_check reads it. */
+typedef struct qk_kv_cache {
+    void *k;
+    void *v;
+    int type;
+    int64_t pages;
+    int64_t page_size;
+    int64_t kv_heads;
+    int64_t head_dim;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    uint32_t *fault;
+} qk_kv_cache;
+
+enum { QK_KV_FAULT_PAGE = 1, QK_KV_FAULT_LENGTH = 2 };
+
+/* The new tokens of one step, `tokens` rows of all sequences one after
+ * another. Device arrays, so that a captured step serves every length:
+ * token_start[sequences + 1], sequence s owns rows token_start[s] ..
+ * token_start[s + 1] (any number of them, none included; rows that no sequence
+ * owns are left alone); context[sequences], the tokens of the sequence up to
+ * and with its new ones, so that its new token i of n has position
+ * context - n + i; page_table[sequences x table_stride], the page id of its
+ * positions p*page_size .. in entry p. */
+typedef struct qk_kv_batch {
+    int64_t sequences;
+    int64_t tokens;
+    const int32_t *token_start;
+    const int32_t *context;
+    const int32_t *page_table;
+    int64_t table_stride;
+} qk_kv_batch;
+
+/* What happens to q and k heads on their way: RMSNorm with the head_dim
+ * weights q_norm / k_norm (NULL: none) and eps, then the rotation of the first
+ * `dims` values (a multiple of 8, at most head_dim; 0: none) by the angles
+ * position * base^(-2j/dims): pair j is values (j, j + dims/2), or (2j, 2j+1)
+ * if `interleaved`. */
+typedef struct qk_rope {
+    const float *q_norm;
+    const float *k_norm;
+    float eps;
+    float base;
+    int64_t dims;
+    int interleaved;
+} qk_rope;
+
+/* Appends the new tokens' keys and values to the cache and rotates their
+ * queries, in one launch: k and v (fp32, kv_heads x head_dim a token, tokens
+ * k_stride / v_stride floats apart) are rounded once to the cache's type and
+ * written to the page slots of their positions, k after `rope`; q (fp32,
+ * q_heads x head_dim a token, q_stride floats apart) after `rope` goes to
+ * q_out [tokens x q_heads x head_dim] as q_type (F32 or the cache's type;
+ * q_out == q is allowed for F32 with q_stride == q_heads*head_dim). q_heads ==
+ * 0 appends alone (q and q_out are not looked at). Replaces the q/k
+ * rms_norm, rope and cache writes of src/Engine.cpp:87-91. Rows whose page id
+ * or position is out of range are not stored (see qk_kv_cache::fault).
+ * Floats need 4-byte alignment; strides are multiples of 1 and at least a
+ * token's values. Angles are formed in 64 bits, everything else in fp32. */
+int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float *q,
+                 int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                 int64_t v_stride, int64_t q_heads, const qk_rope *rope, void *q_out, int q_type,
+                 qk_stream_t stream);
+
+/* out [tokens x q_heads x head_dim] = softmax(scale * q . K^T) . V for the new
+ * tokens over their sequences' cached tokens: a token at position t sees the
+ * positions j <= t, and only those with j > t - window if window > 0; query
+ * head h reads key/value head h / (q_heads / kv_heads). q rows are q_stride
+ * elements apart (a multiple of 4, rows 16-byte aligned), F32 or the cache's
+ * type (q_type); out is of q_type. lse (NULL, or fp32 [tokens x q_heads])
+ * receives log(sum of exp(scale * q . k)) for callers that join parts of a
+ * context. A row that sees nothing is 0 with lse -inf. Whatever unused page
+ * slots and later positions hold, NaN and infinities included, has no effect;
+ * pages wholly before every token's window are not looked up. If a page id that is needed
+ * is out of range, rows of that sequence are NaN (see qk_kv_cache::fault).
+ * Scores, the softmax and the sums are fp32. F32 q: q and the softmax weights
+ * meet the cached values as two F16 (three BF16) parts, so the result has
+ * fp32's precision; 16-bit q: the weights are rounded to the cache's type for
+ * the product with V, the result once at the end.
+ * max_context: the largest context the call may meet, a bound for the split of
+ * long contexts over workgroups; longer ones are still right, only slower.
+ * workspace: qk_paged_attention_workspace_size bytes, 256-byte aligned (may be
+ * NULL when that is 0), zero-filled once; every call leaves it ready for the
+ * next, calls that may run concurrently need separate ones. Nothing is
+ * allocated: the call can be captured. Replaces kernels::attention
+ * (include/Kernels.hpp:66-68, src/cuda/attention.cu:95-110). */
+int qk_paged_attention(const qk_kv_cache *cache, const qk_kv_batch *batch, const void *q,
+                       int q_type, int64_t q_stride, int64_t q_heads, float scale, int64_t window,
+                       int64_t max_context, void *out, float *lse, void *workspace,
+                       size_t workspace_bytes, qk_stream_t stream);
+
+/* Workspace bytes of qk_paged_attention for these arguments (0 for arguments
+ * that it rejects); looks at no device memory. Grows neither with the page
+ * tables nor with the cache. */
+size_t qk_paged_attention_workspace_size(const qk_kv_cache *cache, const qk_kv_batch *batch,
+                                         int q_type, int64_t q_heads, int64_t window,
+                                         int64_t max_context);
+
+/* Synchronises `stream`, then returns QK_ERR_RUNTIME (and clears the word) if
+ * a call on this cache met a fault since the last check, else QK_OK. */
+int qk_kv_check(const qk_kv_cache *cache, qk_stream_t stream);
+
+/* token[r] = an index drawn from logits[r*row_stride + 0 .. vocabulary) for
+ * each row r < rows, with the row's own parameters (device arrays of `rows`;
+ * top_k, top_p and min_p may be NULL: off): weights w = exp((logit - max) /
+ * temperature); the top_k largest are kept (<= 0: all), of these the fewest
+ * largest whose weights reach top_p of their sum (>= 1: all), of these the
+ * ones with w >= min_p; equal logits rank by index, the largest logit always
+ * stays. The result is the first kept index whose running sum, in index order,
+ * exceeds uniform[r] times the kept sum (uniform in [0, 1)). temperature 0 is
+ * argmax. NaN and -inf are never drawn; 0xFFFFFFFF if a row has nothing else;
+ * of +inf logits each weighs 1 and the rest nothing. probability (NULL, or
+ * float[rows]) receives the drawn token's share of the kept sum (0 if none).
+ * Weights are 64-bit, their sums exact in fixed point, so a result does not
+ * depend on the order of any sum. vocabulary in [1, 2^24]; row_stride >= vocabulary.
+ * workspace: qk_sample_workspace_size bytes, 256-byte aligned (may be NULL
+ * when that is 0), zero-filled once; every call leaves it ready for the next.
+ * Nothing is allocated. The reference decodes by argmax alone. */
+int qk_sample(const float *logits, int64_t rows, int64_t vocabulary, int64_t row_stride,
+              const float *temperature, const int32_t *top_k, const float *top_p,
+              const float *min_p, const float *uniform, uint32_t *token, float *probability,
+              void *workspace, size_t workspace_bytes, qk_stream_t stream);
+
+/* Workspace bytes of qk_sample (0 for arguments that it rejects). */
+size_t qk_sample_workspace_size(int64_t rows, int64_t vocabulary);
 
 /* Dequantize `rows` rows of K weights (row stride row_bytes) to fp32
  * out[rows x K], bit-identical to the formulas of src/cuda/embedding.cu:6-59.

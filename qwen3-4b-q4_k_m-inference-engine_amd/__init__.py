@@ -34,6 +34,9 @@ TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_Q4_K = 12
 TYPE_Q6_K = 14
+TYPE_BF16 = 30
+KV_FAULT_PAGE = 1
+KV_FAULT_LENGTH = 2
 SUPERBLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210}
 QK = 256
 Q8_BLOCK_BYTES = 48
@@ -50,6 +53,28 @@ class Segment(ctypes.Structure):
 
     _fields_ = [("w", ctypes.c_void_p), ("type", ctypes.c_int), ("N", ctypes.c_int64),
                 ("y", ctypes.c_void_p)]
+
+
+class KVCache(ctypes.Structure):
+    """qk_kv_cache: one layer's paged keys and values."""
+
+    _fields_ = [("k", _c_void_p), ("v", _c_void_p), ("type", _int), ("pages", _i64), ("page_size", _i64),
+                ("kv_heads", _i64), ("head_dim", _i64), ("page_stride", _i64), ("token_stride", _i64),
+                ("head_stride", _i64), ("fault", _c_void_p)]
+
+
+class KVBatch(ctypes.Structure):
+    """qk_kv_batch: the new tokens of one step."""
+
+    _fields_ = [("sequences", _i64), ("tokens", _i64), ("token_start", _c_void_p), ("context", _c_void_p),
+                ("page_table", _c_void_p), ("table_stride", _i64)]
+
+
+class Rope(ctypes.Structure):
+    """qk_rope: head norms and rotation of q and k."""
+
+    _fields_ = [("q_norm", _c_void_p), ("k_norm", _c_void_p), ("eps", _float), ("base", _float), ("dims", _i64),
+                ("interleaved", _int)]
 
 
 # name -> argument types (every function returns int status unless listed in _RESTYPES)
@@ -84,6 +109,15 @@ _SIGNATURES = {
     "qk_argmax": [_c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p],
     "qk_matmul_argmax": [_c_void_p, _c_void_p, _int, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                          _size, _c_void_p],
+    "qk_kv_append": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                     _i64, _i64, ctypes.POINTER(Rope), _c_void_p, _int, _c_void_p],
+    "qk_paged_attention": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _int, _i64, _i64, _float,
+                           _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
+    "qk_paged_attention_workspace_size": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _int, _i64, _i64, _i64],
+    "qk_kv_check": [ctypes.POINTER(KVCache), _c_void_p],
+    "qk_sample": [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                  _c_void_p, _c_void_p, _size, _c_void_p],
+    "qk_sample_workspace_size": [_i64, _i64],
     "qk_dequantize_rows": [_c_void_p, _c_void_p, _i64, _i64, _size, _int, _c_void_p],
     "qk_silu_multiply": [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p],
     "qk_rms_norm": [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _float, _c_void_p],
@@ -121,6 +155,7 @@ _SIGNATURES = {
 _RESTYPES = {"qk_last_error": ctypes.c_char_p, "qk_last_launch": ctypes.c_char_p,
              "qk_matmul_workspace_size": _size,
              "qk_argmax_workspace_size": _size, "qk_ffn_workspace_size": _size,
+             "qk_paged_attention_workspace_size": _size, "qk_sample_workspace_size": _size,
              "qk_ffn_gate_up_workspace_size": _size, "qk_matmul_segments_workspace_size": _size}
 
 _LIB = None
@@ -470,6 +505,42 @@ def quantize_q8(x, M: int, K: int, q8, stream=None) -> None:
 
 def matmul_q8(q8, w, qtype: int, K: int, N: int, y, M: int, stream=None) -> None:
     check(load().qk_matmul_q8(_ptr(q8), _ptr(w), qtype, K, N, _ptr(y), M, _stream_ptr(stream)))
+
+
+def kv_append(cache: KVCache, batch: KVBatch, q, q_stride: int, k, k_stride: int, v, v_stride: int, q_heads: int,
+              rope: Rope | None, q_out, q_type: int, stream=None) -> None:
+    """qk_kv_append: keys and values of the new tokens into their pages, q and k normed and rotated on the way."""
+    check(load().qk_kv_append(cache, batch, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride, q_heads, rope,
+                              _ptr(q_out), q_type, _stream_ptr(stream)))
+
+
+def paged_attention_workspace_size(cache: KVCache, batch: KVBatch, q_type: int, q_heads: int, window: int,
+                                   max_context: int) -> int:
+    return load().qk_paged_attention_workspace_size(cache, batch, q_type, q_heads, window, max_context)
+
+
+def paged_attention(cache: KVCache, batch: KVBatch, q, q_type: int, q_stride: int, q_heads: int, scale: float,
+                    window: int, max_context: int, out, lse, workspace, workspace_bytes: int, stream=None) -> None:
+    """qk_paged_attention: the new tokens' attention over their cached contexts."""
+    check(load().qk_paged_attention(cache, batch, _ptr(q), q_type, q_stride, q_heads, scale, window, max_context,
+                                    _ptr(out), _ptr(lse), _ptr(workspace), workspace_bytes, _stream_ptr(stream)))
+
+
+def kv_check(cache: KVCache, stream=None) -> None:
+    """Raises QKError if a call on this cache met a bad page or length (then clears the word)."""
+    check(load().qk_kv_check(cache, _stream_ptr(stream)))
+
+
+def sample_workspace_size(rows: int, vocabulary: int) -> int:
+    return load().qk_sample_workspace_size(rows, vocabulary)
+
+
+def sample(logits, rows: int, vocabulary: int, row_stride: int, temperature, top_k, top_p, min_p, uniform, token,
+           probability, workspace, workspace_bytes: int, stream=None) -> None:
+    """qk_sample: next tokens drawn with temperature, top-k, top-p and min-p from given uniforms."""
+    check(load().qk_sample(_ptr(logits), rows, vocabulary, row_stride, _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                           _ptr(min_p), _ptr(uniform), _ptr(token), _ptr(probability), _ptr(workspace),
+                           workspace_bytes, _stream_ptr(stream)))
 
 
 def dequantize_rows(packed, out, rows: int, K: int, row_stride: int, qtype: int,

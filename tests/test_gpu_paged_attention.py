@@ -1,0 +1,294 @@
+"""qk_paged_attention against the definition in 64 bits.
+
+Tolerances: u = 2^-24. A score is a sum of D products in fp32 of parts that
+hold q to 2 u; a blocked sum of that length is off by at most D/4 u of
+sum |q k|: d = (D/4 + 4) u reach, plus 2 u of the largest |score| for the
+scaling and the exponential's argument and 4 u for the exponential. A weight
+is so off by e = d + 2 u reach + 4 u relatively, the result by 2 e (weights
+and their sum) and the sums' own (64 + sqrt(keys)) u, all of sum p|v|. 16-bit q
+adds half a step of the type for the rounded weights, twice (they meet V, and
+their sum need not be theirs), and half a step of the result."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from serving_ref import BF16, F16, F32, Paged
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+class Attend:
+    def __init__(self, qk, p: Paged, q_heads, *, q_type=F32, window=0, scale=None, lse=True, pad=0, max_context=None,
+                 q_size=1.5):
+        self.qk, self.p, self.q_heads, self.q_type, self.window = qk, p, q_heads, q_type, window
+        D, T = p.dim, p.tokens
+        self.scale = np.float32(D ** -0.5 if scale is None else scale)
+        self.stride = q_heads * D + pad
+        self.q = ref.encode(p.rng.standard_normal((T, self.stride)) * q_size, q_type)
+        p.upload(qk)
+        self.qd = qk.DeviceBuffer.from_array(self.q)
+        self.out = qk.DeviceBuffer.from_array(np.full(T * q_heads * D, 0xA5A5A5A5 if q_type == F32 else 0xA5A5,
+                                                      np.uint32 if q_type == F32 else np.uint16))
+        self.lse = qk.DeviceBuffer.from_array(np.full(T * q_heads, 12345.0, np.float32)) if lse else None
+        self.max_context = max(p.contexts, default=0) if max_context is None else max_context
+        n = qk.paged_attention_workspace_size(p.cache, p.batch, q_type, q_heads, window, self.max_context)
+        self.ws = qk.DeviceBuffer.from_array(np.zeros(max(n, 256), np.uint8))
+
+    def call(self, stream=None):
+        self.qk.paged_attention(self.p.cache, self.p.batch, self.qd, self.q_type, self.stride, self.q_heads, self.scale,
+                                self.window, self.max_context, self.out, self.lse, self.ws, self.ws.nbytes, stream)
+
+    def results(self):
+        T, H, D = self.p.tokens, self.q_heads, self.p.dim
+        out = self.out.download(np.uint32 if self.q_type == F32 else np.uint16).reshape(T, H, D)
+        return out, self.lse.download(np.float32).reshape(T, H) if self.lse else None
+
+    def check(self, sequences=None):
+        p, H, D = self.p, self.q_heads, self.p.dim
+        bits, lse = self.results()
+        got = ref.decode(bits, self.q_type)
+        owned = np.zeros(p.tokens, bool)
+        step = 0.0 if self.q_type == F32 else ref.HALF_STEP[self.q_type]
+        for s, (n, c) in enumerate(zip(p.new, p.contexts)):
+            rows = slice(p.start[s], p.start[s] + n)
+            owned[rows] = True
+            if n == 0 or (sequences is not None and s not in sequences):
+                continue
+            q = ref.decode(self.q[rows, :H * D].reshape(n, H, D), self.q_type)
+            K, V = (ref.decode(p.rows(s, pool), p.kind) for pool in (p.k, p.v))
+            out, want_lse, weight, reach = ref.attention(q, K, V, c - n, float(self.scale), self.window)
+            e = ((D / 4 + 6) * reach + 4) * U
+            off = (2 * e + (64 + math.sqrt(max(c, 1))) * U + 2 * step)[..., None] * weight
+            off = off + step * (np.abs(out) + off) + (ref.TINY[self.q_type] if step else 0)
+            err = np.abs(got[rows] - out)
+            assert (err <= off).all(), (s, np.nanmax(np.where(off > 0, err / np.where(off > 0, off, 1), err * np.inf)))
+            if lse is not None:
+                none = np.isneginf(want_lse)
+                assert np.array_equal(np.isneginf(lse[rows]), none)
+                err = np.abs(np.where(none, 0, lse[rows] - want_lse))
+                top = np.where(none, 0, np.abs(want_lse))
+                assert (err <= 2 * e + (64 + math.sqrt(max(c, 1))) * U + 4 * U * top).all(), s
+        assert (bits[~owned] == (0xA5A5A5A5 if self.q_type == F32 else 0xA5A5)).all(), "rows of no sequence"
+        if lse is not None:
+            assert (lse[~owned] == 12345.0).all()
+        assert p.fault() == 0
+
+
+TYPES = {"f16-f32": (F16, F32), "f16-f16": (F16, F16), "bf16-f32": (BF16, F32), "bf16-bf16": (BF16, BF16)}
+CASES = {
+    "one-key": dict(new=[1], contexts=[1], q_heads=2),
+    "decode": dict(new=[1] * 5, contexts=[1, 15, 16, 17, 200], q_heads=8),
+    "decode-long": dict(new=[1, 1], contexts=[3000, 1025], q_heads=8, page=64),
+    "drafts": dict(new=[3, 4, 2], contexts=[3, 70, 130], q_heads=8, page=24),
+    "ragged": dict(new=[1, 37, 0, 130, 1], contexts=[300, 37, 50, 140, 1], q_heads=4),
+    "chunk": dict(new=[150], contexts=[410], q_heads=4, page=7),
+    "odd-group": dict(new=[9, 1], contexts=[30, 333], q_heads=14, kv_heads=2),
+    "no-group": dict(new=[20, 1], contexts=[31, 90], q_heads=3, kv_heads=3),
+    "wide-group": dict(new=[2, 1], contexts=[33, 65], q_heads=40, kv_heads=1),
+    "page-1": dict(new=[5], contexts=[77], q_heads=2, page=1),
+    "page-256": dict(new=[70, 1], contexts=[300, 257], q_heads=2, page=256),
+    "padding-rows": dict(new=[2, 0, 40], contexts=[9, 3, 45], q_heads=4, gaps=(3, 5)),
+    "empty-context": dict(new=[0, 2, 0], contexts=[0, 2, 0], q_heads=2),
+}
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("name", CASES)
+def test_attention_matches_its_definition(gpu, name, types):
+    kind, q_type = TYPES[types]
+    case = dict(CASES[name])
+    q_heads = case.pop("q_heads")
+    for dim, head_major in ((128, False), (64, True)):
+        print(f"[case] attention {name} {types} dim={dim}", flush=True)
+        p = Paged(kind=kind, dim=dim, head_major=head_major, seed=len(name) + dim, **case)
+        a = Attend(gpu, p, q_heads, q_type=q_type, pad=8)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", ["f16-f32", "bf16-bf16"])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 5000])
+def test_sliding_window(gpu, window, types):
+    """Pages wholly before every window may be gone: their table entries are no pages."""
+    kind, q_type = TYPES[types]
+    p = Paged([1, 90, 3], [400, 300, 3], kind=kind, dim=128, seed=window)
+    for s, (n, c) in enumerate(zip(p.new, p.contexts)):
+        gone = max(0, c - n - window + 1) // p.page
+        K, V = p.seen(p.k), p.seen(p.v)
+        for e in range(gone):  # the reference still reads the rows; it masks them
+            K[p.table[s, e]], V[p.table[s, e]] = ref.encode(np.nan, kind), ref.encode(np.nan, kind)
+    a = Attend(gpu, p, 4, q_type=q_type, window=window)
+    spoiled = p.table.copy()
+    for s, (n, c) in enumerate(zip(p.new, p.contexts)):
+        spoiled[s, :max(0, c - n - window + 1) // p.page] = -1
+    p.dev["table"].upload(spoiled)
+    a.call()
+    gpu.synchronize()
+    a.check()
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_masked_places_may_hold_anything(gpu, types):
+    """NaN and infinities in unused slots, unused pages and at positions after
+    a row: rows that do not see them are what they were."""
+    kind, q_type = TYPES[types]
+    for new, contexts in (([1, 1], [50, 131]), ([40, 3], [60, 35]), ([200], [200])):
+        p = Paged(new, contexts, kind=kind, dim=128, seed=sum(new))
+        used = np.zeros((p.pages, p.page), bool)
+        for s, c in enumerate(p.contexts):
+            pos = np.arange(c)
+            used[p.table[s, pos // p.page], pos % p.page] = True
+        for pool, value in ((p.k, np.nan), (p.v, np.inf)):
+            p.seen(pool)[~used] = ref.encode(value, kind)
+        a = Attend(gpu, p, 4, q_type=q_type)
+        a.call()
+        gpu.synchronize()
+        a.check()
+    # the last token's own key and value are not finite: rows before it do not see them
+    for value in (np.nan, np.inf, -np.inf):
+        p = Paged([40], [60], kind=kind, dim=128, seed=3)
+        K, V = p.seen(p.k), p.seen(p.v)
+        K[p.table[0, 59 // 16], 59 % 16, :, 3] = ref.encode(value, kind)
+        V[p.table[0, 59 // 16], 59 % 16, :, 5] = ref.encode(value, kind)
+        a = Attend(gpu, p, 4, q_type=q_type)
+        a.call()
+        gpu.synchronize()
+        bits, _ = a.results()
+        before = ref.decode(bits, q_type)[:39]
+        assert np.isfinite(before).all()
+        with np.errstate(invalid="ignore"):
+            K64, V64 = (ref.decode(p.rows(0, pool), kind)[:59] for pool in (p.k, p.v))
+        q = ref.decode(a.q[:39].reshape(39, 4, 128), q_type)
+        want = ref.attention(q, K64, V64, 20, float(a.scale), 0)[0]
+        assert np.abs(before - want).max() <= (1e-4 if q_type == F32 else 8 * ref.HALF_STEP[q_type])
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_a_value_that_is_infinite_reaches_only_the_rows_that_see_it(gpu, types):
+    """+inf in one value of one position: +inf in that column from there on."""
+    kind, q_type = TYPES[types]
+    p = Paged([30], [30], kind=kind, dim=64, seed=4)
+    p.seen(p.v)[p.table[0, 0], 10, :, 7] = ref.encode(np.inf, kind)
+    a = Attend(gpu, p, 2, q_type=q_type)
+    a.call()
+    gpu.synchronize()
+    out = ref.decode(a.results()[0], q_type)
+    assert np.isfinite(out[:10]).all() and np.isfinite(np.delete(out, 7, axis=2)).all()
+    assert (out[10:, :, 7] == np.inf).all()
+
+
+def test_rows_that_see_nothing_are_zero(gpu):
+    """A context shorter than its new tokens: the first of them have no
+    position, see nothing, and the misfit is reported."""
+    for q_type in (F32, F16):
+        p = Paged([5, 2], [2, 40], seed=8)
+        a = Attend(gpu, p, 4, q_type=q_type)
+        a.call()
+        gpu.synchronize()
+        bits, lse = a.results()
+        assert (bits[:3] == 0).all() and np.isneginf(lse[:3]).all()
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        with pytest.raises(gpu.QKError):
+            gpu.kv_check(p.cache)
+        a.check()
+
+
+def test_large_scores_do_not_overflow(gpu):
+    for types in TYPES:
+        kind, q_type = TYPES[types]
+        p = Paged([3, 1], [90, 300], kind=kind, dim=128, seed=13)
+        p.k = ref.encode(ref.decode(p.k, kind) * 30, kind)
+        a = Attend(gpu, p, 4, q_type=q_type, q_size=100.0, scale=1.0)
+        a.call()
+        gpu.synchronize()
+        out, lse = a.results()
+        assert np.isfinite(ref.decode(out, q_type)).all() and np.isfinite(lse).all()
+        q = ref.decode(a.q[:3].reshape(3, 4, 128), q_type)
+        K, V = (ref.decode(p.rows(0, pool), kind) for pool in (p.k, p.v))
+        want = ref.attention(q, K, V, 87, 1.0, 0)
+        assert np.abs(lse[:3] / want[1] - 1).max() <= 1e-5
+
+
+def test_q_of_any_size_keeps_its_precision(gpu):
+    """fp32 queries far outside fp16's range, their scale the inverse."""
+    for size in (1e-12, 1e9):
+        p = Paged([2, 1], [40, 77], dim=64, seed=14)
+        a = Attend(gpu, p, 4, q_size=size, scale=0.1 / size)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+def test_max_context_is_only_a_bound_for_the_split(gpu):
+    p = Paged([1, 2], [2500, 1700], dim=128, kv_heads=2, seed=15)
+    for bound in (0, 1, 100, 2500, 1 << 20):
+        a = Attend(gpu, p, 8, max_context=bound)
+        a.call()
+        a.call()  # the workspace is ready again
+        gpu.synchronize()
+        a.check()
+
+
+def test_bad_pages_are_reported_and_reach_no_other_sequence(gpu):
+    for new, contexts in (([1, 1, 1], [40, 40, 40]), ([30, 30, 30], [40, 40, 40])):
+        p = Paged(new, contexts, page=8, dim=128, seed=16)
+        p.table[1, 3] = p.pages + 5
+        a = Attend(gpu, p, 4)
+        a.call()
+        gpu.synchronize()
+        out, _ = a.results()
+        last = out[p.start[2] - 1].view(np.float32)
+        assert np.isnan(last).all()
+        assert p.fault() == gpu.KV_FAULT_PAGE
+        with pytest.raises(gpu.QKError, match="page"):
+            gpu.kv_check(p.cache)
+        a.check(sequences=(0, 2))
+
+
+def test_another_stream_and_captured_replays(gpu):
+    """A captured step over lengths that change between replays, eager calls and
+    synchronizations between them: every replay is the eager result, bit for bit."""
+    p = Paged([1, 1, 1], [600, 40, 1300], dim=128, kv_heads=2, spare=4, seed=17)
+    a = Attend(gpu, p, 8, max_context=1300)
+    stream = gpu.Stream()
+    graph = gpu.Graph.capture(stream, lambda: a.call(stream))
+    for step, contexts in enumerate(([600, 40, 1300], [601, 41, 1], [17, 33, 1299], [600, 40, 1300])):
+        print(f"[case] attention graph replay {step}", flush=True)
+        p.contexts = list(contexts)
+        p.dev["context"].upload(np.asarray(contexts, np.int32))
+        graph.launch(stream)
+        stream.synchronize()
+        replay = [x.copy() for x in a.results()]
+        a.check()
+        a.out.fill(0x5A)
+        a.call()
+        gpu.synchronize()
+        assert all(np.array_equal(x.view(np.uint32), y.view(np.uint32)) for x, y in zip(replay, a.results()))
+    graph.destroy()
+    stream.destroy()
+
+
+def test_a_page_far_into_a_large_pool(gpu):
+    """Offsets past 2^32 bytes: a pool of 4.5 GB, pages at its end."""
+    P, H, D = 64, 8, 128
+    pages = (9 << 28) // (P * H * D * 2) + 3
+    p = Paged([2], [130], kv_heads=H, dim=D, page=P, seed=18)
+    big = {n: gpu.DeviceBuffer(pages * P * H * D * 2) for n in "kv"}
+    a = Attend(gpu, p, 16)
+    far = np.array([[pages - 1, pages - 3, pages - 2]], np.int32)
+    for n, pool in (("k", p.k), ("v", p.v)):
+        for e in range(3):
+            big[n].upload(pool[p.table[0, e]], offset=int(far[0, e]) * P * H * D * 2)
+    p.dev["table"].upload(far)
+    p.cache.k, p.cache.v, p.cache.pages = big["k"].ptr, big["v"].ptr, pages
+    a.call()
+    gpu.synchronize()
+    a.check()
+    for b in big.values():
+        b.free()
