@@ -65,12 +65,19 @@ QK_HD int kv_find_sequence(const KvArgs& a, int row) {
   return lo;
 }
 
+// Where the page table holds entry `entry` of sequence s, or 0 (a place that
+// every table has) with ok cleared.
+QK_HD int64_t kv_table_at(const KvArgs& a, int s, int32_t entry, bool& ok) {
+  ok = entry >= 0 && entry < a.table_pages;
+  return ok ? s * a.table_stride + entry : 0;
+}
+
 // The page that holds entry `entry` of sequence s, or -1 if the table has no
 // such entry or the entry no such page.
 QK_HD int32_t kv_page(const KvArgs& a, int s, int32_t entry) {
-  if (entry < 0 || entry >= a.table_pages) return -1;
-  const int32_t page = a.page_table[s * a.table_stride + entry];
-  return page >= 0 && page < a.pages ? page : -1;
+  bool ok;
+  const int32_t page = a.page_table[kv_table_at(a, s, entry, ok)];
+  return ok && page >= 0 && page < a.pages ? page : -1;
 }
 
 // Element offset of (page, slot, head); page in [0, pages), slot in [0, page_size).

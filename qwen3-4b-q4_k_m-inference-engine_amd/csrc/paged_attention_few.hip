@@ -1,0 +1,350 @@
+// Paged attention for few rows a sequence: the single tokens of a decode step,
+// drafted tokens. HBM bounds it: every key and value is read once for a tile
+// of 16 rows, which one 16x16x32 MFMA takes as its columns.
+//
+// The four waves of a workgroup share nothing while they run: wave w takes
+// blocks w, w + 4, .. of 32 keys. Keys go from memory straight into the A
+// operand's layout (a lane holds 8 values of one key), values through the
+// wave's own 8 KB of LDS, from where ds_read_b64_tr_b16 brings four keys of a
+// column at a time; no barrier in the loop. Each block's loads are issued one
+// block ahead, its page ids two ahead, so 16 KB a wave are in flight under the
+// arithmetic.
+#include "paged_attention.hpp"
+
+namespace qk {
+namespace {
+
+constexpr int kRows = 16, kBlock = 32, kWaves = 4, kStep = kBlock * kWaves;
+
+// 16-byte chunks of V rows in LDS are permuted so that the eight keys which one
+// pass of a transposing read touches lie in different banks.
+template <int D>
+__device__ __forceinline__ int v_chunk(int key, int chunk) {
+  const int f = D == 128 ? (key & 7) << 1 : (key >> 1 & 3) << 1;
+  return key * (2 * D) + ((chunk ^ f) << 4);
+}
+
+template <int D, bool BF16, bool Q32>
+__global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionArgs a) {
+  typedef Num<BF16> N;
+  typedef typename N::T T;
+  typedef typename N::V8 V8;
+  constexpr int NP = kParts<BF16, Q32>;
+  constexpr int KS = D / 32, DT = D / 16;    // k steps of q.k, 16-wide tiles of the output
+  constexpr int LPK = D / 8;                 // lanes that load one key's values
+  constexpr int VL = kBlock * LPK / 64;      // loads of a block's values
+  constexpr int KPL = 64 / LPK;              // keys a load
+  struct Shared {
+    union {
+      uint8_t v[kWaves][kBlock * 2 * D];
+      float o[kWaves][kRows][D];
+    };
+    int64_t place[kWaves][2][kBlock];
+    float top[kWaves][kRows], sum[kWaves][kRows];
+    uint32_t bad, arrived;
+  };
+  __shared__ __attribute__((aligned(16))) Shared sh;
+
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
+  const int tile = unit / a.splits, split = unit % a.splits;
+  const AttentionTile t = find_tile<kRows>(a, tile);
+  if (t.s < 0) return;
+  const KeyChunk c = key_chunk(t, split, a.splits, kStep, kStep);
+  if (split >= c.used) return;
+  if (tid == 0) sh.bad = 0;
+  if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
+  __syncthreads();
+
+  // the lane's row: column of every accumulator
+  const int col = lane & 15, grp = lane >> 4;
+  const int row = t.begin + col;
+  const bool live = row < t.rows;
+  const int token = t.row + (live ? row / a.group : 0), h = head * a.group + (live ? row % a.group : 0);
+  const int position = t.first + (token - t.row);
+  const int last = live ? (position < c.hi - 1 ? position : c.hi - 1) : -1;  // keys that the row sees here: from .. last
+  const int from = a.window > 0 ? position - a.window + 1 : 0;
+  // every row sees all keys of [all_from, all_last]
+  const int all_last = t.first + t.begin / a.group;
+  const int end_row = t.begin + kRows < t.rows ? t.begin + kRows : t.rows;
+  const int all_from = a.window > 0 ? t.first + (end_row - 1) / a.group - a.window + 1 : 0;
+
+  // page ids two blocks ahead, places one ahead
+  const int blocks = (c.hi - c.lo + kBlock - 1) / kBlock;
+  int32_t page = 0;
+  bool listed = true, bad = false;
+  const auto key_of = [&](int b) {  // the lane's key of block b; keys past the end stand in for by the last one
+    const int key = c.lo + b * kBlock + (lane & 31);
+    return key < c.hi ? key : c.hi - 1;
+  };
+  const auto look_up = [&](int b) {
+    if (b < blocks) page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(b) / a.kv.page_size, listed)];
+  };
+  u32x4 kreg[2][KS], vreg[VL];
+  const auto settle = [&](int b) {  // page id -> place of block b
+    const int key = key_of(b);
+    const bool ok = listed && page >= 0 && page < a.kv.pages;
+    bad |= !ok;
+    if (lane < 32) sh.place[wave][b / kWaves & 1][lane] = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
+    __builtin_amdgcn_wave_barrier();
+  };
+  const auto load_k = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint16_t* p = a.kv.k + sh.place[wave][b / kWaves & 1][16 * i + col] + 8 * grp;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kreg[i][s] = load16(p + 32 * s);
+    }
+  };
+  const auto load_v = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      vreg[i] = load16(a.kv.v + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
+  };
+  if (wave < blocks) {
+    look_up(wave);
+    settle(wave);
+    look_up(wave + kWaves);
+    load_k(wave);
+    load_v(wave);
+  }
+
+  // q, in parts
+  V8 q[KS][NP];
+  float factor = a.scale * kLog2e;
+  {
+    const int64_t at = token * a.q_stride + static_cast<int64_t>(h) * D + 8 * grp;
+    if constexpr (Q32) {
+      float x[KS][8];
+      float most = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at + 32 * s + i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[s][i + j] = live ? v[j] : 0.0f;
+            most = fmaxf(most, fabsf(x[s][i + j]));
+          }
+        }
+      if constexpr (!BF16) {
+        most = swap32_max(swap16_max(most));
+        // 2^(14 - exponent): the row's largest value in [2^13, 2^14)
+        const bool scaled = most > 0.0f && most < __builtin_inff();
+        const int e = scaled ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;
+        factor = ldexpf(factor, -e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[s][i] = ldexpf(x[s][i], e);
+      }
+#pragma unroll
+      for (int s = 0; s < KS; ++s) split8<BF16, NP>(x[s], q[s]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const u32x4 v = load16(static_cast<const uint16_t*>(a.q) + at + 32 * s);
+        q[s][0] = __builtin_bit_cast(V8, live ? v : u32x4{});
+      }
+    }
+  }
+
+  f32x4 o[DT] = {};
+  float top = kNoMax, sum = 0.0f;
+  // the lane's part of a transposing read: key 4 grp + col / 4, and 16 on
+  const int tr_key = 4 * grp + (col >> 2);
+  const int tr_at = v_chunk<D>(tr_key, col >> 1 & 1) + (col & 1) * 8;
+  uint8_t* const vs = sh.v[wave];
+  typedef short i16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) i16x4* LdsRow;
+
+  for (int b = wave; b < blocks; b += kWaves) {
+    const int key0 = c.lo + b * kBlock;
+    f32x4 x[2] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = N::mfma16(__builtin_bit_cast(V8, kreg[i][s]), q[s][p], x[i]);
+    const int next = b + kWaves;
+    if (next < blocks) {
+      settle(next);
+      load_k(next);
+      look_up(next + kWaves);
+    }
+    // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
+    const bool whole = key0 + kBlock - 1 <= all_last && key0 + kBlock <= c.hi && key0 >= all_from;
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[i][r] *= factor;
+        if (!whole) {
+          const int key = key0 + 16 * i + 4 * grp + r;
+          x[i][r] = key <= last && key >= from ? x[i][r] : -__builtin_inff();
+        }
+        most = fmaxf(most, x[i][r]);
+      }
+    most = swap32_max(swap16_max(most));
+    if (__any(most > top + kSlack)) {
+      const float to = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[4 * i + r] = __builtin_amdgcn_exp2f(x[i][r] - (top - kLift));
+        sum += p[4 * i + r];
+      }
+    V8 w[NP];
+    split8<BF16, NP>(p, w);
+
+    // values into LDS; those of keys past the end as zeros (their weight is 0)
+    bool odd = false;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
+        odd |= any_infinite<BF16>(vreg[i]);
+      }
+      odd = __any(odd);
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int key = KPL * i + lane / LPK;
+      *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, lane % LPK)) = odd ? only_finite<BF16>(vreg[i]) : vreg[i];
+    }
+    if (next < blocks) load_v(next);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      uint8_t* const at = vs + (tr_at ^ (d << 5));
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at + 16 * 2 * D));
+      const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) o[d] = N::mfma16(__builtin_bit_cast(V8, both), w[n], o[d]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (odd) {
+      // infinite or NaN values of keys that some rows do not see: 0 times them
+      // is no zero, so they went into the product as zeros and are added here
+      // to the rows that do see them (any weight times them is themselves)
+      for (int j = 0; j < kBlock && key0 + j < c.hi; ++j) {
+        const bool sees = key0 + j <= last && key0 + j >= from;
+        const uint16_t* v = a.kv.v + sh.place[wave][b / kWaves & 1][j] + 4 * grp;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = static_cast<float>(__builtin_bit_cast(T, v[16 * d + r]));
+            if (sees && !(fabsf(e) < __builtin_inff())) o[d][r] += e;
+          }
+      }
+    }
+  }
+
+  // the four waves' parts
+  if (__any(bad) && lane == 0) sh.bad = 1;
+  sum = swap32_sum(swap16_sum(sum));
+  if (grp == 0) {
+    sh.top[wave][col] = top;
+    sh.sum[wave][col] = sum;
+  }
+  __syncthreads();  // every wave is done with its values
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&sh.o[wave][col][16 * d + 4 * grp]) = o[d];
+  __syncthreads();
+  constexpr int E = D / 16;  // values a thread: 16 threads a row
+  const int r = tid >> 4, e0 = (tid & 15) * E;
+  const bool mine = t.begin + r < t.rows;
+  float all = kNoMax, total = 0.0f, y[E] = {};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, sh.top[w][r]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(sh.top[w][r] - all);
+    total += f * sh.sum[w][r];
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] += f * sh.o[w][r][e0 + i];
+  }
+  if (sh.bad) {
+    total = __builtin_nanf("");
+    if (tid == 0) kv_fault(a.kv, QK_KV_FAULT_PAGE);
+  }
+  if (c.used > 1) {
+    const int64_t slot = (static_cast<int64_t>(tile) * a.kv.kv_heads + head) * a.splits;
+    if (mine) {
+      const int64_t at = (slot + split) * kRows + r;
+      if ((tid & 15) == 0) put(a.sums + 2 * at, all, total);
+#pragma unroll
+      for (int i = 0; i < E; i += 2) put(a.parts + at * D + e0 + i, y[i], y[i + 1]);
+    }
+    if (!last_to_arrive(a.arrived + static_cast<int64_t>(tile) * a.kv.kv_heads + head, c.used, sh.arrived)) return;
+    if (mine) {
+      all = kNoMax;
+      for (int k = 0; k < c.used; ++k) {
+        float m, l;
+        get(a.sums + 2 * ((slot + k) * kRows + r), m, l);
+        all = fmaxf(all, m);
+      }
+      total = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = 0.0f;
+#pragma unroll 4
+      for (int k = 0; k < c.used; ++k) {
+        const int64_t at = (slot + k) * kRows + r;
+        float m, l, part[E];
+        get(a.sums + 2 * at, m, l);
+#pragma unroll
+        for (int i = 0; i < E; i += 2) get(a.parts + at * D + e0 + i, part[i], part[i + 1]);
+        const float f = __builtin_amdgcn_exp2f(m - all);
+        total += f * l;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] += f * part[i];
+      }
+    }
+  }
+  if (!mine) return;
+  const int out_row = t.begin + r;
+  const int64_t at = static_cast<int64_t>(t.row + out_row / a.group) * a.q_heads + head * a.group + out_row % a.group;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if constexpr (Q32) {
+    float* out = static_cast<float*>(a.out) + at * D + e0;
+#pragma unroll
+    for (int i = 0; i < E; i += 4) *reinterpret_cast<f32x4*>(out + i) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]} * inv;
+  } else {
+    typedef T TE __attribute__((ext_vector_type(E)));
+    TE v;
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = static_cast<T>(y[i] * inv);
+    *reinterpret_cast<TE*>(static_cast<T*>(a.out) + at * D + e0) = v;
+  }
+  if (a.lse && (tid & 15) == 0) a.lse[at] = row_lse(all, total);
+}
+
+}  // namespace
+
+hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
+  const uint32_t grid = static_cast<uint32_t>(a.tiles) * a.splits * a.kv.kv_heads;
+  const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
+  auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, stream>>>(a); };
+  if (head_dim == 128)
+    bf16 ? (q32 ? go(attention_few_kernel<128, true, true>) : go(attention_few_kernel<128, true, false>))
+         : (q32 ? go(attention_few_kernel<128, false, true>) : go(attention_few_kernel<128, false, false>));
+  else
+    bf16 ? (q32 ? go(attention_few_kernel<64, true, true>) : go(attention_few_kernel<64, true, false>))
+         : (q32 ? go(attention_few_kernel<64, false, true>) : go(attention_few_kernel<64, false, false>));
+  note("attention_few_kernel", grid, head_dim, bf16, q32, a.splits > 1);
+  return hipGetLastError();
+}
+
+}  // namespace qk

@@ -233,7 +233,7 @@ hipError_t launch_sample(const SampleArgs& a, void*, hipStream_t stream) {
   int shift = 62;
   while ((int64_t{1} << (62 - shift)) < a.vocabulary) --shift;
   sample_kernel<<<a.rows, kThreads, 0, stream>>>(a, shift);
-  note("sample_kernel", a.rows, shift);
+  note("sample_kernel", a.rows);
   return hipGetLastError();
 }
 

@@ -141,8 +141,9 @@ size_t qk_paged_attention_workspace_size(const qk_kv_cache* cache, const qk_kv_b
   if (check_shapes(cache, batch) != QK_OK || check_heads(cache, batch, q_heads, q_type) != QK_OK || window < 0 ||
       max_context < 0)
     return 0;
-  return qk::paged_attention_workspace(batch->tokens, batch->sequences, q_heads, cache->kv_heads,
-                                       static_cast<int>(cache->head_dim), cache->type, q_type, window, max_context);
+  return qk::plan_attention(batch->tokens, batch->sequences, q_heads, cache->kv_heads, static_cast<int>(cache->head_dim),
+                            cache->type, q_type, window, max_context)
+      .bytes;
 }
 
 int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const void* q, int q_type, int64_t q_stride,
@@ -162,9 +163,10 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
   if (!q || !out) return refuse("attention pointers must be non-null");
   if (misaligned(q, 16) || misaligned(out, 16) || misaligned(lse, 4))
     return refuse("attention q and out must be 16-byte, lse 4-byte aligned");
-  const size_t need = qk::paged_attention_workspace(batch->tokens, batch->sequences, q_heads, cache->kv_heads,
-                                                    static_cast<int>(cache->head_dim), cache->type, q_type, window,
-                                                    max_context);
+  const qk::AttentionPlan plan =
+      qk::plan_attention(batch->tokens, batch->sequences, q_heads, cache->kv_heads, static_cast<int>(cache->head_dim),
+                         cache->type, q_type, window, max_context);
+  const size_t need = plan.bytes;
   if (need != 0 && !workspace) return refuse("attention workspace must be non-null");
   if (workspace_bytes < need) return refuse("attention workspace too small");
   if (misaligned(workspace, 256)) return refuse("attention workspace must be 256-byte aligned");
@@ -178,8 +180,8 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
   a.window = window < INT32_MAX ? static_cast<int32_t>(window) : 0;  // positions are below 2^31: all are seen
   a.out = out;
   a.lse = lse;
-  return finish(qk::launch_paged_attention(a, cache->type, static_cast<int>(cache->head_dim), q_type, max_context,
-                                           workspace, as_stream(stream)),
+  return finish(qk::launch_paged_attention(a, plan, cache->type, static_cast<int>(cache->head_dim), q_type, workspace,
+                                           as_stream(stream)),
                 "paged attention launch failed");
 }
 

@@ -43,11 +43,27 @@ struct AttentionArgs {
   int32_t window;  // 0: none
   void* out;
   float* lse;
+  // the plan's part (launch_paged_attention)
+  int32_t tiles, splits;
+  uint32_t* arrived;  // [tiles x kv_heads], zero between calls
+  float* sums;        // [tiles x kv_heads x splits x rows] (maximum, sum) pairs
+  float* parts;       // [tiles x kv_heads x splits x rows x head_dim]
 };
-hipError_t launch_paged_attention(const AttentionArgs& a, int type, int head_dim, int q_type, int64_t max_context,
+
+// How a call is laid out, from host values alone.
+struct AttentionPlan {
+  bool few;              // 16-row tiles (paged_attention_few.hip), else 128 or 256 (paged_attention_many.hip)
+  int rows;              // rows of a tile: (new token, query head of the key/value head)
+  int32_t tiles;         // at most so many tiles
+  int32_t splits;        // workgroups that may share a tile's keys
+  size_t sums_at, parts_at, bytes;  // workspace; 0 bytes without splits
+};
+AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int head_dim, int type,
+                             int q_type, int64_t window, int64_t max_context);
+hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, int type, int head_dim, int q_type,
                                   void* workspace, hipStream_t stream);
-size_t paged_attention_workspace(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int head_dim,
-                                 int type, int q_type, int64_t window, int64_t max_context);
+hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
+hipError_t launch_attention_many(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
 
 struct SampleArgs {
   const float* logits;
