@@ -8,6 +8,11 @@ namespace {
 // The card's compute units: a plan, and with it a workspace's size, is the
 // same with and without a device at hand.
 constexpr int64_t kUnits = 256;
+// Keys are shared out only while a plan has fewer (tile, head) units than this,
+// so the counters of every plan fit one fixed region at the workspace's start:
+// no call's parts lie where a call of another batch keeps its counters.
+constexpr int64_t kMostUnits = 2 * kUnits;
+constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -28,14 +33,14 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   p.tiles = static_cast<int32_t>(tiles);
   int64_t keys = max_context < 1 ? 1 : max_context;
   if (window > 0 && keys > window + tile_rows) keys = window + tile_rows;
-  const int64_t want = p.few ? 2 * kUnits : (q_type == QK_TYPE_F32 ? 2 * kUnits : kUnits);
+  const int64_t want = p.few || q_type == QK_TYPE_F32 ? kMostUnits : kUnits;
   const int64_t least = p.few ? 128 : 256;
   int64_t splits = up(want, tiles * kv_heads);
   if (splits > up(keys, least)) splits = up(keys, least);
   p.splits = static_cast<int32_t>(splits);
   if (splits > 1) {
     const size_t units = static_cast<size_t>(tiles * kv_heads), parts = units * splits * tile_rows;
-    p.sums_at = (units * sizeof(uint32_t) + 255) & ~size_t{255};
+    p.sums_at = kCounterBytes;
     p.parts_at = p.sums_at + ((parts * 2 * sizeof(float) + 255) & ~size_t{255});
     p.bytes = p.parts_at + parts * head_dim * sizeof(float);
   }

@@ -24,7 +24,7 @@
 namespace qk {
 
 constexpr float kLift = 8.0f, kSlack = 6.0f;
-constexpr float kNoMax = -3.0e38f;  // the maximum of no score
+constexpr float kNoMax = -3.4028234e38f;  // the maximum of no score: no finite score is below it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <bool BF16>

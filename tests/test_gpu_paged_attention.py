@@ -235,6 +235,22 @@ def test_max_context_is_only_a_bound_for_the_split(gpu):
         a.check()
 
 
+def test_one_workspace_serves_batches_of_all_sizes(gpu):
+    """Batches of few and many tiles in turn on the same bytes, zero-filled once."""
+    calls = []
+    for i, (new, context, q_type) in enumerate((([1], [3000], F32), ([1] * 40, [700] * 40, F16), ([150], [1800], F32),
+                                                ([1] * 9, [1500] * 9, F32), ([300, 290], [2000, 1000], F16))):
+        calls.append(Attend(gpu, Paged(new, context, dim=128, kv_heads=2, seed=30 + i), 8, q_type=q_type))
+    ws = gpu.DeviceBuffer.from_array(np.zeros(max(a.ws.nbytes for a in calls), np.uint8))
+    for a in calls:
+        a.ws = ws
+    for a in calls + calls[::-1]:
+        a.out.fill(0x5A)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
 def test_bad_pages_are_reported_and_reach_no_other_sequence(gpu):
     for new, contexts in (([1, 1, 1], [40, 40, 40]), ([30, 30, 30], [40, 40, 40])):
         p = Paged(new, contexts, page=8, dim=128, seed=16)
