@@ -1,14 +1,29 @@
 // The next token of each row by temperature, top-k, top-p and min-p from a
-// given uniform: one workgroup per row.
+// given uniform, in two launches.
+//
+// sample_scan_kernel reads every logit once, one workgroup per chunk of a row
+// (2048 or 8192 logits, all in registers): the chunk's maximum; how many
+// logits lie in each of 128 bands below it, a quarter of the temperature wide
+// (at most 1/4), and, where no top-k bounds the kept set, the sum of their
+// weights; and the logits of the top bands themselves, as many as the row's
+// top-k can take from one chunk. sample_draw_kernel, one workgroup per row,
+// adds the bands up, which gives the band that a filter's border falls into,
+// and then
+//   - where the chunks' lists reach down to that band (the usual filters),
+//     sorts the listed logits and finds everything among them;
+//   - without top-k, reads the row once more for the logits of that band
+//     alone, or not at all if there is no border (bare temperature), picks the
+//     drawn token's chunk by the chunks' sums and reads that again;
+//   - else (thousands of logits around a border: equal ones, high
+//     temperatures) searches the row digit by digit.
 //
 // Values are ranked by a 32-bit key whose unsigned order is the order of the
-// logits (NaN and -inf: 0, never drawn). top-k and top-p are the same search:
-// the largest key K whose measure of {key >= K} reaches a target, the measure
-// being a count or a sum of weights; it is found digit by digit (11, 11, 10
-// bits) from a histogram of the values that share the digits found so far.
-// Weights are fixed-point integers, rint(exp((z - max) / T) * 2^shift) of a
-// 64-bit exponential with 2^shift * vocabulary < 2^62, so every sum is exact
-// and no order of additions can change a result.
+// logits (NaN and -inf: 0, never drawn). Weights are fixed-point integers,
+// rint(exp((z - max) / T) * 2^shift) of a 64-bit exponential with 2^shift *
+// vocabulary < 2^62, so their sums are exact and no order of additions can
+// change a result; a chunk whose own maximum is not the row's is weighed by
+// its own and scaled once per band, in 64-bit floating point. Bands only say
+// where to look; no result depends on their width.
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -16,8 +31,29 @@
 namespace qk {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;     // of the draw
 constexpr int kBins = 2048;
+constexpr int kScanThreads = 256;
+constexpr int kBands = 128;
+constexpr int kList = 512;         // most listed logits of a chunk
+constexpr int kItems = 8192;       // most logits of a band that the draw holds
+constexpr int kSorted = 2 * kThreads;
+constexpr int kMostChunks = 2048;
+constexpr int kFew = 128;          // listed logits of a chunk without top-k
+
+// What the scan leaves of a chunk.
+struct ChunkHead {
+  uint32_t key, index;     // of its largest logit (0: nothing to draw, and nothing else is written)
+  int32_t listed, through; // entries of its list: the logits of bands 0 .. through - 1
+};
+struct SamplePlan {
+  int32_t chunk, chunks, list, shift;
+  ChunkHead* heads;   // [rows x chunks]
+  uint16_t* counts;   // [rows x chunks][kBands]
+  uint64_t* weights;  // [rows x chunks][kBands]
+  uint64_t* lists;    // [rows x chunks][list]: key << 32 | ~index
+  size_t bytes;
+};
 
 __device__ __forceinline__ uint32_t rank_key(float v) {
   if (!(v > -__builtin_inff())) return 0;
@@ -39,10 +75,162 @@ struct Weigher {
   }
 };
 
+// The band of v below top (v <= top, both above -inf). The same for a chunk's
+// maximum against the row's, so that bands of chunks add up: values times
+// `scale` that are closer than kBands have exact differences.
+__device__ __forceinline__ int band_of(float v, float top, float scale) {
+  if (v == top) return 0;
+  const float d = floorf(top * scale) - floorf(v * scale);
+  return d < static_cast<float>(kBands - 1) ? static_cast<int>(d) : kBands - 1;  // NaN (of infinities): the last
+}
+__device__ __forceinline__ float band_scale(float heat) { return fmaxf(4.0f / heat, 4.0f); }
+__device__ __forceinline__ uint64_t item_of(uint32_t key, int index) {
+  return static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ uint32_t item_key(uint64_t item) { return static_cast<uint32_t>(item >> 32); }
+__device__ __forceinline__ int item_index(uint64_t item) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(item)); }
+__device__ __forceinline__ void lds_add(uint64_t* p, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(p), static_cast<unsigned long long>(v));
+}
+// Four logits from x[at]; what lies past n reads as -inf.
+__device__ __forceinline__ f32x4 load_logits(const float* x, int at, int n) {
+  if (at + 4 <= n) return *reinterpret_cast<const f32x4_a4*>(x + at);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = at + e < n ? x[at + e] : -__builtin_inff();
+  return v;
+}
+// Appends the lanes' items where `mine`, a place for each from *count.
+__device__ __forceinline__ void append(bool mine, uint64_t item, uint64_t* items, uint32_t* count, uint32_t most) {
+  const uint64_t who = __ballot(mine);
+  if (!who) return;
+  const int lane = static_cast<int>(threadIdx.x & 63), leader = __builtin_ctzll(who);
+  uint32_t base = 0;
+  if (lane == leader) base = atomicAdd(count, static_cast<uint32_t>(__popcll(who)));
+  base = __builtin_amdgcn_readlane(base, leader);
+  const uint32_t at = base + static_cast<uint32_t>(__popcll(who & ((uint64_t{1} << lane) - 1)));
+  if (mine && at < most) items[at] = item;
+}
+
+// The scan. HBM bounds it: 200 rows of 151936 logits, 121 MB. A thread's
+// logits are all loaded before any is looked at (16 bytes x E in flight a
+// lane); band counts are spread over four copies by lane, as neighbouring
+// logits often share a band.
+template <int E>
+__global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleArgs a, const SamplePlan p) {
+  __shared__ uint64_t weight[kBands * 4];
+  __shared__ uint32_t count[kBands * 4];
+  __shared__ float tops[kScanThreads / 64];
+  __shared__ uint32_t first, listed;
+  __shared__ int32_t depth;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  const int row = static_cast<int>(blockIdx.y), lo = static_cast<int>(blockIdx.x) * p.chunk;
+  const int n = min(a.vocabulary - lo, p.chunk);
+  const int64_t unit = static_cast<int64_t>(row) * p.chunks + blockIdx.x;
+  const float* x = a.logits + row * a.row_stride + lo;
+  f32x4 v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = load_logits(x, (i * kScanThreads + tid) * 4, n);
+  const float heat = a.temperature[row];
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const bool cut = k > 0 && k < a.vocabulary;  // the kept set is bounded: no sums of bands are needed
+  for (int i = tid; i < kBands * 4; i += kScanThreads) {
+    count[i] = 0;
+    if (!cut) weight[i] = 0;
+  }
+  if (tid == 0) first = 0xFFFFFFFFu, listed = 0;
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);  // NaN: the other operand
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kScanThreads / 64; ++w) top = fmaxf(top, tops[w]);
+  if (!(top > -__builtin_inff())) {
+    if (tid == 0) p.heads[unit] = ChunkHead{0, 0, 0, 0};
+    return;
+  }
+  const uint32_t top_key = rank_key(top);
+  const bool greedy = !(heat > 0.0f);
+  const float scale = band_scale(heat);
+  const Weigher w{static_cast<double>(key_value(top_key)), 1.0 / heat, static_cast<double>(uint64_t{1} << p.shift)};
+  uint32_t mine = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float z = v[i][e];
+      if (z == top) mine = min(mine, static_cast<uint32_t>(lo + (i * kScanThreads + tid) * 4 + e));
+      if (!greedy && z > -__builtin_inff()) {
+        const int at = band_of(z, top, scale) * 4 + (lane & 3);
+        atomicAdd(&count[at], 1u);
+        if (!cut) lds_add(&weight[at], w.fixed(rank_key(z)));
+      }
+    }
+  if (mine != 0xFFFFFFFFu) atomicMin(&first, mine);
+  __syncthreads();
+  if (greedy) {
+    if (tid == 0) p.heads[unit] = ChunkHead{top_key, first, 0, 0};
+    return;
+  }
+  if (wave == 0) {  // lane: bands 2 lane and 2 lane + 1
+    uint32_t c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t* q = count + (2 * lane + i) * 4;
+      c[i] = q[0] + q[1] + q[2] + q[3];
+    }
+    reinterpret_cast<uint32_t*>(p.counts + unit * kBands)[lane] = c[0] | c[1] << 16;
+    uint32_t run = c[0] + c[1];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t other = __shfl_up(run, off);
+      if (lane >= off) run += other;
+    }
+    // as many bands as hold what the row may need of this chunk, and as the list holds
+    const uint32_t want = cut ? k : kFew, most = p.list;
+    const int enough = __popcll(__ballot(run - c[1] < want)) + __popcll(__ballot(run < want)) + 1;
+    const int fit = __popcll(__ballot(run - c[1] <= most)) + __popcll(__ballot(run <= most));
+    const int through = min(min(enough, fit), kBands);
+    const uint32_t held = through == 0 ? 0 : __shfl(through & 1 ? run - c[1] : run, (through - 1) >> 1);
+    if (lane == 0) {
+      depth = through;
+      p.heads[unit] = ChunkHead{top_key, first, static_cast<int32_t>(held), through};
+    }
+  } else if (!cut && wave == 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t* q = weight + (2 * lane + i) * 4;
+      p.weights[unit * kBands + 2 * lane + i] = q[0] + q[1] + q[2] + q[3];
+    }
+  }
+  __syncthreads();
+  const int through = depth;
+  uint64_t* list = p.lists + unit * p.list;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float z = v[i][e];
+      append(z > -__builtin_inff() && band_of(z, top, scale) < through,
+             item_of(rank_key(z), lo + (i * kScanThreads + tid) * 4 + e), list, &listed, p.list);
+    }
+}
+
 struct Shared {
+  uint64_t items[kItems];
   uint64_t bins[kBins];
+  uint64_t sums[kMostChunks];
+  uint64_t weight[kBands];
+  uint32_t count[kBands];  // later its running sums
   uint64_t wave[16];
   uint64_t found[3];
+  uint64_t above, total;
+  uint32_t border, floor_key, n, low, high;
 };
 
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
@@ -144,41 +332,422 @@ __device__ int walk(const float* x, int n, uint64_t beyond, F measure, Shared& s
   return static_cast<int>(sh.found[0]);
 }
 
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, int shift) {
+// Exclusive running sum of v over the workgroup, and the sum of all.
+__device__ uint64_t group_prefix(uint64_t v, uint64_t& all, Shared& sh) {
+  const int lane = static_cast<int>(threadIdx.x & 63), wave = static_cast<int>(threadIdx.x >> 6);
+  uint64_t run = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t other = __shfl_up(run, off);
+    if (lane >= off) run += other;
+  }
+  __syncthreads();
+  if (lane == 63) sh.wave[wave] = run;
+  __syncthreads();
+  uint64_t before = 0;
+  all = 0;
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i < wave) before += sh.wave[i];
+    all += sh.wave[i];
+  }
+  return before + run - v;
+}
+
+// items[0 .. n) sorted downwards, n <= kSorted, in room for the next power of
+// two; all threads call it after a barrier, a barrier ends it. Steps
+// over a distance of up to 64 stay within the 128 items of a wave's 64 pairs.
+__device__ void sort_down(uint64_t* items, int n) {
+  const int tid = static_cast<int>(threadIdx.x);
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int i = n + tid; i < size; i += kThreads) items[i] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run <<= 1)
+    for (int d = run >> 1; d > 0; d >>= 1) {
+      if (tid < size / 2) {
+        const int i = (tid & ~(d - 1)) << 1 | (tid & (d - 1));
+        const uint64_t x = items[i], y = items[i + d];
+        if ((x < y) == ((i & run) == 0)) {
+          items[i] = y;
+          items[i + d] = x;
+        }
+      }
+      const int next = d > 1 ? d >> 1 : run;
+      if (d > 64 || next > 64) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  __syncthreads();
+}
+
+// One pass over the row that appends the logits of `band` to sh.items (more
+// than fit are counted), with the largest and smallest key in sh.high / low.
+__device__ void gather_band(const float* x, int n, int band, float top, float scale, Shared& sh) {
+  const float origin = floorf(top * scale), want = static_cast<float>(band);
+  uint32_t low = 0xFFFFFFFFu, high = 0;
+  constexpr int kAhead = 8;  // loads in flight a lane
+  for (int base = 0; base < n; base += 4 * kThreads * kAhead) {
+    f32x4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = load_logits(x, base + (i * kThreads + static_cast<int>(threadIdx.x)) * 4, n);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = v[i][e], d = origin - floorf(z * scale);  // band_of, decided for one band
+        const bool in = band == kBands - 1 ? !(d < want) : d == want;
+        const bool hit = z == top ? band == 0 : in && z > -__builtin_inff();
+        const uint32_t key = rank_key(z);
+        if (hit) {
+          low = min(low, key);
+          high = max(high, key);
+        }
+        append(hit, item_of(key, base + (i * kThreads + static_cast<int>(threadIdx.x)) * 4 + e), sh.items, &sh.n, kItems);
+      }
+  }
+  if (high) {
+    atomicMin(&sh.low, low);
+    atomicMax(&sh.high, high);
+  }
+  __syncthreads();
+}
+
+// The draw: a few dependent reads of what the scan left, a sort in LDS and
+// running sums; latency bounds it.
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs a, const SamplePlan p) {
   __shared__ Shared sh;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int row = static_cast<int>(blockIdx.x), n = a.vocabulary;
   const float* x = a.logits + row * a.row_stride;
+  const int64_t unit0 = static_cast<int64_t>(row) * p.chunks;
+  const ChunkHead* heads = p.heads + unit0;
   const float heat = a.temperature[row];
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const bool cut = k > 0 && k < n;
+  const double share = a.top_p ? static_cast<double>(a.top_p[row]) : 1.0;
+  const double floor_w = a.min_p ? static_cast<double>(a.min_p[row]) : 0.0;
+  const float uniform = a.uniform[row];
+  if (tid < kBands) sh.count[tid] = 0, sh.weight[tid] = 0;
+  if (tid == 0) sh.n = 0, sh.low = 0xFFFFFFFFu, sh.high = 0;
   uint64_t best = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t key = rank_key(x[i]);
-    const uint64_t c = key ? (static_cast<uint64_t>(key) << 32) | (0xFFFFFFFFu - i) : 0;
-    best = c > best ? c : best;
+  for (int c = tid; c < p.chunks; c += kThreads) {
+    const ChunkHead h = heads[c];
+    const uint64_t item = h.key ? item_of(h.key, static_cast<int>(h.index)) : 0;
+    best = item > best ? item : best;
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     const uint64_t other = __shfl_xor(best, off);
     best = other > best ? other : best;
   }
-  if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = best;
+  if (lane == 0) sh.wave[wave] = best;
   __syncthreads();
   for (int i = 0; i < kThreads / 64; ++i) best = sh.wave[i] > best ? sh.wave[i] : best;
   if (!(heat > 0.0f) || best == 0) {
-    if (threadIdx.x == 0) {
-      a.token[row] = best ? 0xFFFFFFFFu - static_cast<uint32_t>(best) : 0xFFFFFFFFu;
+    if (tid == 0) {
+      a.token[row] = best ? static_cast<uint32_t>(item_index(best)) : 0xFFFFFFFFu;
       if (a.probability) a.probability[row] = best ? 1.0f : 0.0f;
     }
     return;
   }
-  const uint32_t top = static_cast<uint32_t>(best >> 32);
-  const Weigher w{static_cast<double>(key_value(top)), 1.0 / heat, static_cast<double>(uint64_t{1} << shift)};
+  const uint32_t top = item_key(best);
+  const float top_value = key_value(top), scale = band_scale(heat);
+  const Weigher w{static_cast<double>(top_value), 1.0 / heat, static_cast<double>(uint64_t{1} << p.shift)};
 
-  // kept: keys above `least`, and of those equal to it the ones up to index
-  // `last`
+  // the row's bands: those of chunk c are base(c) further down. A unit is
+  // eight bands of a chunk; sum(weights) is their part of them.
+  const auto chunk_sums = [&](const ChunkHead& h, int64_t at, uint64_t (&out)[8]) {
+    const uint64_t* q = p.weights + at;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = q[j];
+    if (h.key != top) {
+      const double factor = w.ratio(h.key);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] = static_cast<uint64_t>(rint(static_cast<double>(out[j]) * factor));
+    }
+  };
+  for (int u = tid; u < p.chunks * (kBands / 8); u += kThreads) {
+    const int c = u / (kBands / 8), j0 = u % (kBands / 8) * 8;
+    const ChunkHead h = heads[c];
+    if (!h.key) continue;
+    const int base = band_of(key_value(h.key), top_value, scale) + j0;
+    const int64_t at = (unit0 + c) * kBands + j0;
+    const u16x8 counts = *reinterpret_cast<const u16x8*>(p.counts + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (counts[j]) atomicAdd(&sh.count[min(base + j, kBands - 1)], static_cast<uint32_t>(counts[j]));
+    if (!cut) {
+      uint64_t sums[8];
+      chunk_sums(h, at, sums);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (sums[j]) lds_add(&sh.weight[min(base + j, kBands - 1)], sums[j]);
+    }
+  }
+  __syncthreads();
+  const auto target_of = [&](uint64_t total) {  // fewest whose weights reach the share: the sum to reach
+    const double goal = ceil(share * static_cast<double>(total));
+    return goal < 1.0 ? uint64_t{1} : min(total, static_cast<uint64_t>(goal));
+  };
+  if (wave == 0) {  // lane: bands 2 lane and 2 lane + 1; the border band of top-k, or else of top-p
+    const uint32_t c0 = sh.count[2 * lane], c1 = sh.count[2 * lane + 1];
+    const uint64_t w0 = sh.weight[2 * lane], w1 = sh.weight[2 * lane + 1];
+    uint32_t counts = c0 + c1;
+    uint64_t sums = w0 + w1;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t c = __shfl_up(counts, off);
+      const uint64_t s = __shfl_up(sums, off);
+      if (lane >= off) counts += c, sums += s;
+    }
+    sh.count[2 * lane] = counts - c1;
+    sh.count[2 * lane + 1] = counts;
+    const uint64_t total = __shfl(sums, 63);
+    if (cut) {
+      const uint32_t want = static_cast<uint32_t>(k);
+      const int b = __popcll(__ballot(counts - c1 < want)) + __popcll(__ballot(counts < want));
+      if (lane == 0) sh.border = min(b, kBands - 1);
+    } else {
+      const uint64_t target = target_of(total);
+      const int b = __popcll(__ballot(sums - w1 < target)) + __popcll(__ballot(sums < target));
+      const uint64_t before = __shfl(b & 1 ? sums - w1 : sums - w1 - w0, min(b >> 1, 63));
+      if (lane == 0) {
+        sh.border = share < 1.0 ? b : kBands;
+        sh.above = before;
+        sh.total = total;
+      }
+    }
+  } else if (wave == 1) {  // the smallest key that min-p keeps, 64 candidates at a time
+    uint32_t lo = 1, hi = top;
+    if (!(floor_w <= 0.0))
+      while (lo < hi) {
+        const uint32_t step = (hi - lo) / 64 + 1, off = step * static_cast<uint32_t>(lane);
+        const uint32_t key = off < hi - lo ? lo + off : hi;
+        const uint64_t stays = __ballot(key == top || w.ratio(key) >= floor_w);
+        const int at = stays ? __builtin_ctzll(stays) : 64;  // 64: between the last candidate and hi
+        if (stays) hi = __shfl(key, at);
+        if (at > 0) lo = __shfl(key, at - 1) + 1;
+      }
+    else
+      hi = 1;
+    if (lane == 0) sh.floor_key = hi;
+  }
+  __syncthreads();
+  const uint32_t floor_key = sh.floor_key;
+  const int share_band = sh.border;  // kBands: top-p takes all
+  const int floor_band = floor_key > 1 ? band_of(key_value(floor_key), top_value, scale) : kBands;
+  const int border = cut ? share_band : min(share_band, floor_band);
+  const auto draw_from = [&](uint64_t total) {
+    const double aim = static_cast<double>(uniform) * static_cast<double>(total);
+    const uint64_t beyond =
+        aim >= 0.0 ? (aim < static_cast<double>(total) ? static_cast<uint64_t>(aim) : total - 1) : 0;
+    return min(beyond, total - 1);
+  };
+  const auto answer = [&](int index, uint64_t weight, uint64_t total) {
+    a.token[row] = static_cast<uint32_t>(index);
+    if (a.probability) a.probability[row] = static_cast<float>(static_cast<double>(weight) / static_cast<double>(total));
+  };
+
+  // do the lists reach through the border band?
+  bool reach = border < kBands && sh.count[min(border, kBands - 1)] <= kSorted;
+  if (reach)
+    for (int c = tid; c < p.chunks; c += kThreads) {
+      const ChunkHead h = heads[c];
+      if (!h.key) continue;
+      const int base = band_of(key_value(h.key), top_value, scale);
+      reach = reach && (border == kBands - 1 ? h.through == kBands : border - base < h.through);
+    }
+  if (__syncthreads_and(reach)) {
+    for (int c = wave; c < p.chunks; c += kThreads / 64) {
+      const ChunkHead h = heads[c];
+      if (!h.key || band_of(key_value(h.key), top_value, scale) > border) continue;
+      const uint64_t* list = p.lists + (unit0 + c) * p.list;
+      for (int base = 0; base < h.listed; base += 64) {
+        const uint64_t item = base + lane < h.listed ? list[base + lane] : 0;
+        append(item && band_of(key_value(item_key(item)), top_value, scale) <= border, item, sh.items, &sh.n, kSorted);
+      }
+    }
+    __syncthreads();
+    const int listed = min(static_cast<int>(sh.n), kSorted);
+    sort_down(sh.items, listed);
+    // rank 2 tid and 2 tid + 1
+    const int held = cut ? min(listed, k) : listed;
+    uint64_t mine[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < held ? w.fixed(item_key(sh.items[2 * tid + i])) : 0;
+    uint64_t all;
+    const uint64_t before = group_prefix(mine[0] + mine[1], all, sh);
+    const uint64_t target = share < 1.0 ? target_of(cut ? all : sh.total) : ~uint64_t{0};
+    uint32_t stay = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rank = 2 * tid + i;
+      const bool kept = rank < held && (rank == 0 || (before + (i ? mine[0] : 0) < target && item_key(sh.items[rank]) >= floor_key));
+      if (!kept) mine[i] = 0;
+      stay += kept;
+    }
+    uint64_t total, count;
+    group_prefix(mine[0] + mine[1], total, sh);
+    group_prefix(stay, count, sh);  // the kept ones are the first ranks
+    // in the order of the vocabulary
+    const int kept = static_cast<int>(count);
+    uint64_t* order = sh.items + kSorted;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rank = 2 * tid + i;
+      sh.bins[rank] = mine[i];
+      if (rank < kept) order[rank] = ~(static_cast<uint64_t>(item_index(sh.items[rank])) << 11 | static_cast<uint64_t>(rank));
+    }
+    __syncthreads();
+    sort_down(order, kept);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < kept ? sh.bins[~order[2 * tid + i] & (kSorted - 1)] : 0;
+    const uint64_t run = group_prefix(mine[0] + mine[1], all, sh);
+    const uint64_t beyond = draw_from(total);
+    if (run <= beyond && run + mine[0] + mine[1] > beyond) {
+      const int i = run + mine[0] > beyond ? 0 : 1;
+      answer(static_cast<int>(~order[2 * tid + i] >> 11), mine[i], total);
+    }
+    return;
+  }
+
   uint32_t least = 1;
   int last = n;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && k < n) {
+  const int in_border = border < kBands ? sh.count[border] - (border > 0 ? sh.count[border - 1] : 0) : 0;
+  if (!cut && in_border <= kItems) {
+    bool done = true;
+    int items = 0;
+    if (border < kBands) {
+      gather_band(x, n, border, top_value, scale, sh);
+      items = min(static_cast<int>(sh.n), kItems);
+      __syncthreads();
+      if (border == share_band) {
+        // top-p's border: which of kBins even parts of the band's keys, then the rank in it
+        const uint32_t low = sh.low, high = sh.high;
+        int step = 0;
+        while ((high - low) >> step >= static_cast<uint32_t>(kBins)) ++step;
+        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+        if (tid == 0) sh.n = 0, sh.found[0] = ~uint64_t{0};
+        __syncthreads();
+        for (int i = tid; i < items; i += kThreads) {
+          const uint32_t key = item_key(sh.items[i]);
+          const uint64_t f = w.fixed(key);
+          if (f) lds_add(&sh.bins[(high - key) >> step], f);
+        }
+        __syncthreads();
+        const uint64_t target = target_of(sh.total) - sh.above;
+        const uint64_t b0 = sh.bins[2 * tid], b1 = sh.bins[2 * tid + 1];
+        uint64_t all;
+        const uint64_t before = group_prefix(b0 + b1, all, sh);
+        if (before < target && before + b0 + b1 >= target) {
+          const bool second = before + b0 < target;
+          sh.found[0] = static_cast<uint64_t>(2 * tid + second);
+          sh.found[1] = second ? before + b0 : before;
+        }
+        __syncthreads();
+        const bool met = sh.found[0] != ~uint64_t{0};  // else (a rounding short of the band's sum): its last item
+        const uint32_t part = met ? static_cast<uint32_t>(sh.found[0]) : (high - low) >> step;
+        const uint64_t ahead = met ? sh.found[1] : all;
+        for (int base = 0; base < items; base += kThreads) {
+          const int i = base + tid;
+          const bool in = i < items && (high - item_key(sh.items[i])) >> step == part;
+          append(in, i < items ? sh.items[i] : 0, sh.sums, &sh.n, kSorted);
+        }
+        __syncthreads();
+        const int listed = static_cast<int>(sh.n);
+        done = listed <= kSorted;
+        if (done) {
+          sort_down(sh.sums, listed);
+          uint64_t mine[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < listed ? w.fixed(item_key(sh.sums[2 * tid + i])) : 0;
+          const uint64_t run = ahead + group_prefix(mine[0] + mine[1], all, sh);
+          if (tid == 0) sh.found[2] = static_cast<uint64_t>(listed - 1);
+          __syncthreads();
+          if (run < target && run + mine[0] + mine[1] >= target) sh.found[2] = static_cast<uint64_t>(2 * tid + (run + mine[0] < target));
+          __syncthreads();
+          const uint64_t item = sh.sums[sh.found[2]];
+          least = item_key(item);
+          last = item_index(item);
+          __syncthreads();
+        }
+      }
+    }
+    if (done) {
+      for (int c = tid; c < p.chunks; c += kThreads) sh.sums[c] = 0;
+      __syncthreads();
+      const auto kept = [&](uint32_t key, int i) {
+        return (key > least || (key == least && i <= last)) && key >= floor_key ? w.fixed(key) : 0;
+      };
+      // the kept sum of each chunk: its bands above the border, and its part of that
+      for (int u = tid; u < p.chunks * (kBands / 8); u += kThreads) {
+        const int c = u / (kBands / 8), j0 = u % (kBands / 8) * 8;
+        const ChunkHead h = heads[c];
+        if (!h.key) continue;
+        const int base = band_of(key_value(h.key), top_value, scale) + j0;
+        uint64_t sums[8], sum = 0;
+        chunk_sums(h, (unit0 + c) * kBands + j0, sums);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (min(base + j, kBands - 1) < border) sum += sums[j];
+        if (sum) lds_add(&sh.sums[c], sum);
+      }
+      for (int i = tid; i < items; i += kThreads) {
+        const uint64_t item = sh.items[i];
+        const uint64_t f = kept(item_key(item), item_index(item));
+        if (f) lds_add(&sh.sums[item_index(item) / p.chunk], f);
+      }
+      __syncthreads();
+      // the chunk where the running sum passes the draw (two a thread), then the place in it
+      const uint64_t s0 = 2 * tid < p.chunks ? sh.sums[2 * tid] : 0, s1 = 2 * tid + 1 < p.chunks ? sh.sums[2 * tid + 1] : 0;
+      uint64_t total;
+      uint64_t run = group_prefix(s0 + s1, total, sh);
+      uint64_t beyond = draw_from(total);
+      if (run <= beyond && run + s0 + s1 > beyond) {
+        const bool second = run + s0 <= beyond;
+        sh.found[0] = static_cast<uint64_t>(2 * tid + second);
+        sh.found[1] = second ? run + s0 : run;
+      }
+      if (tid == 0) sh.found[2] = 0;
+      __syncthreads();
+      const int per = p.chunk / kThreads, at = static_cast<int>(sh.found[0]) * p.chunk + tid * per;
+      beyond -= sh.found[1];
+      uint64_t mine[kItems / kThreads], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kItems / kThreads; ++i) {
+        mine[i] = i < per && at + i < n ? kept(rank_key(x[at + i]), at + i) : 0;
+        sum += mine[i];
+      }
+      uint64_t all;
+      run = group_prefix(sum, all, sh);
+      // a chunk weighed by its own maximum may add up to a rounding less here:
+      // then its last kept token (its largest, if all weights round to nothing)
+      if (all == 0) {
+        if (tid == 0) answer(static_cast<int>(heads[sh.found[0]].index), 0, total);
+        return;
+      }
+      if (beyond >= all) beyond = all - 1;
+      if (run <= beyond && run + sum > beyond) {
+        int i = 0;
+#pragma unroll
+        for (int j = 0; j < kItems / kThreads; ++j)
+          if (run <= beyond) {
+            run += mine[j];
+            i = j;
+          }
+        answer(at + i, kept(rank_key(x[at + i]), at + i), total);
+      }
+      return;
+    }
+  }
+
+  // digit by digit
+  // kept: keys above `least`, and of those equal to it the ones up to index
+  // `last`
+  if (cut) {
     uint64_t mine = 0, above;
     for (int i = threadIdx.x; i < n; i += kThreads) mine += rank_key(x[i]) != 0;
     if (group_sum(mine, sh) > static_cast<uint64_t>(k)) {
@@ -189,13 +758,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
   const auto weigh = [&](uint32_t key, int i) {
     return key > least || (key == least && i <= last) ? w.fixed(key) : 0;
   };
-  const double p = a.top_p ? static_cast<double>(a.top_p[row]) : 1.0;
-  if (p < 1.0) {
+  if (share < 1.0) {
     uint64_t mine = 0, above;
     for (int i = threadIdx.x; i < n; i += kThreads) mine += weigh(rank_key(x[i]), i);
     const uint64_t total = group_sum(mine, sh);
-    const double goal = ceil(p * static_cast<double>(total));
-    const uint64_t target = goal < 1.0 ? 1 : min(total, static_cast<uint64_t>(goal));
+    const uint64_t target = target_of(total);
     // equal keys beyond `last` weigh more than their share here; the search
     // then ends at `least` itself, and the count below is cut to `last`
     const uint32_t key = descend(x, n, target, [&](uint32_t q) { return q >= least ? w.fixed(q) : 0; }, above, sh);
@@ -208,32 +775,60 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs a, in
       last = min(last, upto);
     }
   }
-  const double floor_w = a.min_p ? static_cast<double>(a.min_p[row]) : 0.0;
   const auto kept = [&](uint32_t key, int i) -> uint64_t {
     if (key < least || (key == least && i > last)) return 0;
-    return key == top || w.ratio(key) >= floor_w ? w.fixed(key) : 0;
+    return key >= floor_key ? w.fixed(key) : 0;
   };
   uint64_t mine = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) mine += kept(rank_key(x[i]), i);
   const uint64_t total = group_sum(mine, sh);
-  const double aim = static_cast<double>(a.uniform[row]) * static_cast<double>(total);
-  const uint64_t beyond = aim >= 0.0 ? (aim < static_cast<double>(total) ? static_cast<uint64_t>(aim) : total - 1) : 0;
-  const int index = walk(x, n, min(beyond, total - 1), kept, sh);
-  if (threadIdx.x == 0) {
-    a.token[row] = static_cast<uint32_t>(index);
-    if (a.probability) a.probability[row] = static_cast<float>(static_cast<double>(kept(rank_key(x[index]), index)) / static_cast<double>(total));
-  }
+  const int index = walk(x, n, draw_from(total), kept, sh);
+  if (tid == 0) answer(index, kept(rank_key(x[index]), index), total);
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Small problems in chunks of 2048 (one row of 151936: 75 workgroups instead
+// of 19), large ones of 8192 (fewer bands and lists to write and add).
+SamplePlan plan_sample(int64_t rows, int64_t vocabulary, void* workspace) {
+  SamplePlan p{};
+  const bool fine = rows * up(vocabulary, 8192) < 512 && vocabulary <= 2048 * kMostChunks;
+  p.chunk = fine ? 2048 : 8192;
+  p.chunks = static_cast<int32_t>(up(vocabulary, p.chunk));
+  p.list = static_cast<int32_t>(vocabulary < kList ? vocabulary : kList);
+  p.shift = 62;
+  while ((int64_t{1} << (62 - p.shift)) < vocabulary) --p.shift;
+  const size_t units = static_cast<size_t>(rows) * p.chunks;
+  char* at = static_cast<char*>(workspace);
+  size_t bytes = 0;
+  const auto take = [&](size_t size) {
+    char* part = at ? at + bytes : nullptr;
+    bytes += (size + 255) & ~size_t{255};
+    return part;
+  };
+  p.heads = reinterpret_cast<ChunkHead*>(take(units * sizeof(ChunkHead)));
+  p.counts = reinterpret_cast<uint16_t*>(take(units * kBands * sizeof(uint16_t)));
+  p.weights = reinterpret_cast<uint64_t*>(take(units * kBands * sizeof(uint64_t)));
+  p.lists = reinterpret_cast<uint64_t*>(take(units * p.list * sizeof(uint64_t)));
+  p.bytes = bytes;
+  return p;
 }
 
 }  // namespace
 
-size_t sample_workspace(int64_t, int64_t) { return 0; }
+size_t sample_workspace(int64_t rows, int64_t vocabulary) { return rows == 0 ? 0 : plan_sample(rows, vocabulary, nullptr).bytes; }
 
-hipError_t launch_sample(const SampleArgs& a, void*, hipStream_t stream) {
-  int shift = 62;
-  while ((int64_t{1} << (62 - shift)) < a.vocabulary) --shift;
-  sample_kernel<<<a.rows, kThreads, 0, stream>>>(a, shift);
-  note("sample_kernel", a.rows);
+hipError_t launch_sample(const SampleArgs& a, void* workspace, hipStream_t stream) {
+  const SamplePlan p = plan_sample(a.rows, a.vocabulary, workspace);
+  const dim3 grid(static_cast<uint32_t>(p.chunks), static_cast<uint32_t>(a.rows));
+  if (p.chunk == 2048)
+    sample_scan_kernel<2><<<grid, kScanThreads, 0, stream>>>(a, p);
+  else
+    sample_scan_kernel<8><<<grid, kScanThreads, 0, stream>>>(a, p);
+  const hipError_t error = hipGetLastError();
+  if (error != hipSuccess) return error;
+  sample_draw_kernel<<<a.rows, kThreads, 0, stream>>>(a, p);
+  note("sample_scan_kernel", static_cast<int64_t>(p.chunks) * a.rows, p.chunk);
   return hipGetLastError();
 }
 
