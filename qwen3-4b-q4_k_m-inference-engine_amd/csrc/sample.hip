@@ -20,7 +20,7 @@
 // Values are ranked by a 32-bit key whose unsigned order is the order of the
 // logits (NaN and -inf: 0, never drawn). Weights are fixed-point integers,
 // rint(exp((z - max) / T) * 2^shift) of a 64-bit exponential with 2^shift *
-// vocabulary < 2^62, so their sums are exact and no order of additions can
+// vocabulary <= 2^62 and shift <= 44, so their sums are exact and no order of additions can
 // change a result; a chunk whose own maximum is not the row's is weighed by
 // its own and scaled once per band, in 64-bit floating point. Bands only say
 // where to look; no result depends on their width.
@@ -39,6 +39,9 @@ constexpr int kList = 512;         // most listed logits of a chunk
 constexpr int kItems = 8192;       // most logits of a band that the draw holds
 constexpr int kSorted = 2 * kThreads;
 constexpr int kMostChunks = 2048;
+constexpr int kShift = 44;         // most fraction bits of a weight
+constexpr int kCopies = 16;        // of the scan's bands: a wave's lanes with the same two low bits share one
+constexpr int kCountAt = 54;       // a band's count above its sum: 512 logits of 2^44 stay below 2^54
 constexpr int kFew = 128;          // listed logits of a chunk without top-k
 
 // What the scan leaves of a chunk.
@@ -64,16 +67,46 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __builtin_bit_cast(float, (key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
 }
 
+// 2^t for t <= 0, to about 2^-50 of itself; nothing below 2^-128: the power
+// series of e^(f ln 2) up to f^12 over |f| <= 1/2, a third of the instructions
+// of a correctly scaled 64-bit exponential.
+__device__ __forceinline__ double exp2_part(double t) {
+  t = fmax(t, -128.0);  // NaN too
+  const double n = rint(t), f = t - n;
+  constexpr double c[13] = {1.0,
+                            0.69314718055994531,
+                            0.24022650695910072,
+                            0.055504108664821580,
+                            0.0096181291076284772,
+                            0.0013333558146428443,
+                            0.00015403530393381610,
+                            0.000015252733804059841,
+                            0.0000013215486790144310,
+                            1.0178086009239699e-7,
+                            7.0549116208011234e-9,
+                            4.4455382718708114e-10,
+                            2.5678435993488206e-11};
+  double y = c[12];
+#pragma unroll
+  for (int i = 11; i >= 0; --i) y = __builtin_fma(y, f, c[i]);
+  return ldexp(y, static_cast<int>(n));
+}
+
 struct Weigher {
-  double max, inv_t, one;
-  __device__ __forceinline__ double ratio(uint32_t key) const {
-    const double z = key_value(key);
-    return z == max ? 1.0 : exp((z - max) * inv_t);
+  double max, rate, one;  // rate: log2(e) / T
+  __device__ __forceinline__ double ratio_of(float z) const {
+    return exp2_part(z == max ? 0.0 : (static_cast<double>(z) - max) * rate);
   }
-  __device__ __forceinline__ uint64_t fixed(uint32_t key) const {
-    return key == 0 ? 0 : static_cast<uint64_t>(rint(ratio(key) * one));
+  __device__ __forceinline__ double ratio(uint32_t key) const { return ratio_of(key_value(key)); }
+  // The sum's low 52 bits are the product, at most 2^44, rounded to an integer.
+  __device__ __forceinline__ uint64_t fixed_of(float z) const {
+    return __builtin_bit_cast(uint64_t, __builtin_fma(ratio_of(z), one, 0x1p52)) & 0xFFFFFFFFFFFFFull;
   }
+  __device__ __forceinline__ uint64_t fixed(uint32_t key) const { return key == 0 ? 0 : fixed_of(key_value(key)); }
 };
+__device__ __forceinline__ Weigher weigher(uint32_t top, float heat, int shift) {
+  return Weigher{static_cast<double>(key_value(top)), 1.4426950408889634 / heat, static_cast<double>(uint64_t{1} << shift)};
+}
 
 // The band of v below top (v <= top, both above -inf). The same for a chunk's
 // maximum against the row's, so that bands of chunks add up: values times
@@ -114,13 +147,13 @@ __device__ __forceinline__ void append(bool mine, uint64_t item, uint64_t* items
 
 // The scan. HBM bounds it: 200 rows of 151936 logits, 121 MB. A thread's
 // logits are all loaded before any is looked at (16 bytes x E in flight a
-// lane); band counts are spread over four copies by lane, as neighbouring
-// logits often share a band.
+// lane). Band counts are spread over copies, as neighbouring logits often
+// share a band; with weights, count and sum are one 64-bit addition.
 template <int E>
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleArgs a, const SamplePlan p) {
-  __shared__ uint64_t weight[kBands * 4];
-  __shared__ uint32_t count[kBands * 4];
-  __shared__ float tops[kScanThreads / 64];
+  static_assert(E <= 8 && kScanThreads / 64 * 4 == kCopies && 16 * E * 4 <= 512);
+  __shared__ uint64_t bands[kBands * kCopies];
+  __shared__ float tops[kScanThreads / 64], groups[kScanThreads];
   __shared__ uint32_t first, listed;
   __shared__ int32_t depth;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
@@ -128,22 +161,36 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
   const int n = min(a.vocabulary - lo, p.chunk);
   const int64_t unit = static_cast<int64_t>(row) * p.chunks + blockIdx.x;
   const float* x = a.logits + row * a.row_stride + lo;
+  const int at0 = tid * 4;  // element e of load i is logit lo + at0 + i * 4 * kScanThreads + e
   f32x4 v[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = load_logits(x, (i * kScanThreads + tid) * 4, n);
+  for (int i = 0; i < E; ++i) v[i] = load_logits(x, at0 + i * 4 * kScanThreads, n);
   const float heat = a.temperature[row];
   const int k = a.top_k ? a.top_k[row] : 0;
+  const bool greedy = !(heat > 0.0f);
   const bool cut = k > 0 && k < a.vocabulary;  // the kept set is bounded: no sums of bands are needed
-  for (int i = tid; i < kBands * 4; i += kScanThreads) {
-    count[i] = 0;
-    if (!cut) weight[i] = 0;
+  const bool bounded = cut && k <= kScanThreads && !greedy;
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(bands);  // of a cut row: [band][4]
+  if (cut) {
+    for (int i = tid; i < kBands * 2; i += kScanThreads) bands[i] = 0;
+  } else if (!greedy) {
+    for (int i = tid; i < kBands * kCopies; i += kScanThreads) bands[i] = 0;
   }
   if (tid == 0) first = 0xFFFFFFFFu, listed = 0;
-  float top = -__builtin_inff();
+  float mine = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < E; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);  // NaN: the other operand
+    for (int e = 0; e < 4; ++e) mine = fmaxf(mine, v[i][e]);  // NaN: the other operand
+  if (bounded) {
+    float group = mine;
+    if (k <= kScanThreads / 4) {
+      group = fmaxf(group, __shfl_xor(group, 1));
+      group = fmaxf(group, __shfl_xor(group, 2));
+    }
+    groups[tid] = group;
+  }
+  float top = mine;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   if (lane == 0) tops[wave] = top;
@@ -155,34 +202,94 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
     return;
   }
   const uint32_t top_key = rank_key(top);
-  const bool greedy = !(heat > 0.0f);
-  const float scale = band_scale(heat);
-  const Weigher w{static_cast<double>(key_value(top_key)), 1.0 / heat, static_cast<double>(uint64_t{1} << p.shift)};
-  uint32_t mine = 0xFFFFFFFFu;
+  if (mine == top) {
+    uint32_t at = 0xFFFFFFFFu;
 #pragma unroll
-  for (int i = 0; i < E; ++i)
+    for (int i = E - 1; i >= 0; --i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float z = v[i][e];
-      if (z == top) mine = min(mine, static_cast<uint32_t>(lo + (i * kScanThreads + tid) * 4 + e));
-      if (!greedy && z > -__builtin_inff()) {
-        const int at = band_of(z, top, scale) * 4 + (lane & 3);
-        atomicAdd(&count[at], 1u);
-        if (!cut) lds_add(&weight[at], w.fixed(rank_key(z)));
-      }
-    }
-  if (mine != 0xFFFFFFFFu) atomicMin(&first, mine);
-  __syncthreads();
+      for (int e = 3; e >= 0; --e)
+        if (v[i][e] == top) at = static_cast<uint32_t>(lo + at0 + i * 4 * kScanThreads + e);
+    atomicMin(&first, at);
+  }
   if (greedy) {
+    __syncthreads();
     if (tid == 0) p.heads[unit] = ChunkHead{top_key, first, 0, 0};
     return;
   }
+  const float scale = band_scale(heat);
+  // the lane's logits to count or to list: bit 4 i + e
+  uint32_t some = 0;
+  const auto each = [&](auto visit) {  // few: read again, not picked from registers
+    for (uint32_t left = some; __any(left != 0); left &= left - 1) {
+      const int bit = left ? __builtin_ctz(left) : 0, at = at0 + (bit >> 2) * 4 * kScanThreads + (bit & 3);
+      visit(left != 0, left ? x[at] : 0.0f, at);
+    }
+  };
+  if (bounded) {
+    // The k-th largest of the maxima of k groups or more has k logits of the
+    // chunk at or above it: what is below it is in no row's top-k and need not
+    // be looked at. Its upper 18 bits, by bisection: groups of four lanes
+    // (k <= 64) leave little more than k logits, single lanes a few times k.
+    const bool quads = k <= kScanThreads / 4;
+    uint32_t key[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) key[j] = quads ? (j ? 0 : rank_key(groups[4 * lane])) : rank_key(groups[64 * j + lane]);
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 14; --bit) {
+      const uint32_t candidate = least | 1u << bit;
+      int reach = __popcll(__ballot(key[0] >= candidate));
+      if (!quads) {
+#pragma unroll
+        for (int j = 1; j < 4; ++j) reach += __popcll(__ballot(key[j] >= candidate));
+      }
+      if (reach >= k) least = candidate;
+    }
+    const float bound = least >= rank_key(-3.4028234e38f) ? key_value(least) : -3.4028234e38f;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) some |= v[i][e] >= bound ? 1u << (4 * i + e) : 0u;
+    each([&](bool in, float z, int) {
+      if (in) atomicAdd(&counts[band_of(z, top, scale) * 4 + (lane & 3)], 1u);
+    });
+  } else if (cut) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (v[i][e] > -__builtin_inff()) atomicAdd(&counts[band_of(v[i][e], top, scale) * 4 + (lane & 3)], 1u);
+  } else {
+    const Weigher w = weigher(top_key, heat, p.shift);
+    const int copy = wave * 4 + (lane & 3);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = v[i][e];
+        if (z > -__builtin_inff())
+          lds_add(&bands[band_of(z, top, scale) * kCopies + copy], w.fixed_of(z) | uint64_t{1} << kCountAt);
+      }
+  }
+  __syncthreads();
   if (wave == 0) {  // lane: bands 2 lane and 2 lane + 1
     uint32_t c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t* q = count + (2 * lane + i) * 4;
-      c[i] = q[0] + q[1] + q[2] + q[3];
+      const int band = 2 * lane + i;
+      c[i] = 0;
+      if (cut) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[i] += counts[band * 4 + j];
+      } else {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const uint64_t both = bands[band * kCopies + ((j + lane) & (kCopies - 1))];  // lanes start at different banks
+          c[i] += static_cast<uint32_t>(both >> kCountAt);
+          sum += both & ((uint64_t{1} << kCountAt) - 1);
+        }
+        p.weights[unit * kBands + band] = sum;
+      }
     }
     reinterpret_cast<uint32_t*>(p.counts + unit * kBands)[lane] = c[0] | c[1] << 16;
     uint32_t run = c[0] + c[1];
@@ -201,24 +308,20 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
       depth = through;
       p.heads[unit] = ChunkHead{top_key, first, static_cast<int32_t>(held), through};
     }
-  } else if (!cut && wave == 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint64_t* q = weight + (2 * lane + i) * 4;
-      p.weights[unit * kBands + 2 * lane + i] = q[0] + q[1] + q[2] + q[3];
-    }
   }
   __syncthreads();
   const int through = depth;
+  if (!bounded) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        some |= v[i][e] > -__builtin_inff() && band_of(v[i][e], top, scale) < through ? 1u << (4 * i + e) : 0u;
+  }
   uint64_t* list = p.lists + unit * p.list;
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float z = v[i][e];
-      append(z > -__builtin_inff() && band_of(z, top, scale) < through,
-             item_of(rank_key(z), lo + (i * kScanThreads + tid) * 4 + e), list, &listed, p.list);
-    }
+  each([&](bool in, float z, int at) {
+    append(in && band_of(z, top, scale) < through, item_of(rank_key(z), lo + at), list, &listed, p.list);
+  });
 }
 
 struct Shared {
@@ -227,10 +330,14 @@ struct Shared {
   uint64_t sums[kMostChunks];
   uint64_t weight[kBands];
   uint32_t count[kBands];  // later its running sums
+  // of each chunk: where its bands lie in the row's (kBands: it has none), and
+  // its head's `through` and `listed`
+  uint8_t base[kMostChunks], through[kMostChunks];
+  uint16_t listed[kMostChunks], active[kMostChunks];
   uint64_t wave[16];
   uint64_t found[3];
   uint64_t above, total;
-  uint32_t border, floor_key, n, low, high;
+  uint32_t border, floor_key, n, actives, low, high;
 };
 
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
@@ -332,6 +439,12 @@ __device__ int walk(const float* x, int n, uint64_t beyond, F measure, Shared& s
   return static_cast<int>(sh.found[0]);
 }
 
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
 // Exclusive running sum of v over the workgroup, and the sum of all.
 __device__ uint64_t group_prefix(uint64_t v, uint64_t& all, Shared& sh) {
   const int lane = static_cast<int>(threadIdx.x & 63), wave = static_cast<int>(threadIdx.x >> 6);
@@ -387,26 +500,36 @@ __device__ void sort_down(uint64_t* items, int n) {
 // than fit are counted), with the largest and smallest key in sh.high / low.
 __device__ void gather_band(const float* x, int n, int band, float top, float scale, Shared& sh) {
   const float origin = floorf(top * scale), want = static_cast<float>(band);
+  // band_of decided for one band: one subtraction and a comparison where
+  // neither infinities nor NaN can be in it
+  const bool plain = band < kBands - 1 && fabsf(origin) < __builtin_inff();
   uint32_t low = 0xFFFFFFFFu, high = 0;
   constexpr int kAhead = 8;  // loads in flight a lane
-  for (int base = 0; base < n; base += 4 * kThreads * kAhead) {
+  for (int base = static_cast<int>(threadIdx.x) * 4; __any(base < n); base += 4 * kThreads * kAhead) {
     f32x4 v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = load_logits(x, base + (i * kThreads + static_cast<int>(threadIdx.x)) * 4, n);
+    for (int i = 0; i < kAhead; ++i) v[i] = load_logits(x, base + i * 4 * kThreads, n);
+    uint32_t hits = 0;
+    if (plain) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+      for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float z = v[i][e], d = origin - floorf(z * scale);  // band_of, decided for one band
-        const bool in = band == kBands - 1 ? !(d < want) : d == want;
-        const bool hit = z == top ? band == 0 : in && z > -__builtin_inff();
-        const uint32_t key = rank_key(z);
-        if (hit) {
-          low = min(low, key);
-          high = max(high, key);
-        }
-        append(hit, item_of(key, base + (i * kThreads + static_cast<int>(threadIdx.x)) * 4 + e), sh.items, &sh.n, kItems);
-      }
+        for (int e = 0; e < 4; ++e) hits |= origin - floorf(v[i][e] * scale) == want ? 1u << (4 * i + e) : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          hits |= v[i][e] > -__builtin_inff() && band_of(v[i][e], top, scale) == band ? 1u << (4 * i + e) : 0u;
+    }
+    uint32_t at = hits ? atomicAdd(&sh.n, static_cast<uint32_t>(__popc(hits))) : 0;
+    for (; hits; hits &= hits - 1, ++at) {  // few: read again, not picked from registers
+      const int bit = __builtin_ctz(hits), index = base + (bit >> 2) * 4 * kThreads + (bit & 3);
+      const uint32_t key = rank_key(x[index]);
+      low = min(low, key);
+      high = max(high, key);
+      if (at < kItems) sh.items[at] = item_of(key, index);
+    }
   }
   if (high) {
     atomicMin(&sh.low, low);
@@ -431,10 +554,16 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   const double floor_w = a.min_p ? static_cast<double>(a.min_p[row]) : 0.0;
   const float uniform = a.uniform[row];
   if (tid < kBands) sh.count[tid] = 0, sh.weight[tid] = 0;
-  if (tid == 0) sh.n = 0, sh.low = 0xFFFFFFFFu, sh.high = 0;
+  if (tid == 0) sh.n = 0, sh.actives = 0, sh.low = 0xFFFFFFFFu, sh.high = 0;
+  // the first of the chunks' counts are on their way before the row's maximum is known
+  const int units = p.chunks * (kBands / 8);
+  u16x8 counts{};
+  if (tid < units) counts = *reinterpret_cast<const u16x8*>(p.counts + unit0 * kBands + 8 * tid);
   uint64_t best = 0;
   for (int c = tid; c < p.chunks; c += kThreads) {
     const ChunkHead h = heads[c];
+    sh.through[c] = static_cast<uint8_t>(h.through);
+    sh.listed[c] = static_cast<uint16_t>(h.listed);
     const uint64_t item = h.key ? item_of(h.key, static_cast<int>(h.index)) : 0;
     best = item > best ? item : best;
   }
@@ -455,33 +584,38 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   }
   const uint32_t top = item_key(best);
   const float top_value = key_value(top), scale = band_scale(heat);
-  const Weigher w{static_cast<double>(top_value), 1.0 / heat, static_cast<double>(uint64_t{1} << p.shift)};
+  const Weigher w = weigher(top, heat, p.shift);
 
-  // the row's bands: those of chunk c are base(c) further down. A unit is
-  // eight bands of a chunk; sum(weights) is their part of them.
-  const auto chunk_sums = [&](const ChunkHead& h, int64_t at, uint64_t (&out)[8]) {
+  for (int c = tid; c < p.chunks; c += kThreads) {
+    const uint32_t key = heads[c].key;
+    sh.base[c] = static_cast<uint8_t>(key ? band_of(key_value(key), top_value, scale) : kBands);
+  }
+  __syncthreads();
+  // the row's bands: those of chunk c are base[c] further down. A unit is
+  // eight bands of a chunk.
+  const auto chunk_sums = [&](int c, int64_t at, uint64_t (&out)[8]) {
     const uint64_t* q = p.weights + at;
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = q[j];
-    if (h.key != top) {
-      const double factor = w.ratio(h.key);
+    const uint32_t key = heads[c].key;
+    if (key != top) {
+      const double factor = w.ratio(key);
 #pragma unroll
       for (int j = 0; j < 8; ++j) out[j] = static_cast<uint64_t>(rint(static_cast<double>(out[j]) * factor));
     }
   };
-  for (int u = tid; u < p.chunks * (kBands / 8); u += kThreads) {
+  for (int u = tid; u < units; u += kThreads) {
     const int c = u / (kBands / 8), j0 = u % (kBands / 8) * 8;
-    const ChunkHead h = heads[c];
-    if (!h.key) continue;
-    const int base = band_of(key_value(h.key), top_value, scale) + j0;
+    if (sh.base[c] == kBands) continue;
+    const int base = sh.base[c] + j0;
     const int64_t at = (unit0 + c) * kBands + j0;
-    const u16x8 counts = *reinterpret_cast<const u16x8*>(p.counts + at);
+    if (u != tid) counts = *reinterpret_cast<const u16x8*>(p.counts + at);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (counts[j]) atomicAdd(&sh.count[min(base + j, kBands - 1)], static_cast<uint32_t>(counts[j]));
     if (!cut) {
       uint64_t sums[8];
-      chunk_sums(h, at, sums);
+      chunk_sums(c, at, sums);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (sums[j]) lds_add(&sh.weight[min(base + j, kBands - 1)], sums[j]);
@@ -555,53 +689,85 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   bool reach = border < kBands && sh.count[min(border, kBands - 1)] <= kSorted;
   if (reach)
     for (int c = tid; c < p.chunks; c += kThreads) {
-      const ChunkHead h = heads[c];
-      if (!h.key) continue;
-      const int base = band_of(key_value(h.key), top_value, scale);
-      reach = reach && (border == kBands - 1 ? h.through == kBands : border - base < h.through);
+      if (sh.base[c] > border) continue;
+      reach = reach && (border == kBands - 1 ? sh.through[c] == kBands : border - sh.base[c] < sh.through[c]);
+      sh.active[atomicAdd(&sh.actives, 1u)] = static_cast<uint16_t>(c);
     }
   if (__syncthreads_and(reach)) {
-    for (int c = wave; c < p.chunks; c += kThreads / 64) {
-      const ChunkHead h = heads[c];
-      if (!h.key || band_of(key_value(h.key), top_value, scale) > border) continue;
+    // 32 lanes a chunk
+    const int actives = static_cast<int>(sh.actives);
+    for (int i = tid >> 5; __any(i < actives); i += kThreads / 32) {
+      const int c = i < actives ? sh.active[i] : 0, listed = i < actives ? sh.listed[c] : 0;
       const uint64_t* list = p.lists + (unit0 + c) * p.list;
-      for (int base = 0; base < h.listed; base += 64) {
-        const uint64_t item = base + lane < h.listed ? list[base + lane] : 0;
+      for (int at = lane & 31; __any(at < listed); at += 32) {
+        const uint64_t item = at < listed ? list[at] : 0;
         append(item && band_of(key_value(item_key(item)), top_value, scale) <= border, item, sh.items, &sh.n, kSorted);
       }
     }
     __syncthreads();
     const int listed = min(static_cast<int>(sh.n), kSorted);
-    sort_down(sh.items, listed);
-    // rank 2 tid and 2 tid + 1
     const int held = cut ? min(listed, k) : listed;
+    if (listed <= 64) {
+      // one wave, an item a lane; what ranks before it and what precedes it in
+      // the vocabulary are sums over the others' values, lane by lane
+      if (wave != 0) return;
+      const uint64_t item = lane < listed ? sh.items[lane] : 0;
+      const uint64_t f = lane < listed ? w.fixed(item_key(item)) : 0;
+      uint64_t before = 0;
+      int rank = 0;
+      for (int i = 0; i < listed; ++i) {
+        const bool ahead = lane_value(item, i) > item;
+        before += ahead ? lane_value(f, i) : 0;
+        rank += ahead;
+      }
+      uint64_t all = lane < listed && rank == held - 1 ? before + f : 0;
+      all = lane_value(all, __builtin_ctzll(__ballot(lane < listed && rank == held - 1)));
+      const uint64_t target = share < 1.0 ? target_of(cut ? all : sh.total) : ~uint64_t{0};
+      const bool kept = lane < listed && rank < held && (rank == 0 || (before < target && item_key(item) >= floor_key));
+      const uint64_t mine = kept ? f : 0;
+      uint64_t total = 0, run = 0;  // run: of the kept up to the lane's
+      for (int i = 0; i < listed; ++i) {
+        const uint64_t other = lane_value(mine, i);
+        total += other;
+        run += item_index(lane_value(item, i)) <= item_index(item) ? other : 0;
+      }
+      const uint64_t beyond = draw_from(total);
+      if (mine && run > beyond && run - mine <= beyond) answer(item_index(item), mine, total);
+      return;
+    }
+    sort_down(sh.items, listed);
+    // ranks 2 tid and 2 tid + 1
     uint64_t mine[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < held ? w.fixed(item_key(sh.items[2 * tid + i])) : 0;
+    if (tid == 0) sh.found[0] = sh.found[1] = 0;
     uint64_t all;
     const uint64_t before = group_prefix(mine[0] + mine[1], all, sh);
     const uint64_t target = share < 1.0 ? target_of(cut ? all : sh.total) : ~uint64_t{0};
-    uint32_t stay = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int rank = 2 * tid + i;
-      const bool kept = rank < held && (rank == 0 || (before + (i ? mine[0] : 0) < target && item_key(sh.items[rank]) >= floor_key));
-      if (!kept) mine[i] = 0;
-      stay += kept;
+    // the kept ones are the first ranks
+    const auto stays = [&](int rank, uint64_t ahead) {
+      return rank < held && (rank == 0 || (ahead < target && item_key(sh.items[rank]) >= floor_key));
+    };
+    const bool stay0 = stays(2 * tid, before), stay1 = stays(2 * tid + 1, before + mine[0]);
+    if (!stay0) mine[0] = 0;
+    if (!stay1) mine[1] = 0;
+    const uint64_t some = __ballot(stay0);
+    if (some && lane == 63 - __builtin_clzll(some)) {
+      atomicMax(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(2 * tid + 1 + stay1));
+      atomicMax(reinterpret_cast<unsigned long long*>(&sh.found[1]),
+                static_cast<unsigned long long>(before + mine[0] + mine[1]));
     }
-    uint64_t total, count;
-    group_prefix(mine[0] + mine[1], total, sh);
-    group_prefix(stay, count, sh);  // the kept ones are the first ranks
     // in the order of the vocabulary
-    const int kept = static_cast<int>(count);
     uint64_t* order = sh.items + kSorted;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int rank = 2 * tid + i;
       sh.bins[rank] = mine[i];
-      if (rank < kept) order[rank] = ~(static_cast<uint64_t>(item_index(sh.items[rank])) << 11 | static_cast<uint64_t>(rank));
+      if (i ? stay1 : stay0) order[rank] = ~(static_cast<uint64_t>(item_index(sh.items[rank])) << 11 | static_cast<uint64_t>(rank));
     }
     __syncthreads();
+    const int kept = static_cast<int>(sh.found[0]);
+    const uint64_t total = sh.found[1];
     sort_down(order, kept);
 #pragma unroll
     for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < kept ? sh.bins[~order[2 * tid + i] & (kSorted - 1)] : 0;
@@ -683,13 +849,12 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
         return (key > least || (key == least && i <= last)) && key >= floor_key ? w.fixed(key) : 0;
       };
       // the kept sum of each chunk: its bands above the border, and its part of that
-      for (int u = tid; u < p.chunks * (kBands / 8); u += kThreads) {
+      for (int u = tid; u < units; u += kThreads) {
         const int c = u / (kBands / 8), j0 = u % (kBands / 8) * 8;
-        const ChunkHead h = heads[c];
-        if (!h.key) continue;
-        const int base = band_of(key_value(h.key), top_value, scale) + j0;
+        if (sh.base[c] == kBands) continue;
+        const int base = sh.base[c] + j0;
         uint64_t sums[8], sum = 0;
-        chunk_sums(h, (unit0 + c) * kBands + j0, sums);
+        chunk_sums(c, (unit0 + c) * kBands + j0, sums);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (min(base + j, kBands - 1) < border) sum += sums[j];
@@ -796,7 +961,7 @@ SamplePlan plan_sample(int64_t rows, int64_t vocabulary, void* workspace) {
   p.chunk = fine ? 2048 : 8192;
   p.chunks = static_cast<int32_t>(up(vocabulary, p.chunk));
   p.list = static_cast<int32_t>(vocabulary < kList ? vocabulary : kList);
-  p.shift = 62;
+  p.shift = kShift;
   while ((int64_t{1} << (62 - p.shift)) < vocabulary) --p.shift;
   const size_t units = static_cast<size_t>(rows) * p.chunks;
   char* at = static_cast<char*>(workspace);

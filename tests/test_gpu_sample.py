@@ -93,6 +93,17 @@ def test_equal_logits_rank_by_index(gpu, V):
             Sample(gpu, x, 1.0, k, p, 0.0, u).run()
 
 
+def test_large_batches_of_equal_logits(gpu):
+    """Chunks whose logits all weigh 1, and rows of few distinct ones, in the layout of large batches."""
+    rng = np.random.default_rng(11)
+    x = np.full((110, 40001), 0.75, np.float32)
+    x[1::2] = rng.choice(np.float32([0.5, 0.25, -1.0]), (55, 40001))
+    x[::7, ::3] = -np.inf
+    for k, p, min_p in ((0, 1.0, 0.0), (0, 0.63, 0.0), (0, 1.0, 0.9), (3000, 0.71, 0.0)):
+        print(f"[case] sample equal logits k={k} p={p}", flush=True)
+        Sample(gpu, x, 1.0, k, p, min_p, 0.123 + 0.8 * rng.random(110)).run()
+
+
 def test_the_whole_line_of_uniforms(gpu):
     """Uniforms over [0, 1) draw every kept token, in index order."""
     V, R = 130, 400
