@@ -24,7 +24,7 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   if (tokens == 0 || sequences == 0) return p;
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   p.few = rows <= 32 * sequences;
-  const int tile_rows = p.few ? 16 : q_type == QK_TYPE_F32 ? 128 : 256;
+  const int tile_rows = p.few ? 16 : 32 * attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
   p.rows = tile_rows;
   // every sequence may end in a part of a tile, and none has a tile without a row
   int64_t tiles = rows / tile_rows + sequences;
@@ -33,7 +33,7 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   p.tiles = static_cast<int32_t>(tiles);
   int64_t keys = max_context < 1 ? 1 : max_context;
   if (window > 0 && keys > window + tile_rows) keys = window + tile_rows;
-  const int64_t want = p.few || q_type == QK_TYPE_F32 ? kMostUnits : kUnits;
+  const int64_t want = p.few ? kMostUnits : kUnits;
   const int64_t least = p.few ? 128 : 256;
   int64_t splits = up(want, tiles * kv_heads);
   if (splits > up(keys, least)) splits = up(keys, least);

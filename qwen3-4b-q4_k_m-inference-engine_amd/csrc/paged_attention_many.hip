@@ -1,12 +1,14 @@
 // Paged attention for many rows a sequence: prompts and chunks of prompts. The
 // matrix cores bound it.
 //
-// A workgroup's four waves hold 32 (F32 q) or 64 (16-bit q) rows each, as the
-// columns of 32x32x16 MFMAs, and share tiles of 64 keys in LDS, two in turn:
-// the next tile's loads are issued before a tile's products and written to the
-// other buffer after them, one barrier a tile. A fragment of K or V read from
-// LDS feeds two MFMAs (two parts of F32 q, or two columns of 32 rows): with one
-// the LDS reads alone (128 B a cycle) would take as long as the products.
+// A workgroup's waves hold 32 rows each, as the columns of 32x32x16 MFMAs, and
+// share tiles of 64 keys in LDS. Eight waves, two on a SIMD, so that one's
+// softmax runs under the other's products; within a wave too the scores of the
+// next 32 keys are formed next to the softmax of these (four waves where
+// three parts of an F32 q leave no registers for that). A tile's loads are
+// issued a tile ahead and written to LDS half a tile before its first use,
+// one barrier a tile; three tiles lie in LDS, as the slowest wave may still read
+// the one before while the fastest writes the one after.
 // Rows of 2 D bytes are stored with their 16-byte chunks permuted by the key
 // (tile_chunk), which keeps both the row reads of K and the transposing reads
 // of V off each other's banks.
@@ -15,7 +17,7 @@
 namespace qk {
 namespace {
 
-constexpr int kKeys = 64, kWaves = 4;
+constexpr int kKeys = 64;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // The 16-byte chunk of a row is XORed so that 16 consecutive keys (a K read)
@@ -30,21 +32,24 @@ __device__ __forceinline__ int tile_chunk(int key, int chunk) {
 }
 
 template <int D, bool BF16, bool Q32>
-__global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(64 * attention_many_waves(BF16, Q32), attention_many_waves(BF16, Q32) / 4) void
+attention_many_kernel(const AttentionArgs a) {
   typedef Num<BF16> N;
   typedef typename N::T T;
   typedef typename N::V8 V8;
+  constexpr int kWaves = attention_many_waves(BF16, Q32);
   constexpr int NP = kParts<BF16, Q32>;
-  constexpr int RT = Q32 ? 1 : 2;           // 32-row columns a wave
-  constexpr int kRows = 32 * RT * kWaves;   // rows of a tile
+  constexpr int kRows = 32 * kWaves;        // rows of a tile
   constexpr int KS = D / 16, DT = D / 32;   // k steps of q.k, 32-wide tiles of the output
   constexpr int LPK = D / 8;                // lanes that load one key
-  constexpr int KPL = 256 / LPK;            // keys a load of the workgroup
+  constexpr int KPL = 64 * kWaves / LPK;    // keys a load of the workgroup
   constexpr int NL = kKeys / KPL;           // such loads a tile
+  constexpr int kTile = kKeys * 2 * D;      // bytes of a tile's keys, or values
+  constexpr int kRing = 8;                  // tiles whose places are kept
   struct Shared {
-    uint8_t k[2][kKeys * 2 * D];
-    uint8_t v[2][kKeys * 2 * D];
-    int64_t place[3][kKeys];
+    uint8_t k[3][kTile];
+    uint8_t v[3][kTile];
+    int64_t place[kRing][kKeys];
     uint32_t odd[4], bad, arrived;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
@@ -59,24 +64,22 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
   if (tid == 0) sh.bad = sh.odd[0] = sh.odd[1] = 0;  // odd[n & 3] is cleared while tile n - 2 runs
   if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
 
-  // the lane's rows
+  // the lane's row
   const int col = lane & 31, half = lane >> 5;
-  int last[RT], from[RT];
-  int64_t out_at[RT];
-  V8 q[RT][KS][NP];
-  float factor[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int row = t.begin + (wave * RT + i) * 32 + col;
-    const bool live = row < t.rows;
-    const int token = t.row + (live ? row / a.group : 0), h = head * a.group + (live ? row % a.group : 0);
-    const int position = t.first + (token - t.row);
-    last[i] = live ? min(position, c.hi - 1) : -1;
-    from[i] = a.window > 0 ? position - a.window + 1 : 0;
-    out_at[i] = live ? static_cast<int64_t>(token) * a.q_heads + h : -1;
-    factor[i] = a.scale * kLog2e;
+  const int wave_row = t.begin + wave * 32;
+  const int row = wave_row + col;
+  const bool live = row < t.rows;
+  const int token = t.row + (live ? row / a.group : 0), h = head * a.group + (live ? row % a.group : 0);
+  const int position = t.first + (token - t.row);
+  const int last = live ? min(position, c.hi - 1) : -1;
+  const int from = a.window > 0 ? position - a.window + 1 : 0;
+  const int64_t out_at = live ? static_cast<int64_t>(token) * a.q_heads + h : -1;
+  V8 q[KS][NP];
+  float factor = fabsf(a.scale) * kLog2e;  // a negative scale's sign goes into q, so that the largest score is the largest q.k
+  {
     const int64_t at = token * a.q_stride + static_cast<int64_t>(h) * D + 8 * half;
     if constexpr (Q32) {
+      const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
       float x[KS][8];
       float most = 0.0f;
 #pragma unroll
@@ -86,7 +89,7 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
           const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at + 16 * s + e);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            x[s][e + j] = live ? v[j] : 0.0f;
+            x[s][e + j] = live ? v[j] * sign : 0.0f;
             most = fmaxf(most, fabsf(x[s][e + j]));
           }
         }
@@ -94,33 +97,35 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
         most = swap32_max(most);
         const bool scaled = most > 0.0f && most < __builtin_inff();
         const int e = scaled ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;  // the row's largest in [2^13, 2^14)
-        factor[i] = ldexpf(factor[i], -e);
+        factor = ldexpf(factor, -e);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[s][j] = ldexpf(x[s][j], e);
       }
 #pragma unroll
-      for (int s = 0; s < KS; ++s) split8<BF16, NP>(x[s], q[i][s]);
+      for (int s = 0; s < KS; ++s) split8<BF16, NP>(x[s], q[s]);
     } else {
+      const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const u32x4 v = load16(static_cast<const uint16_t*>(a.q) + at + 16 * s);
-        q[i][s][0] = __builtin_bit_cast(V8, live ? v : u32x4{});
+        const u32x4 v = load16(static_cast<const uint16_t*>(a.q) + at + 16 * s) ^ sign;
+        q[s][0] = __builtin_bit_cast(V8, live ? v : u32x4{});
       }
     }
   }
+  // a factor of nothing would turn the -inf of masked scores into NaN
+  factor = fmaxf(factor, 0x1p-126f);
   // all rows of the wave / of the workgroup see the keys of [.._from, .._last]
-  const int wave_row = t.begin + wave * RT * 32;
-  const int wave_end = min(wave_row + RT * 32, t.rows), tile_end = min(t.begin + kRows, t.rows);
+  const int wave_end = min(wave_row + 32, t.rows), tile_end = min(t.begin + kRows, t.rows);
   const int wave_last = t.first + wave_row / a.group, tile_last = t.first + t.begin / a.group;
   const int wave_from = a.window > 0 ? t.first + (wave_end - 1) / a.group - a.window + 1 : 0;
   const int tile_from = a.window > 0 ? t.first + (tile_end - 1) / a.group - a.window + 1 : 0;
   // and some row of the wave sees a key of [any_from, any_last]
-  const int any_last = wave_row < t.rows ? t.first + (wave_end - 1) / a.group : -1;
+  const int any_last = wave_row < t.rows ? min(t.first + (wave_end - 1) / a.group, c.hi - 1) : -1;
   const int any_from = a.window > 0 ? wave_last - a.window + 1 : 0;
 
-  // tiles of keys: page ids (wave 0, a lane a key) three ahead, places two, loads one
+  // tiles of keys: page ids (wave 0, a lane a key) four ahead, places three, loads two
   const int count = (c.hi - c.lo + kKeys - 1) / kKeys;
   int32_t page = 0;
   bool listed = true, bad = false;
@@ -132,24 +137,26 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
     if (n >= count) return;
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
-    sh.place[n % 3][lane] = kv_place(a.kv, ok ? page : 0, key_of(n) % a.kv.page_size, head);
+    sh.place[n & (kRing - 1)][lane] = kv_place(a.kv, ok ? page : 0, key_of(n) % a.kv.page_size, head);
   };
   u32x4 kreg[NL], vreg[NL];
   const auto load = [&](int n) {
+    if (n >= count) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int64_t at = sh.place[n % 3][KPL * i + tid / LPK] + 8 * (tid % LPK);
+      const int64_t at = sh.place[n & (kRing - 1)][KPL * i + tid / LPK] + 8 * (tid % LPK);
       kreg[i] = load16(a.kv.k + at);
       vreg[i] = load16(a.kv.v + at);
     }
   };
-  // registers -> LDS buffer n & 1; values of keys past the end become zeros,
-  // and where some row does not see some key, so do infinite ones (odd)
-  const auto store = [&](int n) {
+  // registers -> LDS; values of keys past the end become zeros, and where some
+  // row does not see some key, so do infinite ones (odd)
+  const auto store = [&](int n, int buffer) {
+    if (n >= count) return;
     const int key0 = c.lo + n * kKeys;
     const bool edge = !(key0 + kKeys - 1 <= tile_last && key0 + kKeys <= c.hi && key0 >= tile_from);
-    bool odd = false;
     if (edge) {
+      bool odd = false;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         if (key0 + KPL * i + tid / LPK >= c.hi) vreg[i] = u32x4{};
@@ -162,31 +169,14 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int at = tile_chunk<D>(KPL * i + tid / LPK, tid % LPK);
-      *reinterpret_cast<u32x4*>(sh.k[n & 1] + at) = kreg[i];
-      *reinterpret_cast<u32x4*>(sh.v[n & 1] + at) = vreg[i];
+      const int at = buffer * kTile + tile_chunk<D>(KPL * i + tid / LPK, tid % LPK);
+      *reinterpret_cast<u32x4*>(sh.k[0] + at) = kreg[i];
+      *reinterpret_cast<u32x4*>(sh.v[0] + at) = vreg[i];
     }
   };
-  if (count > 0) {
-    if (wave == 0) {
-      look_up(0);
-      settle(0);
-      look_up(1);
-    }
-    __syncthreads();
-    load(0);
-    if (wave == 0) {
-      settle(1);
-      look_up(2);
-    }
-    store(0);
-  }
-  __syncthreads();
 
-  f32x16 o[RT][DT] = {};
-  float top[RT], sum[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) top[i] = kNoMax, sum[i] = 0.0f;
+  f32x16 o[DT] = {};
+  float top = kNoMax, sum = 0.0f;
   const int k_at = tile_chunk<D>(col, half);  // chunk 2 s + half: ^ (s << 5)
   // V: key 4 half + (lane & 15) / 4, then 8 on; chunk 4 d + 2 (lane >> 4 & 1) + (lane >> 1 & 1)
   const int v_key = 4 * half + (lane >> 2 & 3), v_chunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
@@ -195,99 +185,131 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
   typedef short i16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) i16x4* LdsRow;
 
-  for (int n = 0; n < count; ++n) {
-    if (n + 1 < count) load(n + 1);
-    if (wave == 0) {
-      settle(n + 2);
-      look_up(n + 3);
+  // blocks of 32 keys; `at`: of the block in sh.k and sh.v
+  const auto scores = [&](int at, f32x16& x) {
+    x = f32x16{};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const V8 k = __builtin_bit_cast(V8, load16(sh.k[0] + at + (k_at ^ (s << 5))));
+#pragma unroll
+      for (int p = 0; p < NP; ++p) x = N::mfma32(k, q[s][p], x);
     }
-    const int tile0 = c.lo + n * kKeys;
-    uint8_t *ks = sh.k[n & 1], *vs = sh.v[n & 1];
-    const bool odd = sh.odd[n & 3] != 0;
-    if (tid == 0) sh.odd[(n + 2) & 3] = 0;  // read last for tile n - 2, set next after this tile's barrier
+  };
+  // The softmax step of the block whose q.k are in x and the product with its
+  // values; between the two, next to the exponentials, the scores of the next
+  // block into y. Registers 8 g + 4 e + r of x hold key 16 g + 8 e + 4 half + r.
+  const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16& y) {
+    if (!(key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from)) {  // some row does not see some key
 #pragma unroll
-    for (int j = 0; j < kKeys / 32; ++j) {
-      const int key0 = tile0 + 32 * j;
-      if (key0 > any_last || key0 + 31 < any_from || key0 >= c.hi) continue;  // nothing for this wave
-      f32x16 x[RT] = {};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const V8 k = __builtin_bit_cast(V8, load16(ks + j * 32 * 2 * D + (k_at ^ (s << 5))));
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int p = 0; p < NP; ++p) x[i] = N::mfma32(k, q[i][s][p], x[i]);
+      for (int r = 0; r < 16; ++r) {
+        const int key = key0 + (r >> 3) * 16 + (r >> 2 & 1) * 8 + 4 * half + (r & 3);
+        x[r] = key <= last && key >= from ? x[r] : -__builtin_inff();
       }
-      // registers 8 g + 4 e + r hold key 16 g + 8 e + 4 half + r
-      const bool whole = key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from;
-      V8 w[RT][2][NP];
+    }
+    float most = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        float most = -__builtin_inff();
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, x[r]);
+    most = swap32_max(most) * factor;
+    if (__any(most > top + kSlack)) {
+      const float to = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
+    }
+    scores(next_at, y);
+    const float base = kLift - top;
+    V8 w[2][NP];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * g + e], factor, base));
+        sum += p[e];
+      }
+      split8<BF16, NP>(p, w[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        uint8_t* const row = sh.v[0] + at + 16 * g * 2 * D;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at0 ^ (d << 6))));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at1 ^ (d << 6))));
+        const V8 v = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) o[d] = N::mfma32(v, w[g][p], o[d]);
+      }
+  };
+  // infinite or NaN values went into the product as zeros (0 times them is no
+  // zero); the rows that see them get them here
+  const auto add_infinite = [&](int n) {
+    for (int m = 0; m < kKeys; ++m) {
+      const int key = c.lo + n * kKeys + m;
+      if (key >= c.hi) break;
+      const uint16_t* v = a.kv.v + sh.place[n & (kRing - 1)][m] + 4 * half;
+      const bool sees = key <= last && key >= from;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          x[i][r] *= factor[i];
-          if (!whole) {
-            const int key = key0 + (r >> 3) * 16 + (r >> 2 & 1) * 8 + 4 * half + (r & 3);
-            x[i][r] = key <= last[i] && key >= from[i] ? x[i][r] : -__builtin_inff();
-          }
-          most = fmaxf(most, x[i][r]);
+          const float e = static_cast<float>(__builtin_bit_cast(T, v[32 * d + (r >> 2) * 8 + (r & 3)]));
+          if (sees && !(fabsf(e) < __builtin_inff())) o[d][r] += e;
         }
-        most = swap32_max(most);
-        if (__any(most > top[i] + kSlack)) {
-          const float to = fmaxf(top[i], most), f = __builtin_amdgcn_exp2f(top[i] - to);
-          top[i] = to;
-          sum[i] *= f;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[i][d] = o[i][d] * f;
-        }
-        const float base = top[i] - kLift;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(x[i][8 * g + e] - base);
-            sum[i] += p[e];
-          }
-          split8<BF16, NP>(p, w[i][g]);
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          uint8_t* const row = vs + (32 * j + 16 * g) * 2 * D;
-          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at0 ^ (d << 6))));
-          const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at1 ^ (d << 6))));
-          const V8 v = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) o[i][d] = N::mfma32(v, w[i][g][p], o[i][d]);
-        }
-      if (odd) {
-        // infinite or NaN values went into the product as zeros (0 times them
-        // is no zero); the rows that see them get them here
-        for (int m = 0; m < 32 && key0 + m < c.hi; ++m) {
-          const uint16_t* v = a.kv.v + sh.place[n % 3][32 * j + m] + 4 * half;
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            const bool sees = key0 + m <= last[i] && key0 + m >= from[i];
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const float e = static_cast<float>(__builtin_bit_cast(T, v[32 * d + (r >> 2) * 8 + (r & 3)]));
-                if (sees && !(fabsf(e) < __builtin_inff())) o[i][d][r] += e;
-              }
-          }
-        }
-      }
     }
-    // the other buffer: its last reads were before the barrier that ended tile n - 1
-    if (n + 1 < count) store(n + 1);
+  };
+  // tile n + 1 into LDS, the loads and look-ups after it; then all may read it
+  int buffer = 0;  // of tile n
+  const auto advance = [&](int n) {
+    store(n + 1, buffer == 2 ? 0 : buffer + 1);
+    load(n + 2);
+    if (wave == 0) {
+      settle(n + 3);
+      look_up(n + 4);
+    }
+    if (tid == 0) sh.odd[(n + 2) & 3] = 0;  // read last before the barrier of tile n - 1, set next after this one
     __syncthreads();
+  };
+
+  if (count > 0) {
+    if (wave == 0) {
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        look_up(n);
+        settle(n);
+      }
+      look_up(3);
+    }
+    __syncthreads();
+    load(0);
+    store(0, 0);
+    load(1);
+    __syncthreads();
+  }
+  // the tiles that some row of the wave sees; through the others it only helps to load
+  const int first = any_last < any_from ? count : max(any_from - c.lo, 0) / kKeys;
+  const int end = any_last < any_from ? count : min((any_last - c.lo + kKeys) / kKeys, count);
+  int n = 0;
+  for (; n < min(first, count); ++n) {
+    advance(n);
+    buffer = buffer == 2 ? 0 : buffer + 1;
+  }
+  if (n < end) {
+    f32x16 x0, x1;
+    scores(buffer * kTile, x0);
+    for (; n < end; ++n) {
+      const int key0 = c.lo + n * kKeys, at = buffer * kTile, next = buffer == 2 ? 0 : buffer + 1;
+      attend(key0, at, x0, at + 32 * 2 * D, x1);
+      advance(n);
+      attend(key0 + 32, at + 32 * 2 * D, x1, next * kTile, x0);  // past the last tile: scores that are not used
+      if (sh.odd[n & 3]) add_infinite(n);
+      buffer = next;
+    }
+  }
+  for (; n < count; ++n) {
+    advance(n);
+    buffer = buffer == 2 ? 0 : buffer + 1;
   }
 
   if (wave == 0 && __any(bad) && lane == 0) {
@@ -295,87 +317,73 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
     kv_fault(a.kv, QK_KV_FAULT_PAGE);
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    sum[i] = swap32_sum(sum[i]);
-    if (sh.bad) sum[i] = __builtin_nanf("");
-  }
+  sum = swap32_sum(sum);
+  if (sh.bad) sum = __builtin_nanf("");
   if (c.used > 1) {
-    // parts as the registers hold them: [row tile][d tile][register quad][lane]
+    // parts as the registers hold them: [wave][d tile][register quad][lane]
     const int64_t slot = (static_cast<int64_t>(tile) * a.kv.kv_heads + head) * a.splits;
-    const auto sums_of = [&](int k, int i) { return a.sums + 2 * (((slot + k) * kWaves + wave) * RT + i) * 32 + 2 * col; };
-    const auto part_of = [&](int k, int i) {
-      return a.parts + (((slot + k) * kWaves + wave) * RT + i) * (32 * D) + 4 * lane;
-    };
+    const auto sums_of = [&](int k) { return a.sums + 2 * (((slot + k) * kWaves + wave) * 32 + col); };
+    const auto part_of = [&](int k) { return a.parts + ((slot + k) * kWaves + wave) * (32 * D) + 4 * lane; };
     const bool any = wave_row < t.rows;
     if (any) {
+      if (half == 0) put(sums_of(split), top, sum);
+      float* part = part_of(split);
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (half == 0) put(sums_of(split, i), top[i], sum[i]);
-        float* part = part_of(split, i);
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            put(part + (4 * d + r / 4) * 256, o[i][d][r], o[i][d][r + 1]);
-            put(part + (4 * d + r / 4) * 256 + 2, o[i][d][r + 2], o[i][d][r + 3]);
-          }
-      }
+        for (int r = 0; r < 16; r += 4) {
+          put(part + (4 * d + r / 4) * 256, o[d][r], o[d][r + 1]);
+          put(part + (4 * d + r / 4) * 256 + 2, o[d][r + 2], o[d][r + 3]);
+        }
     }
     if (!last_to_arrive(a.arrived + static_cast<int64_t>(tile) * a.kv.kv_heads + head, c.used, sh.arrived)) return;
     if (!any) return;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      float all = kNoMax;
-      for (int k = 0; k < c.used; ++k) {
-        float m, l;
-        get(sums_of(k, i), m, l);
-        all = fmaxf(all, m);
-      }
-      sum[i] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[i][d] = f32x16{};
-      for (int k = 0; k < c.used; ++k) {
-        float m, l;
-        get(sums_of(k, i), m, l);
-        const float f = __builtin_amdgcn_exp2f(m - all);
-        sum[i] += f * l;
-        const float* part = part_of(k, i);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) {
-            float y0, y1;
-            get(part + (4 * d + r / 4) * 256 + (r & 2), y0, y1);
-            o[i][d][r] += f * y0;
-            o[i][d][r + 1] += f * y1;
-          }
-      }
-      top[i] = all;
+    float all = kNoMax;
+    for (int k = 0; k < c.used; ++k) {
+      float m, l;
+      get(sums_of(k), m, l);
+      all = fmaxf(all, m);
     }
-  }
+    sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    if (out_at[i] < 0) continue;
-    const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+    for (int d = 0; d < DT; ++d) o[d] = f32x16{};
+    for (int k = 0; k < c.used; ++k) {
+      float m, l;
+      get(sums_of(k), m, l);
+      const float f = __builtin_amdgcn_exp2f(m - all);
+      sum += f * l;
+      const float* part = part_of(k);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int64_t at = out_at[i] * D + 32 * d + 2 * r + 4 * half;
-        const f32x4 y = f32x4{o[i][d][r], o[i][d][r + 1], o[i][d][r + 2], o[i][d][r + 3]} * inv;
-        if constexpr (Q32) {
-          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
-        } else {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 z;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z[e] = static_cast<T>(y[e]);
-          *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = z;
+        for (int r = 0; r < 16; r += 2) {
+          float y0, y1;
+          get(part + (4 * d + r / 4) * 256 + (r & 2), y0, y1);
+          o[d][r] += f * y0;
+          o[d][r + 1] += f * y1;
         }
-      }
-    if (a.lse && half == 0) a.lse[out_at[i]] = row_lse(top[i], sum[i]);
+    }
+    top = all;
   }
+  if (out_at < 0) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int64_t at = out_at * D + 32 * d + 2 * r + 4 * half;
+      const f32x4 y = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]} * inv;
+      if constexpr (Q32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
+      } else {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = static_cast<T>(y[e]);
+        *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at) = z;
+      }
+    }
+  if (a.lse && half == 0) a.lse[out_at] = row_lse(top, sum);
 }
 
 }  // namespace
@@ -383,7 +391,8 @@ __global__ __launch_bounds__(256, Q32 && !BF16 ? 2 : 1) void attention_many_kern
 hipError_t launch_attention_many(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(a.tiles) * a.splits * a.kv.kv_heads;
   const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
-  auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, stream>>>(a); };
+  const int threads = 64 * attention_many_waves(bf16, q32);
+  auto go = [&](auto kernel) { kernel<<<grid, threads, 0, stream>>>(a); };
   if (head_dim == 128)
     bf16 ? (q32 ? go(attention_many_kernel<128, true, true>) : go(attention_many_kernel<128, true, false>))
          : (q32 ? go(attention_many_kernel<128, false, true>) : go(attention_many_kernel<128, false, false>));

@@ -699,9 +699,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     for (int i = tid >> 5; __any(i < actives); i += kThreads / 32) {
       const int c = i < actives ? sh.active[i] : 0, listed = i < actives ? sh.listed[c] : 0;
       const uint64_t* list = p.lists + (unit0 + c) * p.list;
-      for (int at = lane & 31; __any(at < listed); at += 32) {
-        const uint64_t item = at < listed ? list[at] : 0;
-        append(item && band_of(key_value(item_key(item)), top_value, scale) <= border, item, sh.items, &sh.n, kSorted);
+      for (int at = lane & 31; __any(at < listed); at += 32 * 8) {
+        uint64_t item[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) item[j] = at + 32 * j < listed ? list[at + 32 * j] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          append(item[j] && band_of(key_value(item_key(item[j])), top_value, scale) <= border, item[j], sh.items, &sh.n, kSorted);
       }
     }
     __syncthreads();
@@ -825,7 +829,21 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
         __syncthreads();
         const int listed = static_cast<int>(sh.n);
         done = listed <= kSorted;
-        if (done) {
+        if (listed <= 64) {  // one wave, an item a lane
+          if (wave == 0) {
+            const uint64_t item = lane < listed ? sh.sums[lane] : 0;
+            const uint64_t f = lane < listed ? w.fixed(item_key(item)) : 0;
+            uint64_t run = ahead + f;  // up to and with the lane's, downwards
+            for (int i = 0; i < listed; ++i) run += lane_value(item, i) > item ? lane_value(f, i) : 0;
+            // the item where the target is met, else the last
+            const uint64_t met_here = __ballot(lane < listed && run >= target && run - f < target);
+            int rank = 0;
+            for (int i = 0; i < listed; ++i) rank += lane_value(item, i) > item;
+            const uint64_t final = __ballot(lane < listed && rank == listed - 1);
+            if (lane == 0) sh.found[2] = static_cast<uint64_t>(__builtin_ctzll(met_here ? met_here : final));
+          }
+          __syncthreads();
+        } else if (done) {
           sort_down(sh.sums, listed);
           uint64_t mine[2];
 #pragma unroll
@@ -835,6 +853,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
           __syncthreads();
           if (run < target && run + mine[0] + mine[1] >= target) sh.found[2] = static_cast<uint64_t>(2 * tid + (run + mine[0] < target));
           __syncthreads();
+        }
+        if (done) {
           const uint64_t item = sh.sums[sh.found[2]];
           least = item_key(item);
           last = item_index(item);

@@ -52,12 +52,15 @@ struct AttentionArgs {
 
 // How a call is laid out, from host values alone.
 struct AttentionPlan {
-  bool few;              // 16-row tiles (paged_attention_few.hip), else 128 or 256 (paged_attention_many.hip)
+  bool few;              // 16-row tiles (paged_attention_few.hip), else 256 or 128 (paged_attention_many.hip)
   int rows;              // rows of a tile: (new token, query head of the key/value head)
   int32_t tiles;         // at most so many tiles
   int32_t splits;        // workgroups that may share a tile's keys
   size_t sums_at, parts_at, bytes;  // workspace; 0 bytes without splits
 };
+// Waves of a workgroup of paged_attention_many.hip, 32 rows each: eight, but
+// four with 512 registers each where F32 q meets a BF16 cache (three parts).
+constexpr int attention_many_waves(bool bf16, bool q32) { return bf16 && q32 ? 4 : 8; }
 AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int head_dim, int type,
                              int q_type, int64_t window, int64_t max_context);
 hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, int type, int head_dim, int q_type,
