@@ -12,6 +12,8 @@
 // Rows of 2 D bytes are stored with their 16-byte chunks permuted by the key
 // (tile_chunk), which keeps both the row reads of K and the transposing reads
 // of V off each other's banks.
+#include <type_traits>
+
 #include "paged_attention.hpp"
 
 namespace qk {
@@ -121,9 +123,8 @@ attention_many_kernel(const AttentionArgs a) {
   const int wave_last = t.first + wave_row / a.group, tile_last = t.first + t.begin / a.group;
   const int wave_from = a.window > 0 ? t.first + (wave_end - 1) / a.group - a.window + 1 : 0;
   const int tile_from = a.window > 0 ? t.first + (tile_end - 1) / a.group - a.window + 1 : 0;
-  // and some row of the wave sees a key of [any_from, any_last]
+  // and no row of the wave sees a key past any_last
   const int any_last = wave_row < t.rows ? min(t.first + (wave_end - 1) / a.group, c.hi - 1) : -1;
-  const int any_from = a.window > 0 ? wave_last - a.window + 1 : 0;
 
   // tiles of keys: page ids (wave 0, a lane a key) four ahead, places three, loads two
   const int count = (c.hi - c.lo + kKeys - 1) / kKeys;
@@ -177,20 +178,34 @@ attention_many_kernel(const AttentionArgs a) {
 
   f32x16 o[DT] = {};
   float top = kNoMax, sum = 0.0f;
-  const int k_at = tile_chunk<D>(col, half);  // chunk 2 s + half: ^ (s << 5)
-  // V: key 4 half + (lane & 15) / 4, then 8 on; chunk 4 d + 2 (lane >> 4 & 1) + (lane >> 1 & 1)
-  const int v_key = 4 * half + (lane >> 2 & 3), v_chunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-  const int v_at0 = tile_chunk<D>(v_key, v_chunk) + (lane & 1) * 8;
-  const int v_at1 = tile_chunk<D>(v_key + 8, v_chunk) + (lane & 1) * 8;
+  // LDS addresses. K: key col, chunk 2 s + half. V: key 4 half + (lane & 15) / 4,
+  // then 8 on, chunk 4 d + 2 (lane >> 4 & 1) + (lane >> 1 & 1). Kept as they
+  // are (opaque), so that buffer and block are constants of the instructions.
   typedef short i16x4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) i16x4* LdsRow;
+  typedef __attribute__((address_space(3))) i16x4* LdsQuad;
+  typedef __attribute__((address_space(3))) u32x4* LdsChunk;
+  typedef __attribute__((address_space(3))) uint8_t* LdsByte;
+  uint32_t k_at[KS], v_at[DT][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    k_at[s] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte)sh.k[0])) + tile_chunk<D>(col, 2 * s + half);
+    asm("" : "+v"(k_at[s]));
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v_at[d][i] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsByte)sh.v[0])) +
+                   tile_chunk<D>(4 * half + (lane >> 2 & 3) + 8 * i, 4 * d + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) + (lane & 1) * 8;
+      asm("" : "+v"(v_at[d][i]));
+    }
 
   // blocks of 32 keys; `at`: of the block in sh.k and sh.v
   const auto scores = [&](int at, f32x16& x) {
     x = f32x16{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const V8 k = __builtin_bit_cast(V8, load16(sh.k[0] + at + (k_at ^ (s << 5))));
+      const V8 k = __builtin_bit_cast(V8, *(LdsChunk)(uintptr_t)(k_at[s] + at));
 #pragma unroll
       for (int p = 0; p < NP; ++p) x = N::mfma32(k, q[s][p], x);
     }
@@ -198,7 +213,7 @@ attention_many_kernel(const AttentionArgs a) {
   // The softmax step of the block whose q.k are in x and the product with its
   // values; between the two, next to the exponentials, the scores of the next
   // block into y. Registers 8 g + 4 e + r of x hold key 16 g + 8 e + 4 half + r.
-  const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16& y) {
+  const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16& y) __attribute__((always_inline)) {
     if (!(key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from)) {  // some row does not see some key
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -234,9 +249,9 @@ attention_many_kernel(const AttentionArgs a) {
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        uint8_t* const row = sh.v[0] + at + 16 * g * 2 * D;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at0 ^ (d << 6))));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(row + (v_at1 ^ (d << 6))));
+        const int row = at + 16 * g * 2 * D;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad)(uintptr_t)(v_at[d][0] + row));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad)(uintptr_t)(v_at[d][1] + row));
         const V8 v = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int p = 0; p < NP; ++p) o[d] = N::mfma32(v, w[g][p], o[d]);
@@ -260,9 +275,8 @@ attention_many_kernel(const AttentionArgs a) {
     }
   };
   // tile n + 1 into LDS, the loads and look-ups after it; then all may read it
-  int buffer = 0;  // of tile n
-  const auto advance = [&](int n) {
-    store(n + 1, buffer == 2 ? 0 : buffer + 1);
+  const auto advance = [&](int n, int next) __attribute__((always_inline)) {
+    store(n + 1, next);
     load(n + 2);
     if (wave == 0) {
       settle(n + 3);
@@ -272,12 +286,13 @@ attention_many_kernel(const AttentionArgs a) {
     __syncthreads();
   };
 
+  int n = 0;
   if (count > 0) {
     if (wave == 0) {
 #pragma unroll
-      for (int n = 0; n < 3; ++n) {
-        look_up(n);
-        settle(n);
+      for (int i = 0; i < 3; ++i) {
+        look_up(i);
+        settle(i);
       }
       look_up(3);
     }
@@ -286,30 +301,26 @@ attention_many_kernel(const AttentionArgs a) {
     store(0, 0);
     load(1);
     __syncthreads();
-  }
-  // the tiles that some row of the wave sees; through the others it only helps to load
-  const int first = any_last < any_from ? count : max(any_from - c.lo, 0) / kKeys;
-  const int end = any_last < any_from ? count : min((any_last - c.lo + kKeys) / kKeys, count);
-  int n = 0;
-  for (; n < min(first, count); ++n) {
-    advance(n);
-    buffer = buffer == 2 ? 0 : buffer + 1;
-  }
-  if (n < end) {
-    f32x16 x0, x1;
-    scores(buffer * kTile, x0);
-    for (; n < end; ++n) {
-      const int key0 = c.lo + n * kKeys, at = buffer * kTile, next = buffer == 2 ? 0 : buffer + 1;
-      attend(key0, at, x0, at + 32 * 2 * D, x1);
-      advance(n);
-      attend(key0 + 32, at + 32 * 2 * D, x1, next * kTile, x0);  // past the last tile: scores that are not used
-      if (sh.odd[n & 3]) add_infinite(n);
-      buffer = next;
+    // through the tiles that no row of the wave sees it only helps to load
+    const int end = any_last < c.lo ? 0 : min((any_last - c.lo) / kKeys + 1, count);
+    if (end > 0) {
+      f32x16 x0, x1;
+      scores(0, x0);
+      // tile n in buffer n % 3; past the last tile the scores are of no tile, and not used
+      const auto both = [&](auto buffer) __attribute__((always_inline)) {
+        constexpr int at = decltype(buffer)::value * kTile, next = (decltype(buffer)::value + 1) % 3;
+        const int key0 = c.lo + n * kKeys;
+        attend(key0, at, x0, at + 32 * 2 * D, x1);
+        advance(n, next);
+        attend(key0 + 32, at + 32 * 2 * D, x1, next * kTile, x0);
+        if (sh.odd[n & 3]) add_infinite(n);
+        return ++n < end;
+      };
+      while (both(std::integral_constant<int, 0>{}) && both(std::integral_constant<int, 1>{}) &&
+             both(std::integral_constant<int, 2>{})) {
+      }
     }
-  }
-  for (; n < count; ++n) {
-    advance(n);
-    buffer = buffer == 2 ? 0 : buffer + 1;
+    for (; n < count; ++n) advance(n, (n + 1) % 3);
   }
 
   if (wave == 0 && __any(bad) && lane == 0) {
