@@ -12,6 +12,11 @@ constexpr int64_t kUnits = 256;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
+// Calls too small for a 256-row tile on every unit: up to so many keys, tiles of
+// 64 rows whose waves share the keys are faster than 256-row tiles whose keys
+// workgroups share (us: 512 tokens of 32 heads over 2048 keys 48 against 50, over
+// 4096 keys 91 against 82; four sequences of 128 over 1000 26 against 31).
+constexpr int64_t kPartedKeys = 2048;
 constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -24,15 +29,21 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   if (tokens == 0 || sequences == 0) return p;
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   p.few = rows <= 32 * sequences;
-  const int tile_rows = p.few ? 16 : 32 * attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
-  p.rows = tile_rows;
+  const int waves_rows = 32 * attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
   // every sequence may end in a part of a tile, and none has a tile without a row
-  int64_t tiles = rows / tile_rows + sequences;
-  if (tiles > rows) tiles = rows;
-  if (group <= tile_rows && tiles > tokens) tiles = tokens;
-  p.tiles = static_cast<int32_t>(tiles);
+  const auto tiles_of = [&](int tile_rows) {
+    int64_t tiles = rows / tile_rows + sequences;
+    if (tiles > rows) tiles = rows;
+    if (group <= tile_rows && tiles > tokens) tiles = tokens;
+    return tiles;
+  };
   int64_t keys = max_context < 1 ? 1 : max_context;
-  if (window > 0 && keys > window + tile_rows) keys = window + tile_rows;
+  if (window > 0 && keys > window + waves_rows) keys = window + waves_rows;
+  p.parted = !p.few && tiles_of(waves_rows) * kv_heads < kUnits && keys <= kPartedKeys;
+  const int tile_rows = p.few ? 16 : p.parted ? waves_rows / 4 : waves_rows;
+  p.rows = tile_rows;
+  const int64_t tiles = tiles_of(tile_rows);
+  p.tiles = static_cast<int32_t>(tiles);
   const int64_t want = p.few ? kMostUnits : kUnits;
   const int64_t least = p.few ? 128 : 256;
   int64_t splits = up(want, tiles * kv_heads);
@@ -56,7 +67,7 @@ hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, in
   a.sums = reinterpret_cast<float*>(ws + plan.sums_at);
   a.parts = reinterpret_cast<float*>(ws + plan.parts_at);
   return plan.few ? launch_attention_few(a, type, head_dim, q_type, stream)
-                  : launch_attention_many(a, type, head_dim, q_type, stream);
+                  : launch_attention_many(a, plan.parted, type, head_dim, q_type, stream);
 }
 
 }  // namespace qk

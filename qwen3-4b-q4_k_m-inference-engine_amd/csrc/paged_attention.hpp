@@ -120,10 +120,9 @@ struct AttentionTile {
   bool fault;
 };
 
-// Sequence by sequence, ceil(rows / ROWS) tiles each: wave-parallel running
+// Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
 // sums of the tile counts until they pass `tile`.
-template <int ROWS>
-__device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile) {
+__device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile, int tile_rows) {
   const int lane = static_cast<int>(threadIdx.x & 63);
   AttentionTile t;
   t.s = -1;
@@ -134,7 +133,7 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
     KvSequence q{};
     if (s < a.kv.sequences) {
       q = kv_sequence(a.kv, s);
-      mine = (q.count * a.group + ROWS - 1) / ROWS;
+      mine = (q.count * a.group + tile_rows - 1) / tile_rows;
     }
     int run = mine;
 #pragma unroll
@@ -150,14 +149,14 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
       t.count = __builtin_amdgcn_readlane(q.count, at);
       t.first = __builtin_amdgcn_readlane(q.first, at);
       t.fault = __builtin_amdgcn_readlane(q.fault ? 1 : 0, at) != 0;
-      t.begin = (tile - before - __builtin_amdgcn_readlane(run - mine, at)) * ROWS;
+      t.begin = (tile - before - __builtin_amdgcn_readlane(run - mine, at)) * tile_rows;
       break;
     }
     before += __builtin_amdgcn_readlane(run, 63);
   }
   if (t.s < 0) return t;
   t.rows = t.count * a.group;
-  const int end = t.begin + ROWS < t.rows ? t.begin + ROWS : t.rows;
+  const int end = t.begin + tile_rows < t.rows ? t.begin + tile_rows : t.rows;
   t.key_hi = t.first + (end - 1) / a.group + 1;
   const int lowest = a.window > 0 ? t.first + t.begin / a.group - a.window + 1 : 0;
   t.key_lo = lowest > 0 ? lowest : 0;
@@ -209,6 +208,21 @@ __device__ __forceinline__ bool last_to_arrive(uint32_t* counter, int used, uint
   }
   __syncthreads();
   return shared_word + 1 == static_cast<uint32_t>(used);
+}
+
+// Four values of a row's result in q's type.
+template <bool BF16, bool Q32>
+__device__ __forceinline__ void store_row(void* out, int64_t at, f32x4 y) {
+  if constexpr (Q32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = y;
+  } else {
+    typedef typename Num<BF16>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = static_cast<T>(y[e]);
+    *reinterpret_cast<T4*>(static_cast<T*>(out) + at) = z;
+  }
 }
 
 // A row's sum and maximum as its log of the sum of exp.

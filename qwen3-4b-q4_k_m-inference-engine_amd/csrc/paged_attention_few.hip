@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
   const int tile = unit / a.splits, split = unit % a.splits;
-  const AttentionTile t = find_tile<kRows>(a, tile);
+  const AttentionTile t = find_tile(a, tile, kRows);
   if (t.s < 0) return;
   const KeyChunk c = key_chunk(t, split, a.splits, kStep, kStep);
   if (split >= c.used) return;
