@@ -8,6 +8,13 @@ namespace {
 // The card's compute units: a plan, and with it a workspace's size, is the
 // same with and without a device at hand.
 constexpr int64_t kUnits = 256;
+// Single tokens: contexts are cut where there are fewer (tile, head) units than
+// two a compute unit, into parts of kGoodPart keys, or as short as it takes for
+// that many workgroups. Longer parts leave a batch of uneven contexts unbalanced
+// (16 of up to 32768 keys, us: parts of 8192 237, of 2048 190), shorter ones
+// pay for their joining (one of 131072: parts of 2048 116, of 512 195); 64
+// of up to 8192 are not cut: 225, in parts of 2048 235.
+constexpr int64_t kGoodPart = kGoodPartKeys;
 // Keys are shared out only while a plan has fewer (tile, head) units than this,
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
@@ -44,13 +51,18 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   p.rows = tile_rows;
   const int64_t tiles = tiles_of(tile_rows);
   p.tiles = static_cast<int32_t>(tiles);
-  const int64_t want = p.few ? kMostUnits : kUnits;
+  const int64_t units = tiles * kv_heads;
+  int64_t splits = up(p.few ? kMostUnits : kUnits, units);
+  p.fill = static_cast<int32_t>(splits);
+  if (p.few && splits > 1 && splits < up(keys, kGoodPart)) {
+    const int64_t most = up(4 * kMostUnits, units);
+    splits = up(keys, kGoodPart) < most ? up(keys, kGoodPart) : most;
+  }
   const int64_t least = p.few ? 128 : 256;
-  int64_t splits = up(want, tiles * kv_heads);
   if (splits > up(keys, least)) splits = up(keys, least);
   p.splits = static_cast<int32_t>(splits);
   if (splits > 1) {
-    const size_t units = static_cast<size_t>(tiles * kv_heads), parts = units * splits * tile_rows;
+    const size_t parts = static_cast<size_t>(units * splits * tile_rows);
     p.sums_at = kCounterBytes;
     p.parts_at = p.sums_at + ((parts * 2 * sizeof(float) + 255) & ~size_t{255});
     p.bytes = p.parts_at + parts * head_dim * sizeof(float);
@@ -62,6 +74,7 @@ hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, in
                                   void* workspace, hipStream_t stream) {
   a.tiles = plan.tiles;
   a.splits = plan.splits;
+  a.fill = plan.fill;
   char* ws = static_cast<char*>(workspace);
   a.arrived = reinterpret_cast<uint32_t*>(ws);
   a.sums = reinterpret_cast<float*>(ws + plan.sums_at);

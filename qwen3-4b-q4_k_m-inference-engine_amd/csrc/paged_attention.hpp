@@ -23,6 +23,7 @@
 
 namespace qk {
 
+constexpr int kGoodPartKeys = 2048;  // see plan_attention
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr float kNoMax = -3.4028234e38f;  // the maximum of no score: no finite score is below it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -164,14 +165,32 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
   return t;
 }
 
-// A tile's keys over its workgroups: equal chunks, multiples of `step`, at
-// least `least`; `used` of them are not empty (one at least).
+// The most keys that a row of any sequence sees.
+__device__ __forceinline__ int longest_context(const AttentionArgs& a) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  int most = 0;
+  for (int s = lane; s < a.kv.sequences; s += 64) {
+    const KvSequence q = kv_sequence(a.kv, s);
+    const int keys = q.count > 0 ? q.first + q.count : 0;
+    most = keys > most ? keys : most;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const int other = __shfl_xor(most, off);
+    most = other > most ? other : most;
+  }
+  return __builtin_amdgcn_readfirstlane(a.window > 0 && most > a.window ? a.window : most);
+}
+
+// A tile's keys over its workgroups: chunks of `chunk` keys, but long enough that
+// `splits` of them suffice, in multiples of `step`; `used` of them are not empty
+// (one at least).
 struct KeyChunk {
   int lo, hi, used;
 };
-__device__ __forceinline__ KeyChunk key_chunk(const AttentionTile& t, int split, int splits, int step, int least) {
+__device__ __forceinline__ KeyChunk key_chunk(const AttentionTile& t, int split, int splits, int step, int chunk) {
   const int keys = t.key_hi - t.key_lo;
-  int chunk = (keys + splits - 1) / splits;
+  const int least = (keys + splits - 1) / splits;
   chunk = chunk < least ? least : chunk;
   chunk = (chunk + step - 1) / step * step;
   KeyChunk c;

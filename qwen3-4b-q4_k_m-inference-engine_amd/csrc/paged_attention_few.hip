@@ -3,12 +3,15 @@
 // of 16 rows, which one 16x16x32 MFMA takes as its columns.
 //
 // The four waves of a workgroup share nothing while they run: wave w takes
-// blocks w, w + 4, .. of 32 keys. Keys go from memory straight into the A
-// operand's layout (a lane holds 8 values of one key), values through the
-// wave's own 8 KB of LDS, from where ds_read_b64_tr_b16 brings four keys of a
-// column at a time; no barrier in the loop. Each block's loads are issued one
-// block ahead, its page ids two ahead, so 16 KB a wave are in flight under the
-// arithmetic.
+// blocks w, w + 4, .. of 32 keys and holds keys and values in 16 KB of LDS of its
+// own; keys are read from there as the A operand, values by
+// ds_read_b64_tr_b16, four keys of a column at a time. No barrier in the loop.
+// Each block's loads are issued one block ahead, its page ids two, so 16 KB a
+// wave are in flight under the arithmetic.
+// Loads take whole rows (256 bytes a key, 16 lanes) and are marked as not used
+// again: this card's plain reads reach 6.4 TB/s, those 7.2. 64 sequences of up to
+// 8192 keys, 1.06 GB: 225 us (4.7 TB/s); 263 with keys loaded straight into the
+// operand's layout (64 bytes of a row an instruction); 3 of 131072: 167 (5.2).
 #include "paged_attention.hpp"
 
 namespace qk {
@@ -24,6 +27,12 @@ __device__ __forceinline__ int v_chunk(int key, int chunk) {
   return key * (2 * D) + ((chunk ^ f) << 4);
 }
 
+// And of K rows, so that 16 keys' same chunk lie in different banks.
+template <int D>
+__device__ __forceinline__ int k_chunk(int key, int chunk) {
+  return key * (2 * D) + ((chunk ^ (D == 128 ? key & 15 : key >> 1 & 7)) << 4);
+}
+
 template <int D, bool BF16, bool Q32>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionArgs a) {
   typedef Num<BF16> N;
@@ -36,7 +45,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   constexpr int KPL = 64 / LPK;              // keys a load
   struct Shared {
     union {
-      uint8_t v[kWaves][kBlock * 2 * D];
+      struct {
+        uint8_t k[kWaves][kBlock * 2 * D];
+        uint8_t v[kWaves][kBlock * 2 * D];
+      };
       float o[kWaves][kRows][D];
     };
     int64_t place[kWaves][2][kBlock];
@@ -50,7 +62,15 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int tile = unit / a.splits, split = unit % a.splits;
   const AttentionTile t = find_tile(a, tile, kRows);
   if (t.s < 0) return;
-  const KeyChunk c = key_chunk(t, split, a.splits, kStep, kStep);
+  // chunks of one length for all sequences, so that a batch's longest does not outlast the rest
+  int chunk = kStep;
+  if (a.splits > 1) {
+    const int longest = longest_context(a), filled = longest / a.fill;
+    chunk = filled < kGoodPartKeys ? filled : kGoodPartKeys;
+    chunk = chunk < longest / a.splits ? longest / a.splits : chunk;
+    chunk = chunk < kStep ? kStep : chunk;
+  }
+  const KeyChunk c = key_chunk(t, split, a.splits, kStep, chunk);
   if (split >= c.used) return;
   if (tid == 0) sh.bad = 0;
   if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
@@ -78,28 +98,25 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     return key < c.hi ? key : c.hi - 1;
   };
   const auto look_up = [&](int b) {
-    if (b < blocks) page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(b) / a.kv.page_size, listed)];
+    page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(b) / a.kv.page_size, listed)];
   };
-  u32x4 kreg[2][KS], vreg[VL];
+  u32x4 kreg[VL], vreg[VL];
   const auto settle = [&](int b) {  // page id -> place of block b
     const int key = key_of(b);
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
-    if (lane < 32) sh.place[wave][b / kWaves & 1][lane] = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
+    sh.place[wave][b / kWaves & 1][lane & 31] = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
     __builtin_amdgcn_wave_barrier();
   };
   const auto load_k = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint16_t* p = a.kv.k + sh.place[wave][b / kWaves & 1][16 * i + col] + 8 * grp;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) kreg[i][s] = load16(p + 32 * s);
-    }
+    for (int i = 0; i < VL; ++i)
+      kreg[i] = stream_load16(a.kv.k + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
   };
   const auto load_v = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      vreg[i] = load16(a.kv.v + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
+      vreg[i] = stream_load16(a.kv.v + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
   };
   if (wave < blocks) {
     look_up(wave);
@@ -156,24 +173,29 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int tr_key = 4 * grp + (col >> 2);
   const int tr_at = v_chunk<D>(tr_key, col >> 1 & 1) + (col & 1) * 8;
   uint8_t* const vs = sh.v[wave];
+  uint8_t* const ks = sh.k[wave];
   typedef short i16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) i16x4* LdsRow;
 
   for (int b = wave; b < blocks; b += kWaves) {
     const int key0 = c.lo + b * kBlock;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4*>(ks + k_chunk<D>(KPL * i + lane / LPK, lane % LPK)) = kreg[i];
+    // loads past the last block are of its last key: a branch here would make
+    // every wait one for all loads in flight
+    const int next = b + kWaves;
+    settle(next);
+    load_k(next);
+    look_up(next + kWaves);
     f32x4 x[2] = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+      for (int i = 0; i < 2; ++i) {
+        const V8 k = __builtin_bit_cast(V8, load16(ks + i * (16 * 2 * D) + k_chunk<D>(col, 4 * s + grp)));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = N::mfma16(__builtin_bit_cast(V8, kreg[i][s]), q[s][p], x[i]);
-    const int next = b + kWaves;
-    if (next < blocks) {
-      settle(next);
-      load_k(next);
-      look_up(next + kWaves);
-    }
+        for (int p = 0; p < NP; ++p) x[i] = N::mfma16(k, q[s][p], x[i]);
+      }
     // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
     const bool whole = key0 + kBlock - 1 <= all_last && key0 + kBlock <= c.hi && key0 >= all_from;
     float most = -__builtin_inff();
@@ -222,7 +244,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       const int key = KPL * i + lane / LPK;
       *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, lane % LPK)) = odd ? only_finite<BF16>(vreg[i]) : vreg[i];
     }
-    if (next < blocks) load_v(next);
+    load_v(next);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int d = 0; d < DT; ++d) {

@@ -52,6 +52,9 @@ __device__ __forceinline__ uint32_t load_u32(const void* p) {
 __device__ __forceinline__ u32x4 stream_load16_a4(const void* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p));
 }
+__device__ __forceinline__ u32x4 stream_load16(const void* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
 
 // fp16 bits -> fp32 (exact, subnormals kept: the kernels run with fp16
 // denormals enabled, which is the gfx950 default mode).

@@ -44,7 +44,7 @@ struct AttentionArgs {
   void* out;
   float* lse;
   // the plan's part (launch_paged_attention)
-  int32_t tiles, splits;
+  int32_t tiles, splits, fill;
   uint32_t* arrived;  // [tiles x kv_heads], zero between calls
   float* sums;        // [tiles x kv_heads x splits x rows] (maximum, sum) pairs
   float* parts;       // [tiles x kv_heads x splits x rows x head_dim]
@@ -57,6 +57,7 @@ struct AttentionPlan {
   int rows;              // rows of a tile: (new token, query head of the key/value head)
   int32_t tiles;         // at most so many tiles
   int32_t splits;        // workgroups that may share a tile's keys
+  int32_t fill;          // so many of them fill the card
   size_t sums_at, parts_at, bytes;  // workspace; 0 bytes without splits
 };
 // Waves of a workgroup of paged_attention_many.hip, 32 rows each: eight, but
