@@ -312,27 +312,43 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     }
     if (!last_to_arrive(a.arrived + static_cast<int64_t>(tile) * a.kv.kv_heads + head, c.used, sh.arrived)) return;
     if (mine) {
+      // lane j of a row's 16 has the sums of parts j, j + 16, ..
+      const int j = tid & 15;
       all = kNoMax;
-      for (int k = 0; k < c.used; ++k) {
+      for (int k = j; k < c.used; k += 16) {
         float m, l;
         get(a.sums + 2 * ((slot + k) * kRows + r), m, l);
         all = fmaxf(all, m);
       }
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) all = fmaxf(all, __shfl_xor(all, off));
       total = 0.0f;
 #pragma unroll
       for (int i = 0; i < E; ++i) y[i] = 0.0f;
-#pragma unroll 4
-      for (int k = 0; k < c.used; ++k) {
-        const int64_t at = (slot + k) * kRows + r;
-        float m, l, part[E];
-        get(a.sums + 2 * at, m, l);
-#pragma unroll
-        for (int i = 0; i < E; i += 2) get(a.parts + at * D + e0 + i, part[i], part[i + 1]);
+      for (int base = 0; base < c.used; base += 16) {
+        float m = kNoMax, l = 0.0f;
+        if (base + j < c.used) get(a.sums + 2 * ((slot + base + j) * kRows + r), m, l);
         const float f = __builtin_amdgcn_exp2f(m - all);
         total += f * l;
+        const int some = c.used - base < 16 ? c.used - base : 16;
+        for (int k0 = 0; k0 < some; k0 += 8) {
+          float part[8][E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] += f * part[i];
+          for (int k = 0; k < 8; ++k) {  // past the last part: that one again, with no weight
+            const int64_t at = (slot + base + min(k0 + k, some - 1)) * kRows + r;
+#pragma unroll
+            for (int i = 0; i < E; i += 2) get(a.parts + at * D + e0 + i, part[k][i], part[k][i + 1]);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float g = __shfl(f, (tid & 48) + min(k0 + k, 15));
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] += k0 + k < some ? g * part[k][i] : 0.0f;
+          }
+        }
       }
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) total += __shfl_xor(total, off);
     }
   }
   if (!mine) return;
