@@ -404,8 +404,10 @@ int qk_kv_check(const qk_kv_cache *cache, qk_stream_t stream);
  * Weights are 64-bit, their sums exact in fixed point, so a result does not
  * depend on the order of any sum. vocabulary in [1, 2^24]; row_stride >= vocabulary.
  * workspace: qk_sample_workspace_size bytes, 256-byte aligned (may be NULL
- * when that is 0), zero-filled once; every call leaves it ready for the next.
- * Nothing is allocated. The reference decodes by argmax alone. */
+ * when that is 0), zero-filled once; every call leaves it ready for the next, of
+ * this batch or another; calls that may run concurrently need separate ones.
+ * Nothing is allocated: the call can be captured. The reference decodes by
+ * argmax alone. */
 int qk_sample(const float *logits, int64_t rows, int64_t vocabulary, int64_t row_stride,
               const float *temperature, const int32_t *top_k, const float *top_p,
               const float *min_p, const float *uniform, uint32_t *token, float *probability,

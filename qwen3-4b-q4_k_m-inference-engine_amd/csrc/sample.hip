@@ -4,16 +4,17 @@
 // sample_scan_kernel reads every logit once, one workgroup per chunk of a row
 // (2048 or 8192 logits, all in registers): the chunk's maximum; how many
 // logits lie in each of 128 bands below it, a quarter of the temperature wide
-// (at most 1/4), and, where no top-k bounds the kept set, the sum of their
+// (at most 1/5), and, where no top-k bounds the kept set, the sum of their
 // weights; and the logits of the top bands themselves, as many as the row's
 // top-k can take from one chunk. sample_draw_kernel, one workgroup per row,
 // adds the bands up, which gives the band that a filter's border falls into,
 // and then
 //   - where the chunks' lists reach down to that band (the usual filters),
-//     sorts the listed logits and finds everything among them;
+//     ranks the listed logits and finds everything among them;
 //   - without top-k, reads the row once more for the logits of that band
-//     alone, or not at all if there is no border (bare temperature), picks the
-//     drawn token's chunk by the chunks' sums and reads that again;
+//     alone (several workgroups if there are few rows), or not at all if there
+//     is no border (bare temperature), picks the drawn token's chunk by the
+//     chunks' sums and reads that again;
 //   - else (thousands of logits around a border: equal ones, high
 //     temperatures) searches the row digit by digit.
 //
@@ -24,6 +25,8 @@
 // change a result; a chunk whose own maximum is not the row's is weighed by
 // its own and scaled once per band, in 64-bit floating point. Bands only say
 // where to look; no result depends on their width.
+// Measured: one row of 151936, top-k 20 and top-p 0.95: 15 us; 200 rows: greedy 24
+// (5.1 TB/s), top-k 20 38, filters of their own (a fifth without top-k) 89.
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -32,13 +35,15 @@ namespace qk {
 namespace {
 
 constexpr int kThreads = 1024;     // of the draw
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;        // of a digit; of a band, half as many
 constexpr int kScanThreads = 256;
 constexpr int kBands = 128;
 constexpr int kList = 512;         // most listed logits of a chunk
-constexpr int kItems = 8192;       // most logits of a band that the draw holds
+constexpr int kItems = 6144;       // most logits of a band that the draw holds: two workgroups' LDS fits a compute unit
 constexpr int kSorted = 2 * kThreads;
-constexpr int kMostChunks = 2048;
+constexpr int kMostChunk = 8192;   // logits of a chunk
+constexpr int kMostChunks = 2048;  // chunks of a row
+constexpr int kHelped = 128;       // most rows that get more than one draw workgroup
 constexpr int kShift = 44;         // most fraction bits of a weight
 constexpr int kCopies = 16;        // of the scan's bands: a wave's lanes with the same two low bits share one
 constexpr int kCountAt = 54;       // a band's count above its sum: 512 logits of 2^44 stay below 2^54
@@ -55,6 +60,9 @@ struct SamplePlan {
   uint16_t* counts;   // [rows x chunks][kBands]
   uint64_t* weights;  // [rows x chunks][kBands]
   uint64_t* lists;    // [rows x chunks][list]: key << 32 | ~index
+  int32_t helpers;    // draw workgroups a row; above 1:
+  uint32_t* gathered; // [rows][2]: items and workgroups so far, zero between calls
+  uint64_t* items;    // [rows][kItems]
   size_t bytes;
 };
 
@@ -116,7 +124,7 @@ __device__ __forceinline__ int band_of(float v, float top, float scale) {
   const float d = floorf(top * scale) - floorf(v * scale);
   return d < static_cast<float>(kBands - 1) ? static_cast<int>(d) : kBands - 1;  // NaN (of infinities): the last
 }
-__device__ __forceinline__ float band_scale(float heat) { return fmaxf(4.0f / heat, 4.0f); }
+__device__ __forceinline__ float band_scale(float heat) { return fmaxf(4.0f / heat, 5.0f); }
 __device__ __forceinline__ uint64_t item_of(uint32_t key, int index) {
   return static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
 }
@@ -126,8 +134,12 @@ __device__ __forceinline__ void lds_add(uint64_t* p, uint64_t v) {
   atomicAdd(reinterpret_cast<unsigned long long*>(p), static_cast<unsigned long long>(v));
 }
 // Four logits from x[at]; what lies past n reads as -inf.
+template <bool ONCE = false>
 __device__ __forceinline__ f32x4 load_logits(const float* x, int at, int n) {
-  if (at + 4 <= n) return *reinterpret_cast<const f32x4_a4*>(x + at);
+  if (at + 4 <= n) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const f32x4_a4*>(x + at));
+    return *reinterpret_cast<const f32x4_a4*>(x + at);
+  }
   f32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = at + e < n ? x[at + e] : -__builtin_inff();
@@ -162,13 +174,18 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
   const int64_t unit = static_cast<int64_t>(row) * p.chunks + blockIdx.x;
   const float* x = a.logits + row * a.row_stride + lo;
   const int at0 = tid * 4;  // element e of load i is logit lo + at0 + i * 4 * kScanThreads + e
-  f32x4 v[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = load_logits(x, at0 + i * 4 * kScanThreads, n);
   const float heat = a.temperature[row];
   const int k = a.top_k ? a.top_k[row] : 0;
   const bool greedy = !(heat > 0.0f);
   const bool cut = k > 0 && k < a.vocabulary;  // the kept set is bounded: no sums of bands are needed
+  f32x4 v[E];
+  if (E == 8 && (cut || greedy)) {  // large batches: rows that the draw hardly reads again
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = load_logits<true>(x, at0 + i * 4 * kScanThreads, n);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = load_logits(x, at0 + i * 4 * kScanThreads, n);
+  }
   const bool bounded = cut && k <= kScanThreads && !greedy;
   uint32_t* const counts = reinterpret_cast<uint32_t*>(bands);  // of a cut row: [band][4]
   if (cut) {
@@ -325,9 +342,19 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
 }
 
 struct Shared {
-  uint64_t items[kItems];
-  uint64_t bins[kBins];
-  uint64_t sums[kMostChunks];
+  union {
+    uint64_t items[kItems];
+    struct {
+      uint64_t sorted[2][kSorted], ranked[kSorted];  // listed logits by rank, by index; weights by rank
+    };
+    uint64_t bins[kBins];  // of a digit's search
+  };
+  union {
+    struct {
+      uint64_t parts[kThreads], part[kThreads];  // a band's even parts, and the items of one
+    };
+    uint64_t sums[kMostChunks];  // of the chunks' kept logits
+  };
   uint64_t weight[kBands];
   uint32_t count[kBands];  // later its running sums
   // of each chunk: where its bands lie in the row's (kBands: it has none), and
@@ -339,6 +366,7 @@ struct Shared {
   uint64_t above, total;
   uint32_t border, floor_key, n, actives, low, high;
 };
+static_assert(sizeof(Shared) <= 80 * 1024);
 
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
 #pragma unroll
@@ -496,19 +524,19 @@ __device__ void sort_down(uint64_t* items, int n) {
   __syncthreads();
 }
 
-// One pass over the row that appends the logits of `band` to sh.items (more
-// than fit are counted), with the largest and smallest key in sh.high / low.
-__device__ void gather_band(const float* x, int n, int band, float top, float scale, Shared& sh) {
+// One pass over logits [begin, end) of the row (begin a multiple of 4) that puts
+// those of `band` into sh.items, sh.n of them (more than fit are counted).
+__device__ void gather_band(const float* x, int begin, int end, int band, float top, float scale, Shared& sh) {
   const float origin = floorf(top * scale), want = static_cast<float>(band);
   // band_of decided for one band: one subtraction and a comparison where
   // neither infinities nor NaN can be in it
   const bool plain = band < kBands - 1 && fabsf(origin) < __builtin_inff();
-  uint32_t low = 0xFFFFFFFFu, high = 0;
   constexpr int kAhead = 8;  // loads in flight a lane
-  for (int base = static_cast<int>(threadIdx.x) * 4; __any(base < n); base += 4 * kThreads * kAhead) {
+  const int first = begin + static_cast<int>(threadIdx.x) * 4;
+  for (int base = first; __any(base < end); base += 4 * kThreads * kAhead) {
     f32x4 v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = load_logits(x, base + i * 4 * kThreads, n);
+    for (int i = 0; i < kAhead; ++i) v[i] = load_logits(x, base + i * 4 * kThreads, end);
     uint32_t hits = 0;
     if (plain) {
 #pragma unroll
@@ -523,27 +551,59 @@ __device__ void gather_band(const float* x, int n, int band, float top, float sc
           hits |= v[i][e] > -__builtin_inff() && band_of(v[i][e], top, scale) == band ? 1u << (4 * i + e) : 0u;
     }
     uint32_t at = hits ? atomicAdd(&sh.n, static_cast<uint32_t>(__popc(hits))) : 0;
-    for (; hits; hits &= hits - 1, ++at) {  // few: read again, not picked from registers
-      const int bit = __builtin_ctz(hits), index = base + (bit >> 2) * 4 * kThreads + (bit & 3);
-      const uint32_t key = rank_key(x[index]);
-      low = min(low, key);
-      high = max(high, key);
-      if (at < kItems) sh.items[at] = item_of(key, index);
+    for (; hits; hits &= hits - 1, ++at) {  // the places; a register cannot be picked by its number
+      const int bit = __builtin_ctz(hits);
+      if (at < kItems) sh.items[at] = static_cast<uint64_t>(base + (bit >> 2) * 4 * kThreads + (bit & 3));
     }
   }
-  if (high) {
-    atomicMin(&sh.low, low);
-    atomicMax(&sh.high, high);
+  __syncthreads();
+  const int items = min(static_cast<int>(sh.n), kItems);
+  for (int i = static_cast<int>(threadIdx.x); i < items; i += kThreads) {
+    const int index = static_cast<int>(sh.items[i]);
+    sh.items[i] = item_of(rank_key(x[index]), index);
   }
   __syncthreads();
 }
 
-// The draw: a few dependent reads of what the scan left, a sort in LDS and
-// running sums; latency bounds it.
+// The helpers' items together in the last of a row's workgroups to get here,
+// where this is true.
+__device__ bool join_items(const SamplePlan& p, int row, Shared& sh) {
+  uint32_t* const counters = p.gathered + 2 * row;
+  uint64_t* const all = p.items + static_cast<int64_t>(row) * kItems;
+  const int tid = static_cast<int>(threadIdx.x), mine = min(static_cast<int>(sh.n), kItems);
+  if (tid == 0) sh.low = __hip_atomic_fetch_add(counters, static_cast<uint32_t>(mine), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int at = static_cast<int>(sh.low);
+  for (int i = tid; i < mine && at + i < kItems; i += kThreads)
+    __hip_atomic_store(all + at + i, sh.items[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the thread's stores have reached memory
+  __syncthreads();
+  if (tid == 0) {
+    const uint32_t n = __hip_atomic_fetch_add(counters + 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.high = n + 1 == static_cast<uint32_t>(p.helpers);
+    if (sh.high) {
+      sh.n = __hip_atomic_load(counters, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(counters, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(counters + 1, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  __syncthreads();
+  if (!sh.high) return false;
+  const int items = min(static_cast<int>(sh.n), kItems);
+  for (int i = tid; i < items; i += kThreads)
+    sh.items[i] = __hip_atomic_load(all + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return true;
+}
+
+// The draw: a few dependent reads of what the scan left, a ranking in LDS and
+// running sums; latency bounds it: 9 us a row for top-k 20, 13 for 50, 25 for 300;
+// without top-k 14 where the lists reach the border, 33 to 48 where the row is
+// read again (temperature 1.3).
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs a, const SamplePlan p) {
   __shared__ Shared sh;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-  const int row = static_cast<int>(blockIdx.x), n = a.vocabulary;
+  const int row = static_cast<int>(blockIdx.x), helper = static_cast<int>(blockIdx.y), n = a.vocabulary;
   const float* x = a.logits + row * a.row_stride;
   const int64_t unit0 = static_cast<int64_t>(row) * p.chunks;
   const ChunkHead* heads = p.heads + unit0;
@@ -553,8 +613,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   const double share = a.top_p ? static_cast<double>(a.top_p[row]) : 1.0;
   const double floor_w = a.min_p ? static_cast<double>(a.min_p[row]) : 0.0;
   const float uniform = a.uniform[row];
+  // the others only help where a border may lie deep in the row
+  if (helper > 0 && (cut || !(heat > 0.0f) || (!(share < 1.0) && floor_w <= 0.0))) return;
   if (tid < kBands) sh.count[tid] = 0, sh.weight[tid] = 0;
-  if (tid == 0) sh.n = 0, sh.actives = 0, sh.low = 0xFFFFFFFFu, sh.high = 0;
+  if (tid == 0) sh.n = 0, sh.actives = 0;
   // the first of the chunks' counts are on their way before the row's maximum is known
   const int units = p.chunks * (kBands / 8);
   u16x8 counts{};
@@ -576,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   __syncthreads();
   for (int i = 0; i < kThreads / 64; ++i) best = sh.wave[i] > best ? sh.wave[i] : best;
   if (!(heat > 0.0f) || best == 0) {
-    if (tid == 0) {
+    if (tid == 0 && helper == 0) {
       a.token[row] = best ? static_cast<uint32_t>(item_index(best)) : 0xFFFFFFFFu;
       if (a.probability) a.probability[row] = best ? 1.0f : 0.0f;
     }
@@ -694,6 +756,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       sh.active[atomicAdd(&sh.actives, 1u)] = static_cast<uint16_t>(c);
     }
   if (__syncthreads_and(reach)) {
+    if (helper > 0) return;
     // 32 lanes a chunk
     const int actives = static_cast<int>(sh.actives);
     for (int i = tid >> 5; __any(i < actives); i += kThreads / 32) {
@@ -705,7 +768,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
         for (int j = 0; j < 8; ++j) item[j] = at + 32 * j < listed ? list[at + 32 * j] : 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          append(item[j] && band_of(key_value(item_key(item[j])), top_value, scale) <= border, item[j], sh.items, &sh.n, kSorted);
+          append(item[j] && band_of(key_value(item_key(item[j])), top_value, scale) <= border, item[j], sh.sorted[0], &sh.n, kSorted);
       }
     }
     __syncthreads();
@@ -715,7 +778,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       // one wave, an item a lane; what ranks before it and what precedes it in
       // the vocabulary are sums over the others' values, lane by lane
       if (wave != 0) return;
-      const uint64_t item = lane < listed ? sh.items[lane] : 0;
+      const uint64_t item = lane < listed ? sh.sorted[0][lane] : 0;
       const uint64_t f = lane < listed ? w.fixed(item_key(item)) : 0;
       uint64_t before = 0;
       int rank = 0;
@@ -739,18 +802,18 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       if (mine && run > beyond && run - mine <= beyond) answer(item_index(item), mine, total);
       return;
     }
-    sort_down(sh.items, listed);
+    sort_down(sh.sorted[0], listed);
     // ranks 2 tid and 2 tid + 1
     uint64_t mine[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < held ? w.fixed(item_key(sh.items[2 * tid + i])) : 0;
+    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < held ? w.fixed(item_key(sh.sorted[0][2 * tid + i])) : 0;
     if (tid == 0) sh.found[0] = sh.found[1] = 0;
     uint64_t all;
     const uint64_t before = group_prefix(mine[0] + mine[1], all, sh);
     const uint64_t target = share < 1.0 ? target_of(cut ? all : sh.total) : ~uint64_t{0};
     // the kept ones are the first ranks
     const auto stays = [&](int rank, uint64_t ahead) {
-      return rank < held && (rank == 0 || (ahead < target && item_key(sh.items[rank]) >= floor_key));
+      return rank < held && (rank == 0 || (ahead < target && item_key(sh.sorted[0][rank]) >= floor_key));
     };
     const bool stay0 = stays(2 * tid, before), stay1 = stays(2 * tid + 1, before + mine[0]);
     if (!stay0) mine[0] = 0;
@@ -762,19 +825,19 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
                 static_cast<unsigned long long>(before + mine[0] + mine[1]));
     }
     // in the order of the vocabulary
-    uint64_t* order = sh.items + kSorted;
+    uint64_t* order = sh.sorted[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int rank = 2 * tid + i;
-      sh.bins[rank] = mine[i];
-      if (i ? stay1 : stay0) order[rank] = ~(static_cast<uint64_t>(item_index(sh.items[rank])) << 11 | static_cast<uint64_t>(rank));
+      sh.ranked[rank] = mine[i];
+      if (i ? stay1 : stay0) order[rank] = ~(static_cast<uint64_t>(item_index(sh.sorted[0][rank])) << 11 | static_cast<uint64_t>(rank));
     }
     __syncthreads();
     const int kept = static_cast<int>(sh.found[0]);
     const uint64_t total = sh.found[1];
     sort_down(order, kept);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < kept ? sh.bins[~order[2 * tid + i] & (kSorted - 1)] : 0;
+    for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < kept ? sh.ranked[~order[2 * tid + i] & (kSorted - 1)] : 0;
     const uint64_t run = group_prefix(mine[0] + mine[1], all, sh);
     const uint64_t beyond = draw_from(total);
     if (run <= beyond && run + mine[0] + mine[1] > beyond) {
@@ -784,38 +847,55 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     return;
   }
 
+  bool answers = helper == 0;  // or the last of the helpers to arrive
   uint32_t least = 1;
   int last = n;
   const int in_border = border < kBands ? sh.count[border] - (border > 0 ? sh.count[border - 1] : 0) : 0;
   if (!cut && in_border <= kItems) {
     bool done = true;
     int items = 0;
+    if (border == kBands && helper > 0) return;
     if (border < kBands) {
-      gather_band(x, n, border, top_value, scale, sh);
+      const int per = (n + 4 * p.helpers - 1) / (4 * p.helpers) * 4;
+      gather_band(x, helper * per, min(n, helper * per + per), border, top_value, scale, sh);
+      if (p.helpers > 1 && !join_items(p, row, sh)) return;
+      answers = true;
       items = min(static_cast<int>(sh.n), kItems);
       __syncthreads();
       if (border == share_band) {
-        // top-p's border: which of kBins even parts of the band's keys, then the rank in it
-        const uint32_t low = sh.low, high = sh.high;
+        // top-p's border: which of kThreads even parts of the band's keys, then the rank in it
+        uint32_t low = 0xFFFFFFFFu, high = 0;
+        for (int i = tid; i < items; i += kThreads) {
+          low = min(low, item_key(sh.items[i]));
+          high = max(high, item_key(sh.items[i]));
+        }
+        if (tid == 0) sh.low = 0xFFFFFFFFu, sh.high = 0;
+        __syncthreads();
+        if (high) {
+          atomicMin(&sh.low, low);
+          atomicMax(&sh.high, high);
+        }
+        __syncthreads();
+        low = sh.low;
+        high = sh.high;
         int step = 0;
-        while ((high - low) >> step >= static_cast<uint32_t>(kBins)) ++step;
-        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+        while ((high - low) >> step >= static_cast<uint32_t>(kThreads)) ++step;
+        sh.parts[tid] = 0;
         if (tid == 0) sh.n = 0, sh.found[0] = ~uint64_t{0};
         __syncthreads();
         for (int i = tid; i < items; i += kThreads) {
           const uint32_t key = item_key(sh.items[i]);
           const uint64_t f = w.fixed(key);
-          if (f) lds_add(&sh.bins[(high - key) >> step], f);
+          if (f) lds_add(&sh.parts[(high - key) >> step], f);
         }
         __syncthreads();
         const uint64_t target = target_of(sh.total) - sh.above;
-        const uint64_t b0 = sh.bins[2 * tid], b1 = sh.bins[2 * tid + 1];
+        const uint64_t mine_part = sh.parts[tid];
         uint64_t all;
-        const uint64_t before = group_prefix(b0 + b1, all, sh);
-        if (before < target && before + b0 + b1 >= target) {
-          const bool second = before + b0 < target;
-          sh.found[0] = static_cast<uint64_t>(2 * tid + second);
-          sh.found[1] = second ? before + b0 : before;
+        const uint64_t before = group_prefix(mine_part, all, sh);
+        if (before < target && before + mine_part >= target) {
+          sh.found[0] = static_cast<uint64_t>(tid);
+          sh.found[1] = before;
         }
         __syncthreads();
         const bool met = sh.found[0] != ~uint64_t{0};  // else (a rounding short of the band's sum): its last item
@@ -824,14 +904,14 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
         for (int base = 0; base < items; base += kThreads) {
           const int i = base + tid;
           const bool in = i < items && (high - item_key(sh.items[i])) >> step == part;
-          append(in, i < items ? sh.items[i] : 0, sh.sums, &sh.n, kSorted);
+          append(in, i < items ? sh.items[i] : 0, sh.part, &sh.n, kThreads);
         }
         __syncthreads();
         const int listed = static_cast<int>(sh.n);
-        done = listed <= kSorted;
+        done = listed <= kThreads;
         if (listed <= 64) {  // one wave, an item a lane
           if (wave == 0) {
-            const uint64_t item = lane < listed ? sh.sums[lane] : 0;
+            const uint64_t item = lane < listed ? sh.part[lane] : 0;
             const uint64_t f = lane < listed ? w.fixed(item_key(item)) : 0;
             uint64_t run = ahead + f;  // up to and with the lane's, downwards
             for (int i = 0; i < listed; ++i) run += lane_value(item, i) > item ? lane_value(f, i) : 0;
@@ -844,10 +924,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
           }
           __syncthreads();
         } else if (done) {
-          sort_down(sh.sums, listed);
+          sort_down(sh.part, listed);
           uint64_t mine[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < listed ? w.fixed(item_key(sh.sums[2 * tid + i])) : 0;
+          for (int i = 0; i < 2; ++i) mine[i] = 2 * tid + i < listed ? w.fixed(item_key(sh.part[2 * tid + i])) : 0;
           const uint64_t run = ahead + group_prefix(mine[0] + mine[1], all, sh);
           if (tid == 0) sh.found[2] = static_cast<uint64_t>(listed - 1);
           __syncthreads();
@@ -855,7 +935,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
           __syncthreads();
         }
         if (done) {
-          const uint64_t item = sh.sums[sh.found[2]];
+          const uint64_t item = sh.part[sh.found[2]];
           least = item_key(item);
           last = item_index(item);
           __syncthreads();
@@ -900,9 +980,9 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       __syncthreads();
       const int per = p.chunk / kThreads, at = static_cast<int>(sh.found[0]) * p.chunk + tid * per;
       beyond -= sh.found[1];
-      uint64_t mine[kItems / kThreads], sum = 0;
+      uint64_t mine[kMostChunk / kThreads], sum = 0;
 #pragma unroll
-      for (int i = 0; i < kItems / kThreads; ++i) {
+      for (int i = 0; i < kMostChunk / kThreads; ++i) {
         mine[i] = i < per && at + i < n ? kept(rank_key(x[at + i]), at + i) : 0;
         sum += mine[i];
       }
@@ -918,7 +998,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       if (run <= beyond && run + sum > beyond) {
         int i = 0;
 #pragma unroll
-        for (int j = 0; j < kItems / kThreads; ++j)
+        for (int j = 0; j < kMostChunk / kThreads; ++j)
           if (run <= beyond) {
             run += mine[j];
             i = j;
@@ -930,6 +1010,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
   }
 
   // digit by digit
+  if (!answers) return;
   // kept: keys above `least`, and of those equal to it the ones up to index
   // `last`
   if (cut) {
@@ -991,6 +1072,15 @@ SamplePlan plan_sample(int64_t rows, int64_t vocabulary, void* workspace) {
     bytes += (size + 255) & ~size_t{255};
     return part;
   };
+  // the counters first, whatever the batch: no call's lists lie where another's counters are
+  p.gathered = reinterpret_cast<uint32_t*>(take(kHelped * 2 * sizeof(uint32_t)));
+  // One compute unit reads a row of 151936 in 25 us, sixteen in 3: a row's draw
+  // has as many workgroups as leave one a compute unit, 4096 logits each at least
+  // (us, top-p 0.95 at temperature 1.3, with and without: one row 44 and 59; at
+  // 64 rows 74 and 73).
+  const int64_t share = vocabulary / 4096 < 256 / rows ? vocabulary / 4096 : 256 / rows;
+  p.helpers = static_cast<int32_t>(share < 1 ? 1 : share < 16 ? share : 16);
+  if (p.helpers > 1) p.items = reinterpret_cast<uint64_t*>(take(static_cast<size_t>(rows) * kItems * sizeof(uint64_t)));
   p.heads = reinterpret_cast<ChunkHead*>(take(units * sizeof(ChunkHead)));
   p.counts = reinterpret_cast<uint16_t*>(take(units * kBands * sizeof(uint16_t)));
   p.weights = reinterpret_cast<uint64_t*>(take(units * kBands * sizeof(uint64_t)));
@@ -1012,7 +1102,7 @@ hipError_t launch_sample(const SampleArgs& a, void* workspace, hipStream_t strea
     sample_scan_kernel<8><<<grid, kScanThreads, 0, stream>>>(a, p);
   const hipError_t error = hipGetLastError();
   if (error != hipSuccess) return error;
-  sample_draw_kernel<<<a.rows, kThreads, 0, stream>>>(a, p);
+  sample_draw_kernel<<<dim3(static_cast<uint32_t>(a.rows), static_cast<uint32_t>(p.helpers)), kThreads, 0, stream>>>(a, p);
   note("sample_scan_kernel", static_cast<int64_t>(p.chunks) * a.rows, p.chunk);
   return hipGetLastError();
 }

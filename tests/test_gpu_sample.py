@@ -104,6 +104,20 @@ def test_large_batches_of_equal_logits(gpu):
         Sample(gpu, x, 1.0, k, p, min_p, 0.123 + 0.8 * rng.random(110)).run()
 
 
+def test_one_workspace_serves_batches_of_all_sizes(gpu):
+    """Flat and peaked rows, few and many, in turn on the same bytes, zero-filled once."""
+    rng = np.random.default_rng(12)
+    calls = [Sample(gpu, _logits(rng, R, V), heat, k, p, 0.0, rng.random(R))
+             for R, V, heat, k, p in ((1, 151936, 1.4, 0, 0.9), (130, 9000, 1.2, 0, 0.95), (3, 40000, 1.0, 0, 0.8),
+                                      (2, 151936, 0.6, 20, 0.95), (60, 33000, 2.0, 0, 0.97))]
+    ws = gpu.DeviceBuffer.from_array(np.zeros(max(s.ws.nbytes for s in calls), np.uint8))
+    for s in calls:
+        s.ws = ws
+    for s in calls + calls[::-1]:
+        s.token.fill(0xA5)
+        s.run()
+
+
 def test_the_whole_line_of_uniforms(gpu):
     """Uniforms over [0, 1) draw every kept token, in index order."""
     V, R = 130, 400
