@@ -19,10 +19,14 @@ constexpr int64_t kGoodPart = kGoodPartKeys;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
-// Calls too small for a 256-row tile on every unit: up to so many keys, tiles of
-// 64 rows whose waves share the keys are faster than 256-row tiles whose keys
-// workgroups share (us: 512 tokens of 32 heads over 2048 keys 48 against 50, over
-// 4096 keys 91 against 82; four sequences of 128 over 1000 26 against 31).
+// Many rows: the largest tiles that occupy the compute units, 256 rows, or 128 or
+// 64 whose waves share the keys, but that only up to kPartedKeys keys: then
+// 256-row tiles whose keys workgroups share are faster (us: 512 tokens of 32
+// heads over 2048 keys 48 against 50, over 4096 keys 91 against 82; 12 ragged
+// prompts of up to 300, 28 heads, 128-row tiles 32, 64-row ones 36). 128-row tiles
+// also where 256-row ones would be one uneven round: 2048 tokens of a prompt,
+// 256 tiles, 107 against 90; not at 4000 with a window of 1000, 500 tiles, 93
+// against 116.
 constexpr int64_t kPartedKeys = 2048;
 constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
@@ -38,21 +42,31 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   p.few = rows <= 32 * sequences;
   const int waves_rows = 32 * attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
   // every sequence may end in a part of a tile, and none has a tile without a row
-  const auto tiles_of = [&](int tile_rows) {
-    int64_t tiles = rows / tile_rows + sequences;
+  const auto tiles_of = [&](int64_t tile_rows) {
+    int64_t tiles = (rows + sequences * (tile_rows - 1)) / tile_rows;
     if (tiles > rows) tiles = rows;
     if (group <= tile_rows && tiles > tokens) tiles = tokens;
     return tiles;
   };
+  // half a tile a sequence is nearer to what there will be
+  const auto likely_units = [&](int64_t tile_rows) { return (up(rows, tile_rows) + (sequences - 1) / 2) * kv_heads; };
   int64_t keys = max_context < 1 ? 1 : max_context;
   if (window > 0 && keys > window + waves_rows) keys = window + waves_rows;
-  p.parted = !p.few && tiles_of(waves_rows) * kv_heads < kUnits && keys <= kPartedKeys;
-  const int tile_rows = p.few ? 16 : p.parted ? waves_rows / 4 : waves_rows;
+  p.key_groups = 1;
+  if (!p.few && keys <= kPartedKeys && likely_units(waves_rows) < kUnits * 3 / 2)
+    p.key_groups = likely_units(waves_rows / 2) < kUnits * 5 / 8 ? 4 : 2;
+  const int tile_rows = p.few ? 16 : waves_rows / p.key_groups;
   p.rows = tile_rows;
   const int64_t tiles = tiles_of(tile_rows);
   p.tiles = static_cast<int32_t>(tiles);
   const int64_t units = tiles * kv_heads;
-  int64_t splits = up(p.few ? kMostUnits : kUnits, units);
+  // many rows: as many parts as run at once, or a little over (600 tokens over
+  // 4096 keys in three parts 91 us, in four, a second round, 120)
+  int64_t splits = up(kMostUnits, units);
+  if (!p.few) {
+    splits = (10 * kUnits + 3 * likely_units(tile_rows)) / (10 * likely_units(tile_rows));
+    if (splits < 1) splits = 1;
+  }
   p.fill = static_cast<int32_t>(splits);
   if (p.few && splits > 1 && splits < up(keys, kGoodPart)) {
     const int64_t most = up(4 * kMostUnits, units);
@@ -80,7 +94,7 @@ hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, in
   a.sums = reinterpret_cast<float*>(ws + plan.sums_at);
   a.parts = reinterpret_cast<float*>(ws + plan.parts_at);
   return plan.few ? launch_attention_few(a, type, head_dim, q_type, stream)
-                  : launch_attention_many(a, plan.parted, type, head_dim, q_type, stream);
+                  : launch_attention_many(a, plan.key_groups, type, head_dim, q_type, stream);
 }
 
 }  // namespace qk

@@ -9,10 +9,10 @@
 // issued a tile ahead and written to LDS half a tile before its first use,
 // one barrier a tile; three tiles lie in LDS, as the slowest wave may still read
 // the one before while the fastest writes the one after.
-// With KG = 4, for calls of few rows, four waves share 32 rows instead and take
-// 32 keys each of a tile of 128; their parts are joined in LDS. A quarter of the
-// rows a workgroup, but no part in memory where the others need four
-// (plan_attention has the figures).
+// For calls of few rows KG waves share 32 rows instead, 32 keys each of a tile of
+// 64 (KG = 2) or 128 (KG = 4, in two buffers, without the look ahead); their parts
+// are joined in LDS. Fewer rows a workgroup, but no part in memory where the
+// others need it (plan_attention has the figures).
 // Rows of 2 D bytes are stored with their 16-byte chunks permuted by the key
 // (tile_chunk), which keeps both the row reads of K and the transposing reads
 // of V off each other's banks.
@@ -47,13 +47,13 @@ attention_many_kernel(const AttentionArgs a) {
   constexpr int NP = kParts<BF16, Q32>;
   constexpr int kRows = 32 * kWaves / KG;   // rows of a tile
   constexpr int kKeys = KG == 1 ? 64 : 32 * KG;  // keys of a tile in LDS
-  constexpr int kBuffers = KG == 1 ? 3 : 2;
+  constexpr int kBuffers = KG == 4 ? 2 : 3;
   constexpr int KS = D / 16, DT = D / 32;   // k steps of q.k, 32-wide tiles of the output
   constexpr int LPK = D / 8;                // lanes that load one key
   constexpr int KPL = 64 * kWaves / LPK;    // keys a load of the workgroup
   constexpr int NL = kKeys / KPL;           // such loads a tile
   constexpr int kTile = kKeys * 2 * D;      // bytes of a tile's keys, or values
-  constexpr int kRing = KG == 1 ? 8 : 4;    // tiles whose places are kept
+  constexpr int kRing = KG == 4 ? 4 : 8;    // tiles whose places are kept
   struct Shared {
     union {
       struct {
@@ -292,7 +292,7 @@ attention_many_kernel(const AttentionArgs a) {
   };
   // tile n + 1 into LDS, the loads and look-ups after it; then all may read it
   const auto advance = [&](int n, int next) __attribute__((always_inline)) {
-    if constexpr (KG > 1) __syncthreads();  // tile n is there, and all are done with tile n - 1
+    if constexpr (KG == 4) __syncthreads();  // tile n is there, and all are done with tile n - 1
     store(n + 1, next);
     load(n + 2);
     if (looks) {
@@ -300,7 +300,7 @@ attention_many_kernel(const AttentionArgs a) {
       look_up(n + 4);
     }
     if (tid == 0) sh.odd[(n + 2) & 3] = 0;  // read last before the barrier of tile n - 1, set next after the next one
-    if constexpr (KG == 1) __syncthreads();
+    if constexpr (KG != 4) __syncthreads();
   };
 
   int n = 0;
@@ -336,6 +336,24 @@ attention_many_kernel(const AttentionArgs a) {
         };
         while (both(std::integral_constant<int, 0>{}) && both(std::integral_constant<int, 1>{}) &&
                both(std::integral_constant<int, 2>{})) {
+        }
+      }
+      for (; n < count; ++n) advance(n, (n + 1) % 3);
+    } else if constexpr (KG == 2) {
+      __syncthreads();
+      if (end > 0) {
+        f32x16 x0, x1;
+        scores(0, x0);
+        const auto one = [&](auto buffer, f32x16& x, f32x16& y) __attribute__((always_inline)) {
+          constexpr int at = decltype(buffer)::value * kTile, next = (decltype(buffer)::value + 1) % 3;
+          advance(n, next);
+          attend(c.lo + n * kKeys + 32 * part, at, x, next * kTile, &y);
+          if (sh.odd[n & 3]) add_infinite(n);
+          return ++n < end;
+        };
+        while (one(std::integral_constant<int, 0>{}, x0, x1) && one(std::integral_constant<int, 1>{}, x1, x0) &&
+               one(std::integral_constant<int, 2>{}, x0, x1) && one(std::integral_constant<int, 0>{}, x1, x0) &&
+               one(std::integral_constant<int, 1>{}, x0, x1) && one(std::integral_constant<int, 2>{}, x1, x0)) {
         }
       }
       for (; n < count; ++n) advance(n, (n + 1) % 3);
@@ -490,9 +508,11 @@ hipError_t launch_groups(const AttentionArgs& a, int type, int head_dim, int q_t
 
 }  // namespace
 
-hipError_t launch_attention_many(const AttentionArgs& a, bool parted, int type, int head_dim, int q_type,
+hipError_t launch_attention_many(const AttentionArgs& a, int key_groups, int type, int head_dim, int q_type,
                                  hipStream_t stream) {
-  return parted ? launch_groups<4>(a, type, head_dim, q_type, stream) : launch_groups<1>(a, type, head_dim, q_type, stream);
+  return key_groups == 1   ? launch_groups<1>(a, type, head_dim, q_type, stream)
+         : key_groups == 2 ? launch_groups<2>(a, type, head_dim, q_type, stream)
+                           : launch_groups<4>(a, type, head_dim, q_type, stream);
 }
 
 }  // namespace qk

@@ -53,7 +53,7 @@ struct AttentionArgs {
 // How a call is laid out, from host values alone.
 struct AttentionPlan {
   bool few;              // 16-row tiles (paged_attention_few.hip), else 256 or 128 (paged_attention_many.hip)
-  bool parted;           // of the latter: four waves to 32 rows, each a part of the keys (64 or 32-row tiles)
+  int key_groups;        // of the latter: 1, or 2 or 4 waves that share 32 rows, each with a part of the keys
   int rows;              // rows of a tile: (new token, query head of the key/value head)
   int32_t tiles;         // at most so many tiles
   int32_t splits;        // workgroups that may share a tile's keys
@@ -68,7 +68,7 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
 hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, int type, int head_dim, int q_type,
                                   void* workspace, hipStream_t stream);
 hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
-hipError_t launch_attention_many(const AttentionArgs& a, bool parted, int type, int head_dim, int q_type, hipStream_t stream);
+hipError_t launch_attention_many(const AttentionArgs& a, int key_groups, int type, int head_dim, int q_type, hipStream_t stream);
 
 struct SampleArgs {
   const float* logits;
