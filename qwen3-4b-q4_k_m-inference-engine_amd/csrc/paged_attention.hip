@@ -8,13 +8,16 @@ namespace {
 // The card's compute units: a plan, and with it a workspace's size, is the
 // same with and without a device at hand.
 constexpr int64_t kUnits = 256;
-// Single tokens: contexts are cut where there are fewer (tile, head) units than
-// two a compute unit, into parts of kGoodPart keys, or as short as it takes for
-// that many workgroups. Longer parts leave a batch of uneven contexts unbalanced
-// (16 of up to 32768 keys, us: parts of 8192 237, of 2048 190), shorter ones
-// pay for their joining (one of 131072: parts of 2048 116, of 512 195); 64
-// of up to 8192 are not cut: 225, in parts of 2048 235.
+// Single tokens: where there are more (tile, head) units than compute units the
+// contexts stay whole and are taken by length (us: 40 sequences of up to 4000
+// keys 89, cut in two 103). Else they are cut, into parts of kGoodPart keys, or
+// as short as it takes for two workgroups a unit. Longer parts leave a batch of
+// uneven contexts unbalanced (16 of up to 32768 keys: parts of 8192 237, of 2048
+// 187), shorter ones pay for their joining (one of 131072: parts of 2048 102, of
+// 512 136).
 constexpr int64_t kGoodPart = kGoodPartKeys;
+// Ranking the contexts by length costs a few microseconds: from this many keys on.
+constexpr int64_t kOrderedKeys = 1024;
 // Keys are shared out only while a plan has fewer (tile, head) units than this,
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
@@ -62,7 +65,8 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   const int64_t units = tiles * kv_heads;
   // many rows: as many parts as run at once, or a little over (600 tokens over
   // 4096 keys in three parts 91 us, in four, a second round, 120)
-  int64_t splits = up(kMostUnits, units);
+  const bool ordered = p.few && sequences <= kOrdered && keys >= kOrderedKeys && units > kUnits;
+  int64_t splits = ordered ? 1 : up(kMostUnits, units);
   if (!p.few) {
     splits = (10 * kUnits + 3 * likely_units(tile_rows)) / (10 * likely_units(tile_rows));
     if (splits < 1) splits = 1;
@@ -75,6 +79,7 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   const int64_t least = p.few ? 128 : 256;
   if (splits > up(keys, least)) splits = up(keys, least);
   p.splits = static_cast<int32_t>(splits);
+  if (ordered && splits == 1) p.pairs = static_cast<int32_t>(up(kUnits, kv_heads));
   if (splits > 1) {
     const size_t parts = static_cast<size_t>(units * splits * tile_rows);
     p.sums_at = kCounterBytes;
@@ -89,6 +94,7 @@ hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, in
   a.tiles = plan.tiles;
   a.splits = plan.splits;
   a.fill = plan.fill;
+  a.pairs = plan.pairs;
   char* ws = static_cast<char*>(workspace);
   a.arrived = reinterpret_cast<uint32_t*>(ws);
   a.sums = reinterpret_cast<float*>(ws + plan.sums_at);

@@ -24,6 +24,7 @@
 namespace qk {
 
 constexpr int kGoodPartKeys = 2048;  // see plan_attention
+constexpr int kOrdered = 128;        // most sequences that are taken by length
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr float kNoMax = -3.4028234e38f;  // the maximum of no score: no finite score is below it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -121,6 +122,16 @@ struct AttentionTile {
   bool fault;
 };
 
+// The rest of a tile, from its sequence and first row.
+__device__ __forceinline__ void tile_keys(const AttentionArgs& a, int tile_rows, AttentionTile& t) {
+  t.rows = t.count * a.group;
+  const int end = t.begin + tile_rows < t.rows ? t.begin + tile_rows : t.rows;
+  t.key_hi = t.first + (end - 1) / a.group + 1;
+  const int lowest = a.window > 0 ? t.first + t.begin / a.group - a.window + 1 : 0;
+  t.key_lo = lowest > 0 ? lowest : 0;
+  if (t.key_hi < t.key_lo) t.key_hi = t.key_lo;  // positions before 0 see nothing
+}
+
 // Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
 // sums of the tile counts until they pass `tile`.
 __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile, int tile_rows) {
@@ -155,13 +166,7 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
     }
     before += __builtin_amdgcn_readlane(run, 63);
   }
-  if (t.s < 0) return t;
-  t.rows = t.count * a.group;
-  const int end = t.begin + tile_rows < t.rows ? t.begin + tile_rows : t.rows;
-  t.key_hi = t.first + (end - 1) / a.group + 1;
-  const int lowest = a.window > 0 ? t.first + t.begin / a.group - a.window + 1 : 0;
-  t.key_lo = lowest > 0 ? lowest : 0;
-  if (t.key_hi < t.key_lo) t.key_hi = t.key_lo;  // positions before 0 see nothing
+  if (t.s >= 0) tile_keys(a, tile_rows, t);
   return t;
 }
 

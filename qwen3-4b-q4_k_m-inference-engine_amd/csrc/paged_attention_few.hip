@@ -10,8 +10,9 @@
 // wave are in flight under the arithmetic.
 // Loads take whole rows (256 bytes a key, 16 lanes) and are marked as not used
 // again: this card's plain reads reach 6.4 TB/s, those 7.2. 64 sequences of up to
-// 8192 keys, 1.06 GB: 225 us (4.7 TB/s); 263 with keys loaded straight into the
-// operand's layout (64 bytes of a row an instruction); 3 of 131072: 167 (5.2).
+// 8192 keys, 1.06 GB: 175 us (6.1 TB/s), 3 of 131072: 154 (5.7); before the
+// sequences were taken by length 225, and 263 with keys loaded straight into the
+// operand's layout (64 bytes of a row an instruction).
 #include "paged_attention.hpp"
 
 namespace qk {
@@ -31,6 +32,52 @@ __device__ __forceinline__ int v_chunk(int key, int chunk) {
 template <int D>
 __device__ __forceinline__ int k_chunk(int key, int chunk) {
   return key * (2 * D) + ((chunk ^ (D == 128 ? key & 15 : key >> 1 & 7)) << 4);
+}
+
+// Tiles by the length of their sequences' contexts, where no sequence has more
+// than one (false otherwise): the `pairs` longest in the first round of
+// workgroups, one a compute unit, the next ones in the second, which the card
+// places on the same units in the same order, from the shortest up; then the
+// rest. Each unit's two contexts so have about the same length together: 64
+// sequences of up to 8192 keys, uneven, 225 us as they come, 175 paired. Every
+// workgroup ranks the lengths itself, a thread a sequence.
+__device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile, int32_t (&keys)[kOrdered], int32_t& chosen,
+                                               AttentionTile& t) {
+  const int s = static_cast<int>(threadIdx.x);
+  int mine = -1;
+  bool single = true;
+  if (s < a.kv.sequences) {
+    const KvSequence q = kv_sequence(a.kv, s);
+    single = q.count * a.group <= kRows;
+    if (q.count > 0) {
+      mine = q.first + q.count;
+      mine = mine < 0 ? 0 : a.window > 0 && mine > a.window ? a.window : mine;
+    }
+  }
+  if (s < kOrdered) keys[s] = mine;
+  if (s == 0) chosen = -1;
+  const int tiles = __syncthreads_count(mine >= 0);
+  if (!__syncthreads_and(single)) return false;
+  int rank = 0;
+  for (int i = 0; i < a.kv.sequences; i += 4) {
+    const i32x4 other = *reinterpret_cast<const i32x4*>(&keys[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rank += other[e] > mine || (other[e] == mine && i + e < s);
+  }
+  const int second = 2 * a.pairs < tiles ? 2 * a.pairs : tiles;
+  const int wanted = tile < a.pairs || tile >= second ? tile : second - 1 - (tile - a.pairs);
+  if (mine >= 0 && rank == wanted) chosen = s;
+  __syncthreads();
+  t.s = __builtin_amdgcn_readfirstlane(chosen);
+  if (t.s < 0) return true;
+  const KvSequence q = kv_sequence(a.kv, t.s);
+  t.row = q.row;
+  t.count = q.count;
+  t.first = q.first;
+  t.fault = q.fault;
+  t.begin = 0;
+  tile_keys(a, kRows, t);
+  return true;
 }
 
 template <int D, bool BF16, bool Q32>
@@ -53,6 +100,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     };
     int64_t place[kWaves][2][kBlock];
     float top[kWaves][kRows], sum[kWaves][kRows];
+    __attribute__((aligned(16))) int32_t keys[kOrdered];
+    int32_t chosen;
     uint32_t bad, arrived;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
@@ -60,7 +109,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
   const int tile = unit / a.splits, split = unit % a.splits;
-  const AttentionTile t = find_tile(a, tile, kRows);
+  AttentionTile t;
+  if (a.pairs == 0 || !find_by_length(a, tile, sh.keys, sh.chosen, t)) t = find_tile(a, tile, kRows);
   if (t.s < 0) return;
   // chunks of one length for all sequences, so that a batch's longest does not outlast the rest
   int chunk = kStep;
@@ -231,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
 
     // values into LDS; those of keys past the end as zeros (their weight is 0)
     bool odd = false;
-    if (!whole) {
+    if (!whole || NP > 1) {  // a weight's parts may be of either sign, or nothing
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
         if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};

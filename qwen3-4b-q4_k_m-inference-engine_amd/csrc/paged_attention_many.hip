@@ -165,12 +165,13 @@ attention_many_kernel(const AttentionArgs a) {
     }
   };
   // registers -> LDS; values of keys past the end become zeros, and where some
-  // row does not see some key, so do infinite ones (odd)
+  // row does not see some key, or its weight has parts (of either sign, or
+  // none), so do infinite ones (odd)
   const auto store = [&](int n, int buffer) {
     if (n >= count) return;
     const int key0 = c.lo + n * kKeys;
     const bool edge = !(key0 + kKeys - 1 <= tile_last && key0 + kKeys <= c.hi && key0 >= tile_from);
-    if (edge) {
+    if (edge || NP > 1) {
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {

@@ -45,6 +45,7 @@ struct AttentionArgs {
   float* lse;
   // the plan's part (launch_paged_attention)
   int32_t tiles, splits, fill;
+  int32_t pairs;      // tiles of a round of workgroups, one a compute unit, if sequences are taken by length; else 0
   uint32_t* arrived;  // [tiles x kv_heads], zero between calls
   float* sums;        // [tiles x kv_heads x splits x rows] (maximum, sum) pairs
   float* parts;       // [tiles x kv_heads x splits x rows x head_dim]
@@ -58,6 +59,7 @@ struct AttentionPlan {
   int32_t tiles;         // at most so many tiles
   int32_t splits;        // workgroups that may share a tile's keys
   int32_t fill;          // so many of them fill the card
+  int32_t pairs;         // see AttentionArgs
   size_t sums_at, parts_at, bytes;  // workspace; 0 bytes without splits
 };
 // Waves of a workgroup of paged_attention_many.hip, 32 rows each: eight, but

@@ -251,6 +251,104 @@ def test_one_workspace_serves_batches_of_all_sizes(gpu):
         a.check()
 
 
+# The layouts that large calls take, at sizes that can be checked: a bound on the
+# context above 2048 gives 256-row tiles (their keys in parts where there are
+# few), 160 (tile, head) units of 128 rows give those.
+LAYOUTS = {"wide": dict(max_context=4000), "wide-whole": dict(max_context=2100, kv_heads=96),
+           "pairs": dict(max_context=400, kv_heads=80)}
+
+
+def _layout(name, new, contexts, seed, **more):
+    """A batch in that layout: group 1 where it takes many heads, else 4."""
+    layout = dict(LAYOUTS[name])
+    bound = layout.pop("max_context")
+    heads = layout.pop("kv_heads", 2)
+    q_heads = heads if heads > 2 else 8
+    return Paged(new, contexts, kv_heads=heads, seed=seed, **more), q_heads, bound
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_layouts_of_large_calls(gpu, layout, types, dim):
+    kind, q_type = TYPES[types]
+    for new, contexts, window in (([100, 33, 0, 1], [700, 40, 9, 300], 0), ([90, 60], [400, 130], 70)):
+        print(f"[case] attention {layout} {types} dim={dim} window={window}", flush=True)
+        p, q_heads, bound = _layout(layout, new, contexts, dim, kind=kind, dim=dim, page=24, gaps=(1, 2))
+        a = Attend(gpu, p, q_heads, q_type=q_type, max_context=bound, window=window)
+        a.call()
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_masked_places_in_layouts_of_large_calls(gpu, layout, types):
+    """NaN and infinities in unused slots, in later positions and in one value that some rows see."""
+    kind, q_type = TYPES[types]
+    p, q_heads, bound = _layout(layout, [120, 80], [120, 333], 5, kind=kind, dim=64)
+    used = np.zeros((p.pages, p.page), bool)
+    for s, c in enumerate(p.contexts):
+        used[p.table[s, np.arange(c) // p.page], np.arange(c) % p.page] = True
+    for pool, value in ((p.k, np.nan), (p.v, np.inf)):
+        p.seen(pool)[~used] = ref.encode(value, kind)
+    a = Attend(gpu, p, q_heads, q_type=q_type, max_context=bound)
+    a.call()
+    gpu.synchronize()
+    a.check()
+    p.seen(p.v)[p.table[0, 3], 2, :, 7] = ref.encode(np.inf, kind)  # position 50
+    p.seen(p.k)[p.table[0, 119 // 16], 119 % 16, :, 3] = ref.encode(np.nan, kind)
+    p.dev["k"].upload(p.k)
+    p.dev["v"].upload(p.v)
+    a.call()
+    gpu.synchronize()
+    out = ref.decode(a.results()[0], q_type)[:119]
+    assert np.isfinite(out[:50]).all() and np.isfinite(np.delete(out, 7, axis=2)).all()
+    assert (out[50:, :, 7] == np.inf).all()
+    a.check(sequences=(1,))
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_scales_of_either_sign_and_zero(gpu, types):
+    kind, q_type = TYPES[types]
+    for new, contexts, bound in (([1, 2], [300, 70], 300), ([70], [130], 130), ([70], [130], 4000)):
+        for scale in (-0.11, 0.0):
+            p = Paged(new, contexts, kind=kind, dim=64, seed=6)
+            a = Attend(gpu, p, 4, q_type=q_type, scale=scale, max_context=bound)
+            a.call()
+            gpu.synchronize()
+            a.check()
+
+
+@pytest.mark.parametrize("types", ["f16-f32", "bf16-bf16"])
+@pytest.mark.parametrize("case", ["singles", "drafts", "window", "misfit"])
+def test_batches_that_are_taken_by_length(gpu, case, types):
+    """Many sequences of uneven contexts, some without a new token; drafts of
+    two tiles (then in their own order); a context shorter than its new tokens."""
+    kind, q_type = TYPES[types]
+    rng = np.random.default_rng(21)
+    new = [0 if i % 9 == 4 else 1 for i in range(70)]
+    contexts = [int(c) for c in rng.integers(1, 260, 70)]
+    contexts[5] = contexts[33] = 1300  # equal lengths rank by their order
+    q_heads = 8
+    if case == "drafts":
+        new = [3 * n for n in new]
+        new[2], q_heads = 9, 8  # 18 rows: two tiles
+    contexts = [max(c, n) for c, n in zip(contexts, new)]
+    if case == "misfit":
+        new[7], contexts[7] = 2, 1
+    p = Paged(new, contexts, kv_heads=4, dim=64, kind=kind, seed=22, gaps=(2, 1))
+    a = Attend(gpu, p, q_heads, q_type=q_type, window=90 if case == "window" else 0, max_context=1300)
+    print(f"[case] attention by length {case} {types}", flush=True)
+    a.call()
+    gpu.synchronize()
+    if case == "misfit":
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        p.dev["fault"].upload(np.zeros(1, np.uint32))
+    a.check()
+
+
 def test_bad_pages_are_reported_and_reach_no_other_sequence(gpu):
     for new, contexts in (([1, 1, 1], [40, 40, 40]), ([30, 30, 30], [40, 40, 40])):
         p = Paged(new, contexts, page=8, dim=128, seed=16)
