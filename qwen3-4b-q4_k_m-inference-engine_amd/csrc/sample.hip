@@ -60,7 +60,7 @@ struct SamplePlan {
   ChunkHead* heads;   // [rows x chunks]
   uint16_t* counts;   // [rows x chunks][kBands]
   uint64_t* weights;  // [rows x chunks][kBands]
-  uint64_t* lists;    // [rows x chunks][list]: key << 32 | ~index
+  uint64_t* lists;    // [rows x chunks][list]: key << 32 | ~index, by band
   int32_t helpers;    // draw workgroups a row; above 1:
   uint32_t* gathered; // [rows][2]: items and workgroups so far, zero between calls
   uint64_t* items;    // [rows][kItems]
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
   static_assert(E <= 8 && kScanThreads / 64 * 4 == kCopies && 16 * E * 4 <= 512);
   __shared__ uint64_t bands[kBands * kCopies];
   __shared__ float tops[kScanThreads / 64], groups[kScanThreads];
-  __shared__ uint32_t first, listed;
+  __shared__ uint32_t first, places[kBands];  // where a band's next listed logit goes
   __shared__ int32_t depth;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int row = static_cast<int>(blockIdx.y), lo = static_cast<int>(blockIdx.x) * p.chunk;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
   } else if (!greedy) {
     for (int i = tid; i < kBands * kCopies; i += kScanThreads) bands[i] = 0;
   }
-  if (tid == 0) first = 0xFFFFFFFFu, listed = 0;
+  if (tid == 0) first = 0xFFFFFFFFu;
   float mine = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < E; ++i)
@@ -316,6 +316,8 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
       const uint32_t other = __shfl_up(run, off);
       if (lane >= off) run += other;
     }
+    places[2 * lane] = run - c[1] - c[0];
+    places[2 * lane + 1] = run - c[1];
     // as many bands as hold what the row may need of this chunk, and as the list holds
     const uint32_t want = cut ? k : kFew, most = p.list;
     const int enough = __popcll(__ballot(run - c[1] < want)) + __popcll(__ballot(run < want)) + 1;
@@ -338,7 +340,10 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
   }
   uint64_t* list = p.lists + unit * p.list;
   each([&](bool in, float z, int at) {
-    append(in && band_of(z, top, scale) < through, item_of(rank_key(z), lo + at), list, &listed, p.list);
+    const int band = band_of(z, top, scale);
+    if (!in || band >= through) return;
+    const uint32_t to = atomicAdd(&places[band], 1u);
+    if (to < static_cast<uint32_t>(p.list)) list[to] = item_of(rank_key(z), lo + at);
   });
 }
 
@@ -797,19 +802,23 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     }
   if (__syncthreads_and(reach)) {
     if (helper > 0) return;
-    // 32 lanes a chunk
+    // 8 to 512 lanes a chunk, each until its items are past the border: one step for most
     const int actives = static_cast<int>(sh.actives);
-    for (int i = tid >> 5; __any(i < actives); i += kThreads / 32) {
-      const int c = i < actives ? sh.active[i] : 0, listed = i < actives ? sh.listed[c] : 0;
+    int lanes = 512;
+    while (lanes > 8 && lanes * actives > kThreads) lanes >>= 1;
+    for (int i = tid / lanes; i < actives; i += kThreads / lanes) {
+      const int c = sh.active[i], listed = sh.listed[c];
       const uint64_t* list = p.lists + (unit0 + c) * p.list;
-      for (int at = lane & 31; __any(at < listed); at += 32 * 8) {
+      bool more = true;
+      for (int at = tid & (lanes - 1); more && at < listed; at += lanes * 8) {
         uint64_t item[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) item[j] = at + 32 * j < listed ? list[at + 32 * j] : 0;
+        for (int j = 0; j < 8; ++j) item[j] = at + lanes * j < listed ? list[at + lanes * j] : 0;
         uint32_t hits = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           hits |= item[j] && band_of(key_value(item_key(item[j])), top_value, scale) <= border ? 1u << j : 0u;
+        more = hits >> 7;
         uint32_t to = hits ? atomicAdd(&sh.n, static_cast<uint32_t>(__popc(hits))) : 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
