@@ -125,7 +125,10 @@ __device__ __forceinline__ int band_of(float v, float top, float scale) {
   const float d = floorf(top * scale) - floorf(v * scale);
   return d < static_cast<float>(kBands - 1) ? static_cast<int>(d) : kBands - 1;  // NaN (of infinities): the last
 }
-__device__ __forceinline__ float band_scale(float heat) { return fmaxf(4.0f / heat, 5.0f); }
+// A fifth wide where top-k bounds the kept set and only ranks matter (its border
+// then lies in a band for logits up to 25 below the maximum), else a quarter of
+// the temperature at most.
+__device__ __forceinline__ float band_scale(float heat, bool cut) { return cut ? 5.0f : fmaxf(4.0f / heat, 5.0f); }
 __device__ __forceinline__ uint64_t item_of(uint32_t key, int index) {
   return static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
 }
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
     if (tid == 0) p.heads[unit] = ChunkHead{top_key, first, 0, 0};
     return;
   }
-  const float scale = band_scale(heat);
+  const float scale = band_scale(heat, cut);
   // the lane's logits to count or to list: bit 4 i + e
   uint32_t some = 0;
   const auto each = [&](auto visit) {  // few: read again, not picked from registers
@@ -690,7 +693,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     return;
   }
   const uint32_t top = item_key(best);
-  const float top_value = key_value(top), scale = band_scale(heat);
+  const float top_value = key_value(top), scale = band_scale(heat, cut);
   const Weigher w = weigher(top, heat, p.shift);
 
   for (int c = tid; c < p.chunks; c += kThreads) {
