@@ -1177,10 +1177,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
       __syncthreads();
       const int per = p.chunk / kThreads, at = static_cast<int>(sh.found[0]) * p.chunk + tid * per;
       beyond -= sh.found[1];
+      f32x4 v[kMostChunk / kThreads / 4];
+#pragma unroll
+      for (int i = 0; i < kMostChunk / kThreads / 4; ++i) v[i] = load_logits(x, at + 4 * i, 4 * i < per ? n : 0);
       uint64_t mine[kMostChunk / kThreads], sum = 0;
 #pragma unroll
       for (int i = 0; i < kMostChunk / kThreads; ++i) {
-        mine[i] = i < per && at + i < n ? kept(rank_key(x[at + i]), at + i) : 0;
+        mine[i] = i < per ? kept(rank_key(v[i / 4][i % 4]), at + i) : 0;
         sum += mine[i];
       }
       uint64_t all;
