@@ -335,8 +335,9 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
 #pragma unroll
   for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&sh.o[wave][col][16 * d + 4 * grp]) = o[d];
   __syncthreads();
-  constexpr int E = D / 16;  // values a thread: 16 threads a row
-  const int r = tid >> 4, e0 = (tid & 15) * E;
+  constexpr int E = D / 16;  // values a thread: 16 threads a row, pairs 32 apart, so that a row's threads read and write 128 bytes in one
+  const int r = tid >> 4, e0 = (tid & 15) * 2;
+  const auto pair = [&](int i) { return e0 + 16 * i; };  // of values i and i + 1
   const bool mine = t.begin + r < t.rows;
   float all = kNoMax, total = 0.0f, y[E] = {};
 #pragma unroll
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     const float f = __builtin_amdgcn_exp2f(sh.top[w][r] - all);
     total += f * sh.sum[w][r];
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] += f * sh.o[w][r][e0 + i];
+    for (int i = 0; i < E; ++i) y[i] += f * sh.o[w][r][pair(i & ~1) + (i & 1)];
   }
   if (sh.bad) {
     total = __builtin_nanf("");
@@ -358,42 +359,60 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       const int64_t at = (slot + split) * kRows + r;
       if ((tid & 15) == 0) put(a.sums + 2 * at, all, total);
 #pragma unroll
-      for (int i = 0; i < E; i += 2) put(a.parts + at * D + e0 + i, y[i], y[i + 1]);
+      for (int i = 0; i < E; i += 2) put(a.parts + at * D + pair(i), y[i], y[i + 1]);
     }
     if (!last_to_arrive(a.arrived + static_cast<int64_t>(tile) * a.kv.kv_heads + head, c.used, sh.arrived)) return;
     if (mine) {
-      // lane j of a row's 16 has the sums of parts j, j + 16, ..
+      // lane j of a row's 16 has the sums of parts j, j + 16, .. of each 64
       const int j = tid & 15;
       all = kNoMax;
-      for (int k = j; k < c.used; k += 16) {
-        float m, l;
-        get(a.sums + 2 * ((slot + k) * kRows + r), m, l);
-        all = fmaxf(all, m);
-      }
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) all = fmaxf(all, __shfl_xor(all, off));
       total = 0.0f;
 #pragma unroll
       for (int i = 0; i < E; ++i) y[i] = 0.0f;
-      for (int base = 0; base < c.used; base += 16) {
-        float m = kNoMax, l = 0.0f;
-        if (base + j < c.used) get(a.sums + 2 * ((slot + base + j) * kRows + r), m, l);
-        const float f = __builtin_amdgcn_exp2f(m - all);
-        total += f * l;
-        const int some = c.used - base < 16 ? c.used - base : 16;
-        for (int k0 = 0; k0 < some; k0 += 8) {
+      float next[8][E];
+      const auto fetch = [&](int k0) {  // eight parts; past the last that one again, not added
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float* part = a.parts + ((slot + min(k0 + k, c.used - 1)) * kRows + r) * D;
+#pragma unroll
+          for (int i = 0; i < E; i += 2) get(part + pair(i), next[k][i], next[k][i + 1]);
+        }
+      };
+      for (int base = 0; base < c.used; base += 64) {
+        float m[4], l[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) get(a.sums + 2 * ((slot + min(base + 16 * n + j, c.used - 1)) * kRows + r), m[n], l[n]);
+        fetch(base);
+        float to = all;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) to = fmaxf(to, m[n]);
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) to = fmaxf(to, __shfl_xor(to, off));
+        const float f = __builtin_amdgcn_exp2f(all - to);
+        all = to;
+        total *= f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] *= f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          m[n] = __builtin_amdgcn_exp2f(m[n] - all);
+          total += base + 16 * n + j < c.used ? m[n] * l[n] : 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int k0 = base + 8 * n;
+          if (k0 >= c.used) break;
           float part[8][E];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {  // past the last part: that one again, with no weight
-            const int64_t at = (slot + base + min(k0 + k, some - 1)) * kRows + r;
+          for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int i = 0; i < E; i += 2) get(a.parts + at * D + e0 + i, part[k][i], part[k][i + 1]);
-          }
+            for (int i = 0; i < E; ++i) part[k][i] = next[k][i];
+          if (n < 7 && k0 + 8 < c.used) fetch(k0 + 8);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float g = __shfl(f, (tid & 48) + min(k0 + k, 15));
+            const float g = __shfl(m[n / 2], (tid & 48) + 8 * (n & 1) + k);
 #pragma unroll
-            for (int i = 0; i < E; ++i) y[i] += k0 + k < some ? g * part[k][i] : 0.0f;
+            for (int i = 0; i < E; ++i) y[i] += k0 + k < c.used ? g * part[k][i] : 0.0f;
           }
         }
       }
@@ -406,15 +425,16 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int64_t at = static_cast<int64_t>(t.row + out_row / a.group) * a.q_heads + head * a.group + out_row % a.group;
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   if constexpr (Q32) {
-    float* out = static_cast<float*>(a.out) + at * D + e0;
+    typedef float F2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<f32x4*>(out + i) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]} * inv;
+    for (int i = 0; i < E; i += 2)
+      *reinterpret_cast<F2*>(static_cast<float*>(a.out) + at * D + pair(i)) = F2{y[i] * inv, y[i + 1] * inv};
   } else {
-    typedef T TE __attribute__((ext_vector_type(E)));
-    TE v;
+    typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = static_cast<T>(y[i] * inv);
-    *reinterpret_cast<TE*>(static_cast<T*>(a.out) + at * D + e0) = v;
+    for (int i = 0; i < E; i += 2)
+      *reinterpret_cast<T2*>(static_cast<T*>(a.out) + at * D + pair(i)) =
+          T2{static_cast<T>(y[i] * inv), static_cast<T>(y[i + 1] * inv)};
   }
   if (a.lse && (tid & 15) == 0) a.lse[at] = row_lse(all, total);
 }
