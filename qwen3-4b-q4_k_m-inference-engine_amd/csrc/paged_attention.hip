@@ -15,7 +15,17 @@ constexpr int64_t kUnits = 256;
 // uneven contexts unbalanced (16 of up to 32768 keys: parts of 8192 237, of 2048
 // 187), shorter ones pay for their joining (one of 131072: parts of 2048 102, of
 // 512 136).
+// So are contexts that a sequence's several tiles keep from being taken by length (24
+// sequences of up to 10 new tokens and 10000 keys: whole 186, in parts 125; of up
+// to 4000 103 and 75).
 constexpr int64_t kGoodPart = kGoodPartKeys;
+// Up to four 16-row tiles a sequence, HBM and the joining still bound the
+// kernel for few rows, and it is ahead of the other with its large tiles (us, 16
+// new tokens of 32 heads over 8: 4000 keys 24.5 and 29.6, three such sequences 27.6
+// and 44.6; a bfloat16 cache, 12 of them, 62 and 107); but with q of the cache's type the
+// other one's products cost half, and more than a few sequences occupy the card in it
+// (12 of up to 30 tokens and 4000 keys: 73 and 62).
+constexpr int64_t kAlone = 4;
 // Ranking the contexts by length costs a few microseconds: from this many keys on.
 constexpr int64_t kOrderedKeys = 1024;
 // Keys are shared out only while a plan has fewer (tile, head) units than this,
@@ -42,7 +52,7 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   AttentionPlan p{};
   if (tokens == 0 || sequences == 0) return p;
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
-  p.few = rows <= 32 * sequences;
+  p.few = rows <= (q_type == QK_TYPE_F32 || sequences <= kAlone ? 64 : 32) * sequences;
   const int waves_rows = 32 * attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
   // every sequence may end in a part of a tile, and none has a tile without a row
   const auto tiles_of = [&](int64_t tile_rows) {
@@ -65,14 +75,15 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
   const int64_t units = tiles * kv_heads;
   // many rows: as many parts as run at once, or a little over (600 tokens over
   // 4096 keys in three parts 91 us, in four, a second round, 120)
-  const bool ordered = p.few && sequences <= kOrdered && keys >= kOrderedKeys && units > kUnits;
-  int64_t splits = ordered ? 1 : up(kMostUnits, units);
+  const bool whole = p.few && keys >= kOrderedKeys && units > kUnits;
+  const bool ordered = whole && rows <= 16 * sequences && sequences <= kOrdered;  // else some sequence has two tiles
+  int64_t splits = whole ? 1 : up(kMostUnits, units);
   if (!p.few) {
     splits = (10 * kUnits + 3 * likely_units(tile_rows)) / (10 * likely_units(tile_rows));
     if (splits < 1) splits = 1;
   }
   p.fill = static_cast<int32_t>(splits);
-  if (p.few && splits > 1 && splits < up(keys, kGoodPart)) {
+  if (p.few && !ordered && units <= kMostUnits && splits < up(keys, kGoodPart)) {
     const int64_t most = up(4 * kMostUnits, units);
     splits = up(keys, kGoodPart) < most ? up(keys, kGoodPart) : most;
   }
