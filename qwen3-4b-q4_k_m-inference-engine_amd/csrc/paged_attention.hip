@@ -32,18 +32,62 @@ constexpr int64_t kOrderedKeys = 1024;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
-// Many rows: the largest tiles that occupy the compute units, 256 rows, or 128 or
-// 64 whose waves share the keys, but that only up to kPartedKeys keys: then
-// 256-row tiles whose keys workgroups share are faster (us: 512 tokens of 32
-// heads over 2048 keys 48 against 50, over 4096 keys 91 against 82; 12 ragged
-// prompts of up to 300, 28 heads, 128-row tiles 32, 64-row ones 36). 128-row tiles
-// also where 256-row ones would be one uneven round: 2048 tokens of a prompt,
-// 256 tiles, 107 against 90; not at 4000 with a window of 1000, 500 tiles, 93
-// against 116.
-constexpr int64_t kPartedKeys = 2048;
 constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Many rows: waves to a row (its keys shared among them, in tiles of 256, 128 or
+// 64 rows; half as many with q in three parts) and workgroups to a tile's keys. Each
+// has its price, so the pair is taken whose estimated time is least:
+//   - the compute units' work, in keys: the longest workgroup's, or all of it
+//     spread evenly, or as many of the shortest as one unit gets;
+//   - times a tile's time a key, which a smaller tile has less than its
+//     share of; and each workgroup's start;
+//   - the parts' way through memory, and the launch that joins them.
+// The constants order the pairs rather than tell the time. They are fitted to 368
+// calls (20 to 12000 keys, 64 to 4095 new tokens a sequence, 1 to 12
+// sequences, windows, all types, both head dimensions) with up to 28 pairs each: the
+// pair taken is 1.8% behind the best one in the mean; the largest tiles that
+// occupy the card, sharing keys up to 2048 keys, and else as many parts as run at
+// once, were 7.5% behind (1500 tokens with a window of 1000: 95 us and now 72; 1373
+// over 2380 keys, 28 heads over 4: 126 and 103).
+struct ManyRows {
+  int64_t rows, tokens, sequences, kv_heads, group, window, max_context;
+  int tile_rows, head_dim, parts;
+
+  // half a tile a sequence is nearer to what there will be than a whole one
+  int64_t likely_units(int64_t of_rows) const { return (up(rows, of_rows) + (sequences - 1) / 2) * kv_heads; }
+  double time(int key_groups, int64_t splits) const {
+    const int64_t of_rows = tile_rows / key_groups, seen = window + of_rows / group + 1;
+    const bool bounded = window > 0 && max_context > seen;
+    const int64_t most = bounded ? seen : max_context, early = max_context - up(tokens, sequences);
+    const int64_t least = bounded ? seen : early < 64 ? 64 : early;
+    const auto of_part = [&](int64_t keys) {
+      const int64_t step = splits > 1 ? 256 : key_groups == 4 ? 128 : 64;
+      return static_cast<double>(up(up(keys, splits), step) * step);
+    };
+    const int64_t units = likely_units(of_rows) * splits;
+    const double even = 1.03 * units / kUnits * (of_part(most) + of_part(least)) / 2;
+    double keys = of_part(most);
+    if (keys < even) keys = even;
+    if (keys < up(units, kUnits) * of_part(least)) keys = up(units, kUnits) * of_part(least);
+    const double share = key_groups == 1 ? 1.0 : key_groups == 2 ? (parts == 3 ? 0.71 : 0.76) : parts == 3 ? 0.53 : 0.49;
+    const double key = (parts == 3 ? 0.09 : 0.04) * (head_dim == 128 ? 1.0 : 0.64) * share;
+    const double rounds = units > kUnits ? 1.0 * units / kUnits : 1.0;
+    return key * keys + 1.5 * rounds + (splits > 1 ? 6.5 + 2.2e-6 * units * of_rows * head_dim : 0.0);
+  }
+  void choose(int& key_groups, int64_t& splits) const {
+    double best = 1e30;
+    for (int groups = 1; groups <= 4; groups *= 2)
+      for (int64_t parts_of = 1; parts_of <= 24 && (parts_of == 1 || parts_of <= up(max_context, 256)); ++parts_of) {
+        const double t = time(groups, parts_of);
+        if (t >= best) continue;
+        best = t;
+        key_groups = groups;
+        splits = parts_of;
+      }
+  }
+};
 
 }  // namespace
 
@@ -61,27 +105,22 @@ AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads,
     if (group <= tile_rows && tiles > tokens) tiles = tokens;
     return tiles;
   };
-  // half a tile a sequence is nearer to what there will be
-  const auto likely_units = [&](int64_t tile_rows) { return (up(rows, tile_rows) + (sequences - 1) / 2) * kv_heads; };
   int64_t keys = max_context < 1 ? 1 : max_context;
   if (window > 0 && keys > window + waves_rows) keys = window + waves_rows;
   p.key_groups = 1;
-  if (!p.few && keys <= kPartedKeys && likely_units(waves_rows) < kUnits * 3 / 2)
-    p.key_groups = likely_units(waves_rows / 2) < kUnits * 5 / 8 ? 4 : 2;
+  int64_t splits = 1;
+  if (!p.few)
+    ManyRows{rows, tokens, sequences, kv_heads, group, window, max_context < 1 ? 1 : max_context, waves_rows, head_dim,
+             q_type == QK_TYPE_F32 ? (type == QK_TYPE_BF16 ? 3 : 2) : 1}
+        .choose(p.key_groups, splits);
   const int tile_rows = p.few ? 16 : waves_rows / p.key_groups;
   p.rows = tile_rows;
   const int64_t tiles = tiles_of(tile_rows);
   p.tiles = static_cast<int32_t>(tiles);
   const int64_t units = tiles * kv_heads;
-  // many rows: as many parts as run at once, or a little over (600 tokens over
-  // 4096 keys in three parts 91 us, in four, a second round, 120)
   const bool whole = p.few && keys >= kOrderedKeys && units > kUnits;
   const bool ordered = whole && rows <= 16 * sequences && sequences <= kOrdered;  // else some sequence has two tiles
-  int64_t splits = whole ? 1 : up(kMostUnits, units);
-  if (!p.few) {
-    splits = (10 * kUnits + 3 * likely_units(tile_rows)) / (10 * likely_units(tile_rows));
-    if (splits < 1) splits = 1;
-  }
+  if (p.few) splits = whole ? 1 : up(kMostUnits, units);
   p.fill = static_cast<int32_t>(splits);
   if (p.few && !ordered && units <= kMostUnits && splits < up(keys, kGoodPart)) {
     const int64_t most = up(4 * kMostUnits, units);
