@@ -251,9 +251,8 @@ def test_one_workspace_serves_batches_of_all_sizes(gpu):
         a.check()
 
 
-# The layouts that large calls take, at sizes that can be checked: a bound on the
-# context above 2048 gives 256-row tiles (their keys in parts where there are
-# few), 160 (tile, head) units of 128 rows give those.
+# Layouts that large calls take, at sizes that can be checked: the bound on the
+# context and the number of heads decide on tiles and parts.
 LAYOUTS = {"wide": dict(max_context=4000), "wide-whole": dict(max_context=2100, kv_heads=96),
            "pairs": dict(max_context=400, kv_heads=80)}
 
@@ -319,6 +318,86 @@ def test_scales_of_either_sign_and_zero(gpu, types):
             a.call()
             gpu.synchronize()
             a.check()
+
+
+# Between them every size of tile (256, 128 or 64 rows; 128, 64 or 32 with F32 q
+# over BF16), with its keys whole and in parts, in each pair of types.
+TILES = {
+    "few-keys": dict(new=[100], contexts=[180], kv_heads=1, group=4, bound=200),
+    "parts": dict(new=[100], contexts=[700], kv_heads=1, group=4, bound=1000),
+    "long-bound": dict(new=[100], contexts=[500], kv_heads=1, group=4, bound=6000),
+    "longer-bound": dict(new=[190], contexts=[600], kv_heads=2, group=4, bound=8000),
+    "heads": dict(new=[150], contexts=[300], kv_heads=96, group=1, bound=700),
+    "heads-parts": dict(new=[150], contexts=[600], kv_heads=40, group=1, bound=6000),
+    "two-prompts": dict(new=[170, 130], contexts=[200, 150], kv_heads=96, group=1, bound=700),
+    "more-heads": dict(new=[300], contexts=[330], kv_heads=128, group=1, bound=1000),
+}
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("name", TILES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tiles_and_parts(gpu, name, types, dim):
+    kind, q_type = TYPES[types]
+    case = TILES[name]
+    print(f"[case] attention tiles {name} {types} dim={dim}", flush=True)
+    p = Paged(case["new"], case["contexts"], kv_heads=case["kv_heads"], kind=kind, dim=dim, seed=dim + len(name))
+    used = np.zeros((p.pages, p.page), bool)
+    for s, c in enumerate(p.contexts):
+        used[p.table[s, np.arange(c) // p.page], np.arange(c) % p.page] = True
+    for pool, value in ((p.k, np.inf), (p.v, np.nan)):
+        p.seen(pool)[~used] = ref.encode(value, kind)
+    a = Attend(gpu, p, case["kv_heads"] * case["group"], q_type=q_type, max_context=case["bound"])
+    a.call()
+    a.call()
+    gpu.synchronize()
+    a.check()
+
+
+# Few rows over many keys: 4, 7, 8, 12 and 16 rows of a tile, two to five tiles, from
+# nine parts to more than a hundred.
+MANY_PARTS = {
+    "four-rows": dict(new=[1], contexts=[5000], kv_heads=2, group=4),
+    "seven-rows": dict(new=[1, 1], contexts=[3000, 1300], kv_heads=2, group=7),
+    "eight-rows": dict(new=[1, 2], contexts=[2500, 2050], kv_heads=2, group=8),
+    "twelve-rows": dict(new=[3], contexts=[9000], kv_heads=1, group=4),
+    "sixteen-rows": dict(new=[4, 4, 1], contexts=[3000, 40, 1500], kv_heads=2, group=4),
+    "tiles": dict(new=[16, 5], contexts=[2600, 700], kv_heads=2, group=4),
+    "uneven-tiles": dict(new=[17, 9, 0, 1], contexts=[4500, 130, 0, 2200], kv_heads=2, group=4),
+    "hundred-parts": dict(new=[1], contexts=[20000], kv_heads=1, group=3),
+}
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("name", MANY_PARTS)
+def test_few_rows_in_many_parts(gpu, name, types):
+    kind, q_type = TYPES[types]
+    case = MANY_PARTS[name]
+    for dim in (64, 128):
+        print(f"[case] attention parts {name} {types} dim={dim}", flush=True)
+        p = Paged(case["new"], case["contexts"], kv_heads=case["kv_heads"], kind=kind, dim=dim, page=64, seed=dim + 1)
+        a = Attend(gpu, p, case["kv_heads"] * case["group"], q_type=q_type)
+        a.call()
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", ["f16-f32", "bf16-bf16"])
+def test_batches_of_several_tiles_in_parts(gpu, types):
+    """More (tile, head) units than compute units, too many tiles a sequence to take contexts by length."""
+    kind, q_type = TYPES[types]
+    rng = np.random.default_rng(33)
+    new = [int(n) for n in rng.integers(1, 11, 20)]
+    contexts = [int(c) + n for c, n in zip(rng.integers(1, 500, 20), new)]
+    contexts[3], contexts[11] = 4400, 2300
+    p = Paged(new, contexts, kv_heads=6, kind=kind, dim=64, seed=34, gaps=(1, 2))
+    for window in (0, 2500):
+        a = Attend(gpu, p, 24, q_type=q_type, window=window)
+        a.call()
+        a.call()
+        gpu.synchronize()
+        a.check()
 
 
 @pytest.mark.parametrize("types", ["f16-f32", "bf16-bf16"])

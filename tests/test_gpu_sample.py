@@ -118,6 +118,31 @@ def test_one_workspace_serves_batches_of_all_sizes(gpu):
         s.run()
 
 
+@pytest.mark.parametrize("V", [1182, 2054, 11647, 40000, 151936])
+def test_kept_sets_of_hundreds(gpu, V):
+    """Borders among more listed logits than are ranked one against another,
+    at temperatures from low ones, where the k-th lies far below the maximum."""
+    rng = np.random.default_rng(V)
+    x = _logits(rng, 6, V)
+    for k in (0, 100, 129, 360, 1000, 2047):
+        for p, min_p, heat in ((1.0, 0.0, 0.8), (0.95, 0.0, 1.4), (0.3, 0.001, 1.0), (0.999, 0.01, 0.2)):
+            print(f"[case] sample hundreds V={V} k={k} p={p} T={heat}", flush=True)
+            Sample(gpu, x, heat, k, p, min_p, rng.random(6)).run()
+
+
+def test_neighbours_and_equal_logits_among_hundreds(gpu):
+    """Kept tokens next to one another, and of one value: all in one part of the
+    indices or of the keys."""
+    rng = np.random.default_rng(12)
+    V, R = 151936, 12
+    x = rng.standard_normal((R, V)).astype(np.float32) - 4
+    x[:, 1000:1300] = 6 + rng.random((R, 300)).astype(np.float32)
+    x[4:8, rng.integers(0, V, 400)] = 8.25
+    x[8:, 1000:1300] = 6 + (np.arange(300) // 150).astype(np.float32)
+    for k, p in ((250, 1.0), (299, 0.9), (320, 0.6), (700, 0.95), (0, 0.9)):
+        Sample(gpu, x, 0.7, k, p, 0.0, rng.random(R)).run()
+
+
 def test_the_whole_line_of_uniforms(gpu):
     """Uniforms over [0, 1) draw every kept token, in index order."""
     V, R = 130, 400
