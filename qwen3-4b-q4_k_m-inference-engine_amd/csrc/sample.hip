@@ -3,14 +3,15 @@
 //
 // sample_scan_kernel reads every logit once, one workgroup per chunk of a row
 // (2048 or 8192 logits, all in registers): the chunk's maximum; how many
-// logits lie in each of 128 bands below it, a quarter of the temperature wide
-// (at most 1/5), and, where no top-k bounds the kept set, the sum of their
-// weights; and the logits of the top bands themselves, as many as the row's
-// top-k can take from one chunk. sample_draw_kernel, one workgroup per row,
+// logits lie in each of 128 bands below it, a fifth wide (without top-k a quarter
+// of the temperature at most), and, where no top-k bounds the kept set, the sum of
+// their weights; and the logits of the top bands themselves, band by band, as many
+// as the row's top-k can take from one chunk. sample_draw_kernel, one workgroup per row,
 // adds the bands up, which gives the band that a filter's border falls into,
 // and then
-//   - where the chunks' lists reach down to that band (the usual filters),
-//     ranks the listed logits and finds everything among them;
+//   - where the chunks' lists reach down to that band (the usual filters), finds
+//     everything among the listed logits: few of them, or those of an even part of
+//     them that holds a border, are ranked one against another;
 //   - without top-k, reads the row once more for the logits of that band
 //     alone (several workgroups if there are few rows), or not at all if there
 //     is no border (bare temperature), picks the drawn token's chunk by the
@@ -26,7 +27,7 @@
 // its own and scaled once per band, in 64-bit floating point. Bands only say
 // where to look; no result depends on their width.
 // Measured: one row of 151936, top-k 20 and top-p 0.95: 15 us; 200 rows: greedy 24
-// (5.1 TB/s), top-k 20 38, filters of their own (a fifth without top-k) 89.
+// (5.0 TB/s), top-k 20 37, filters of their own (a fifth without top-k) 82.
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -645,9 +646,9 @@ __device__ bool join_items(const SamplePlan& p, int row, Shared& sh) {
 }
 
 // The draw: a few dependent reads of what the scan left, a ranking in LDS and
-// running sums; latency bounds it: 9 us a row for top-k 20, 13 for 50, 25 for 300;
-// without top-k 14 where the lists reach the border, 33 to 48 where the row is
-// read again (temperature 1.3).
+// running sums; latency bounds it: 8 us a row for top-k 20, 9 for 50, 16 for 300;
+// without top-k 23 to 30 where sixteen workgroups read the row again, 30 to 38
+// where one does.
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs a, const SamplePlan p) {
   __shared__ Shared sh;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
@@ -868,7 +869,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     }
     // More: sums over even parts of the keys, then of the indices, say which
     // part holds an end of the kept set or the drawn token, and its items alone
-    // are ranked: 600 items in 7 us, sorted by both 14. False where a part
+    // are ranked: 600 items in 8 us, sorted by both 14. False where a part
     // holds too many (equal logits).
     const auto draw_by_parts = [&] {
       uint64_t item[2], f[2];
@@ -1277,7 +1278,8 @@ SamplePlan plan_sample(int64_t rows, int64_t vocabulary, void* workspace) {
   // One compute unit reads a row of 151936 in 25 us, sixteen in 3: a row's draw
   // has as many workgroups as leave one a compute unit, 4096 logits each at least
   // (us, top-p 0.95 at temperature 1.3, with and without: one row 44 and 59; at
-  // 64 rows 74 and 73).
+  // 64 rows 74 and 73; two or four times as many: 200 rows 142 and 146 against 121,
+  // though with mixed filters, where most leave at once, 80 and 79 against 83).
   const int64_t share = vocabulary / 4096 < 256 / rows ? vocabulary / 4096 : 256 / rows;
   p.helpers = static_cast<int32_t>(share < 1 ? 1 : share < 16 ? share : 16);
   if (p.helpers > 1) p.items = reinterpret_cast<uint64_t*>(take(static_cast<size_t>(rows) * kItems * sizeof(uint64_t)));

@@ -53,7 +53,7 @@ struct AttentionArgs {
 
 // How a call is laid out, from host values alone.
 struct AttentionPlan {
-  bool few;              // 16-row tiles (paged_attention_few.hip), else 256 or 128 (paged_attention_many.hip)
+  bool few;              // 16-row tiles (paged_attention_few.hip), else 256 to 32 (paged_attention_many.hip)
   int key_groups;        // of the latter: 1, or 2 or 4 waves that share 32 rows, each with a part of the keys
   int rows;              // rows of a tile: (new token, query head of the key/value head)
   int32_t tiles;         // at most so many tiles
