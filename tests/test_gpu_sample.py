@@ -130,6 +130,19 @@ def test_kept_sets_of_hundreds(gpu, V):
             Sample(gpu, x, heat, k, p, min_p, rng.random(6)).run()
 
 
+@pytest.mark.parametrize("V", [5003, 40000, 151936])
+def test_kept_sets_of_thousands(gpu, V):
+    """More than the draw ranks at once; rows without a border; nearly flat rows."""
+    rng = np.random.default_rng(V + 1)
+    x = _logits(rng, 5, V)
+    x[3] = np.float32(0.02) * rng.standard_normal(V).astype(np.float32)
+    x[4] = np.round(x[4])
+    for k in (0, 2500, 4999):
+        for p, min_p, heat in ((1.0, 0.0, 1.0), (0.95, 0.0, 1.5), (0.6, 0.001, 0.9)):
+            print(f"[case] sample thousands V={V} k={k} p={p} T={heat}", flush=True)
+            Sample(gpu, x, heat, k, p, min_p, rng.random(5), stride=V + 1).run()
+
+
 def test_neighbours_and_equal_logits_among_hundreds(gpu):
     """Kept tokens next to one another, and of one value: all in one part of the
     indices or of the keys."""
