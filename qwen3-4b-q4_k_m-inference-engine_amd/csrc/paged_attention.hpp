@@ -23,8 +23,6 @@
 
 namespace qk {
 
-constexpr int kGoodPartKeys = 2048;  // see plan_attention
-constexpr int kOrdered = 128;        // most sequences that are taken by length
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr float kNoMax = -3.4028234e38f;  // the maximum of no score: no finite score is below it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

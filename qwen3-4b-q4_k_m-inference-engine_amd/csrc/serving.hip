@@ -177,7 +177,7 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
   a.q_heads = static_cast<int32_t>(q_heads);
   a.group = static_cast<int32_t>(q_heads / cache->kv_heads);
   a.scale = scale;
-  a.window = window < INT32_MAX ? static_cast<int32_t>(window) : 0;  // positions are below 2^31: all are seen
+  a.window = static_cast<int32_t>(qk::bounded_window(window));
   a.out = out;
   a.lse = lse;
   return finish(qk::launch_paged_attention(a, plan, cache->type, static_cast<int>(cache->head_dim), q_type, workspace,

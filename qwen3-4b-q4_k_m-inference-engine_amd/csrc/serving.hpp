@@ -7,6 +7,7 @@
 
 #include <cstdint>
 
+#include "attention_plan.hpp"
 #include "kv_index.hpp"
 #include "qk_abi.h"
 
@@ -51,22 +52,6 @@ struct AttentionArgs {
   float* parts;       // [tiles x kv_heads x splits x rows x head_dim]
 };
 
-// How a call is laid out, from host values alone.
-struct AttentionPlan {
-  bool few;              // 16-row tiles (paged_attention_few.hip), else 256 to 32 (paged_attention_many.hip)
-  int key_groups;        // of the latter: 1, or 2 or 4 waves that share 32 rows, each with a part of the keys
-  int rows;              // rows of a tile: (new token, query head of the key/value head)
-  int32_t tiles;         // at most so many tiles
-  int32_t splits;        // workgroups that may share a tile's keys
-  int32_t fill;          // so many of them fill the card
-  int32_t pairs;         // see AttentionArgs
-  size_t sums_at, parts_at, bytes;  // workspace; 0 bytes without splits
-};
-// Waves of a workgroup of paged_attention_many.hip, 32 rows each: eight, but
-// four with 512 registers each where F32 q meets a BF16 cache (three parts).
-constexpr int attention_many_waves(bool bf16, bool q32) { return bf16 && q32 ? 4 : 8; }
-AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int head_dim, int type,
-                             int q_type, int64_t window, int64_t max_context);
 hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, int type, int head_dim, int q_type,
                                   void* workspace, hipStream_t stream);
 hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream);

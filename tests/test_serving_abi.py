@@ -143,3 +143,41 @@ def test_batch_indices_stay_in_bounds(tmp_path):
     env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:abort_on_error=1")
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env=env)
     assert res.returncode == 0 and "all checks passed" in res.stdout, res.stdout + res.stderr
+
+
+def _sanitized(tmp_path, name):
+    """tests/cpp/<name>.cpp under the address and UB sanitizers."""
+    exe = tmp_path / name
+    res = subprocess.run(["g++", "-std=c++20", "-g", "-O1", "-Wall", "-Wextra", "-fsanitize=address,undefined",
+                          "-fno-sanitize-recover=undefined", "-I", str(ROOT / "include"), "-I",
+                          str(ROOT / "qwen3-4b-q4_k_m-inference-engine_amd" / "csrc"),
+                          str(ROOT / "tests" / "cpp" / f"{name}.cpp"), "-o", str(exe)],
+                         capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr[-3000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:abort_on_error=1")
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env=env)
+    assert res.returncode == 0 and "all checks passed" in res.stdout, res.stdout + res.stderr
+
+
+def test_attention_plans_hold_for_lengths_of_any_size(tmp_path):
+    _sanitized(tmp_path, "attention_plan_check")
+
+
+@pytest.mark.parametrize("tokens", [1, 512])
+def test_attention_workspace_of_windows_and_bounds_of_any_size(qk, tokens):
+    """INT64_MAX for "no window" takes the workspace of no window, and is refused without it."""
+    lib = qk.load()
+    most = (1 << 63) - 1
+    b = batch(qk, sequences=1, tokens=tokens)
+    c = cache(qk, kv_heads=8, token_stride=1024, page_stride=16384)
+    size = lambda window, context: lib.qk_paged_attention_workspace_size(c, b, 0, 32, window, context)  # noqa: E731
+    for context in (1000, 4096, 131072):
+        none = size(0, context)
+        assert none > 0 or (tokens, context) == (512, 1000)
+        for window in (most, most - 1, most - 255, 1 << 40, (1 << 31) - 1):
+            assert size(window, context) == none, (window, context)
+            call = lambda ws, n: lib.qk_paged_attention(c, b, P, 0, 4096, 32, 0.1, window, context, P, None, ws, n,  # noqa: E731
+                                                        None)
+            if none:
+                assert call(None, 0) == INVALID and call(P, none - 1) == INVALID
+    assert size(0, most) == size(0, (1 << 31) - 1) > 0
