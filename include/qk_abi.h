@@ -361,7 +361,9 @@ int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float
  * context. A row that sees nothing is 0 with lse -inf. Whatever unused page
  * slots and later positions hold, NaN and infinities included, has no effect;
  * pages wholly before every token's window are not looked up. If a page id that is needed
- * is out of range, rows of that sequence are NaN (see qk_kv_cache::fault).
+ * is out of range, rows of that sequence are NaN (see qk_kv_cache::fault); all of
+ * them, and no key is read, where its context is longer than table_stride pages
+ * or than 2^30 tokens.
  * Scores, the softmax and the sums are fp32. F32 q: q and the softmax weights
  * meet the cached values as two F16 (three BF16) parts, so the result has
  * fp32's precision; 16-bit q: the weights are rounded to the cache's type for

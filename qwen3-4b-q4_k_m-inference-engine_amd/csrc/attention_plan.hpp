@@ -6,6 +6,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "kv_index.hpp"
 #include "qk_abi.h"
 
 namespace qk {
@@ -31,10 +32,9 @@ constexpr int attention_many_waves(bool bf16, bool q32) { return bf16 && q32 ? 4
 // Lengths of any size that callers give for "all" (INT64_MAX among them) as ones
 // that sums and the kernels' 32 bits hold: positions are below kMostPositions, so
 // a window that reaches over all of them is none.
-constexpr int64_t kMostPositions = INT32_MAX;
 constexpr int64_t bounded_window(int64_t window) { return window < kMostPositions ? window : 0; }
 constexpr int64_t bounded_context(int64_t max_context) {
-  return max_context < 1 ? 1 : max_context < kMostPositions ? max_context : kMostPositions;
+  return max_context < 1 ? 1 : max_context < kMostPositions ? max_context : int64_t{kMostPositions};
 }
 
 namespace plan {

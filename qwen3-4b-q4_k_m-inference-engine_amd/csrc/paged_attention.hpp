@@ -110,26 +110,6 @@ __device__ __forceinline__ float swap32_max(float v) {
   return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
-// The tile of a workgroup, in scalar registers.
-struct AttentionTile {
-  int s;               // sequence; -1: the workgroup has no tile
-  int row, count;      // first new row and new rows of the sequence
-  int first;           // position of its first new row
-  int begin, rows;     // first row of the tile among the sequence's, rows of the sequence (count * group)
-  int key_lo, key_hi;  // keys that any row of the tile sees
-  bool fault;
-};
-
-// The rest of a tile, from its sequence and first row.
-__device__ __forceinline__ void tile_keys(const AttentionArgs& a, int tile_rows, AttentionTile& t) {
-  t.rows = t.count * a.group;
-  const int end = t.begin + tile_rows < t.rows ? t.begin + tile_rows : t.rows;
-  t.key_hi = t.first + (end - 1) / a.group + 1;
-  const int lowest = a.window > 0 ? t.first + t.begin / a.group - a.window + 1 : 0;
-  t.key_lo = lowest > 0 ? lowest : 0;
-  if (t.key_hi < t.key_lo) t.key_hi = t.key_lo;  // positions before 0 see nothing
-}
-
 // Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
 // sums of the tile counts until they pass `tile`.
 __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile, int tile_rows) {
@@ -159,12 +139,13 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
       t.count = __builtin_amdgcn_readlane(q.count, at);
       t.first = __builtin_amdgcn_readlane(q.first, at);
       t.fault = __builtin_amdgcn_readlane(q.fault ? 1 : 0, at) != 0;
+      t.beyond = __builtin_amdgcn_readlane(q.beyond ? 1 : 0, at) != 0;
       t.begin = (tile - before - __builtin_amdgcn_readlane(run - mine, at)) * tile_rows;
       break;
     }
     before += __builtin_amdgcn_readlane(run, 63);
   }
-  if (t.s >= 0) tile_keys(a, tile_rows, t);
+  if (t.s >= 0) tile_keys(a.group, a.window, tile_rows, t);
   return t;
 }
 
@@ -174,7 +155,7 @@ __device__ __forceinline__ int longest_context(const AttentionArgs& a) {
   int most = 0;
   for (int s = lane; s < a.kv.sequences; s += 64) {
     const KvSequence q = kv_sequence(a.kv, s);
-    const int keys = q.count > 0 ? q.first + q.count : 0;
+    const int keys = kv_keys(q);
     most = keys > most ? keys : most;
   }
 #pragma unroll
@@ -183,24 +164,6 @@ __device__ __forceinline__ int longest_context(const AttentionArgs& a) {
     most = other > most ? other : most;
   }
   return __builtin_amdgcn_readfirstlane(a.window > 0 && most > a.window ? a.window : most);
-}
-
-// A tile's keys over its workgroups: chunks of `chunk` keys, but long enough that
-// `splits` of them suffice, in multiples of `step`; `used` of them are not empty
-// (one at least).
-struct KeyChunk {
-  int lo, hi, used;
-};
-__device__ __forceinline__ KeyChunk key_chunk(const AttentionTile& t, int split, int splits, int step, int chunk) {
-  const int keys = t.key_hi - t.key_lo;
-  const int least = (keys + splits - 1) / splits;
-  chunk = chunk < least ? least : chunk;
-  chunk = (chunk + step - 1) / step * step;
-  KeyChunk c;
-  c.used = keys > 0 ? (keys + chunk - 1) / chunk : 1;
-  c.lo = split < c.used ? t.key_lo + split * chunk : t.key_hi;
-  c.hi = t.key_hi - c.lo > chunk ? c.lo + chunk : t.key_hi;
-  return c;
 }
 
 // Values that another workgroup of the launch reads: coherent at agent scope,

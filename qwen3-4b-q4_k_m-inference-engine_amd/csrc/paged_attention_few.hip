@@ -50,8 +50,8 @@ __device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile,
     const KvSequence q = kv_sequence(a.kv, s);
     single = q.count * a.group <= kRows;
     if (q.count > 0) {
-      mine = q.first + q.count;
-      mine = mine < 0 ? 0 : a.window > 0 && mine > a.window ? a.window : mine;
+      mine = kv_keys(q);
+      mine = a.window > 0 && mine > a.window ? a.window : mine;
     }
   }
   if (s < kOrdered) keys[s] = mine;
@@ -75,8 +75,9 @@ __device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile,
   t.count = q.count;
   t.first = q.first;
   t.fault = q.fault;
+  t.beyond = q.beyond;
   t.begin = 0;
-  tile_keys(a, kRows, t);
+  tile_keys(a.group, a.window, kRows, t);
   return true;
 }
 
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   }
   const KeyChunk c = key_chunk(t, split, a.splits, kStep, chunk);
   if (split >= c.used) return;
-  if (tid == 0) sh.bad = 0;
+  if (tid == 0) sh.bad = t.beyond;
   if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
   __syncthreads();
 

@@ -75,8 +75,9 @@ attention_many_kernel(const AttentionArgs a) {
   if (t.s < 0) return;
   const KeyChunk c = key_chunk(t, split, a.splits, kChunkStep, kLeastChunk);
   if (split >= c.used) return;
-  if (tid == 0) sh.bad = sh.odd[0] = sh.odd[1] = 0;  // odd[n & 3] is cleared while tile n - 2 runs
+  if (tid == 0) sh.bad = t.beyond, sh.odd[0] = sh.odd[1] = 0;  // odd[n & 3] is cleared while tile n - 2 runs
   if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
+  if (t.beyond && tid == 0) kv_fault(a.kv, QK_KV_FAULT_PAGE);
 
   // the lane's row
   const int col = lane & 31, half = lane >> 5;

@@ -485,3 +485,47 @@ def test_a_page_far_into_a_large_pool(gpu):
     a.check()
     for b in big.values():
         b.free()
+
+
+@pytest.mark.parametrize("length", [0x7FFFFFFF, 1500000000, (1 << 30) + 1000, 5 * 8 + 1])
+def test_a_context_beyond_its_page_table_is_reported(gpu, length):
+    """No key of it is walked: its rows are NaN, the others what they are."""
+    for new, contexts, bound in (([1, 1, 1], [40, 40, 40], 40), ([1, 2, 1], [40, 40, 40], 1 << 20),
+                                 ([30, 30, 30], [40, 40, 40], 40), ([90, 30, 30], [90, 40, 40], 1 << 20)):
+        print(f"[case] attention context {length} new={new} bound={bound}", flush=True)
+        p = Paged(new, contexts, page=8, dim=128, seed=23)
+        if max(contexts) > 40:
+            length = max(length, 12 * 8 + 1)
+        a = Attend(gpu, p, 4, max_context=bound)
+        lengths = np.asarray(contexts, np.int32)
+        lengths[1] = length
+        p.dev["context"].upload(lengths)
+        for window in (0, 7):
+            a.window = window
+            a.call()
+            gpu.synchronize()
+            out, lse = a.results()
+            rows = slice(p.start[1], p.start[2])
+            assert np.isnan(out[rows].view(np.float32)).all() and np.isnan(lse[rows]).all()
+            assert p.fault() == gpu.KV_FAULT_PAGE
+            with pytest.raises(gpu.QKError, match="page"):
+                gpu.kv_check(p.cache)
+            a.check(sequences=(0, 2))
+
+
+def test_a_context_beyond_its_page_table_among_many(gpu):
+    """Sequences taken by length."""
+    rng = np.random.default_rng(24)
+    contexts = [int(c) for c in rng.integers(1, 260, 70)]
+    contexts[5] = 1300
+    p = Paged([1] * 70, contexts, kv_heads=4, dim=64, seed=25)
+    a = Attend(gpu, p, 8, max_context=1300)
+    lengths = np.asarray(contexts, np.int32)
+    lengths[9] = 0x7FFFFFFF
+    p.dev["context"].upload(lengths)
+    a.call()
+    gpu.synchronize()
+    assert np.isnan(a.results()[0][9].view(np.float32)).all()
+    assert p.fault() == gpu.KV_FAULT_PAGE
+    p.dev["fault"].upload(np.zeros(1, np.uint32))
+    a.check(sequences=[s for s in range(70) if s != 9])

@@ -181,3 +181,7 @@ def test_attention_workspace_of_windows_and_bounds_of_any_size(qk, tokens):
             if none:
                 assert call(None, 0) == INVALID and call(P, none - 1) == INVALID
     assert size(0, most) == size(0, (1 << 31) - 1) > 0
+
+
+def test_attention_keys_stay_in_the_page_table(tmp_path):
+    _sanitized(tmp_path, "attention_keys_check")
