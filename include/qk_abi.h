@@ -286,7 +286,8 @@ int qk_matmul_argmax(const float *x, const void *w, int type, int64_t K, int64_t
  * fault: NULL, or a device word that the calls on this cache OR bits into (the
  * caller clears it once): QK_KV_FAULT_PAGE, a page id outside [0, pages) or a
  * position beyond the sequence's page table was met; QK_KV_FAULT_LENGTH,
- * token_start or context did not fit together. qk_kv_check reads it. */
+ * token_start or context of any sequence did not fit (descending or beyond
+ * `tokens`; negative or shorter than the new tokens). qk_kv_check reads it. */
 typedef struct qk_kv_cache {
     void *k;
     void *v;

@@ -57,7 +57,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   }
   const int s = kv_find_sequence(a.kv, token);
   const KvSequence seq = kv_sequence(a.kv, s);
-  if (seq.fault && tid == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
+  if (blockIdx.x == 0 && blockIdx.y == 0)  // lengths that do not fit, of sequences without rows too
+    for (int i = tid; i < a.kv.sequences; i += 256)
+      if (kv_sequence(a.kv, i).fault) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
   if (token < seq.row || token >= seq.row + seq.count) return;  // no sequence owns this row
   const int position = seq.first + (token - seq.row);
   if (tid < a.dims / 2) {

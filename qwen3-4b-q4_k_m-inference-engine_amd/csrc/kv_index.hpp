@@ -37,7 +37,7 @@ struct KvArgs {
 };
 
 // A sequence's new rows and the position of the first of them. Lengths that do
-// not fit are cut: row .. row + count lies in [0, tokens], positions are below
+// not fit (fault) are cut: row .. row + count lies in [0, tokens], positions are below
 // 2^31 (negative ones see nothing). beyond: the last of them has no place in the
 // page table, or lies past kMostPositions.
 struct KvSequence {
@@ -49,13 +49,12 @@ QK_HD KvSequence kv_sequence(const KvArgs& a, int s) {
   KvSequence q;
   q.row = lo < 0 ? 0 : lo;
   const int32_t end = hi < a.tokens ? hi : a.tokens;
-  const bool ordered = hi >= lo && context >= 0;
-  q.count = ordered && end > q.row ? end - q.row : 0;
-  q.fault = lo < 0 || hi > a.tokens || !ordered || context < static_cast<int64_t>(hi) - lo;
-  // hi >= q.row >= 0 wherever count > 0, so this neither overflows nor exceeds context;
-  // count is below kMostTokens, so positions cut at its negative stay negative
-  q.first = q.count > 0 ? context - (hi - q.row) : 0;
-  q.first = q.first < -kMostTokens ? -kMostTokens : q.first;
+  q.count = hi >= lo && end > q.row ? end - q.row : 0;
+  q.fault = lo < 0 || hi > a.tokens || hi < lo || context < 0 || context < static_cast<int64_t>(hi) - lo;
+  // hi >= q.row >= 0 wherever count > 0, so this does not exceed context; count is
+  // below kMostTokens, so positions cut at its negative stay negative
+  const int64_t first = q.count > 0 ? static_cast<int64_t>(context) - (hi - q.row) : 0;
+  q.first = first < -kMostTokens ? -kMostTokens : static_cast<int32_t>(first);
   const int64_t room = static_cast<int64_t>(a.table_pages) * a.page_size;
   q.beyond = context > kMostPositions || context > room;
   return q;
@@ -107,7 +106,7 @@ struct AttentionTile {
   int first;           // position of its first new row
   int begin, rows;     // first row of the tile among the sequence's, rows of the sequence (count * group)
   int key_lo, key_hi;  // keys that any row of the tile sees
-  bool fault, beyond;  // of the sequence
+  bool beyond;         // of the sequence
 };
 
 // The rest of a tile, from its sequence and first row. A context that is beyond its

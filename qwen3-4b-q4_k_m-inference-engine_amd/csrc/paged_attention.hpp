@@ -111,8 +111,9 @@ __device__ __forceinline__ float swap32_max(float v) {
 }
 
 // Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
-// sums of the tile counts until they pass `tile`.
-__device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile, int tile_rows) {
+// sums of the tile counts until they pass `tile`. Where `report`, lengths that do
+// not fit are reported, of all sequences: one without rows has no tile.
+__device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int tile, int tile_rows, bool report) {
   const int lane = static_cast<int>(threadIdx.x & 63);
   AttentionTile t;
   t.s = -1;
@@ -125,6 +126,8 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
       q = kv_sequence(a.kv, s);
       mine = (q.count * a.group + tile_rows - 1) / tile_rows;
     }
+    if (report && q.fault) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
+    if (t.s >= 0) continue;
     int run = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -138,10 +141,9 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
       t.row = __builtin_amdgcn_readlane(q.row, at);
       t.count = __builtin_amdgcn_readlane(q.count, at);
       t.first = __builtin_amdgcn_readlane(q.first, at);
-      t.fault = __builtin_amdgcn_readlane(q.fault ? 1 : 0, at) != 0;
       t.beyond = __builtin_amdgcn_readlane(q.beyond ? 1 : 0, at) != 0;
       t.begin = (tile - before - __builtin_amdgcn_readlane(run - mine, at)) * tile_rows;
-      break;
+      if (!report) break;
     }
     before += __builtin_amdgcn_readlane(run, 63);
   }

@@ -41,13 +41,14 @@ __device__ __forceinline__ int k_chunk(int key, int chunk) {
 // rest. Each unit's two contexts so have about the same length together: 64
 // sequences of up to 8192 keys, uneven, 225 us as they come, 175 paired. Every
 // workgroup ranks the lengths itself, a thread a sequence.
-__device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile, int32_t (&keys)[kOrdered], int32_t& chosen,
-                                               AttentionTile& t) {
+__device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile, bool report, int32_t (&keys)[kOrdered],
+                                               int32_t& chosen, AttentionTile& t) {
   const int s = static_cast<int>(threadIdx.x);
   int mine = -1;
   bool single = true;
   if (s < a.kv.sequences) {
     const KvSequence q = kv_sequence(a.kv, s);
+    if (report && q.fault) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
     single = q.count * a.group <= kRows;
     if (q.count > 0) {
       mine = kv_keys(q);
@@ -74,7 +75,6 @@ __device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile,
   t.row = q.row;
   t.count = q.count;
   t.first = q.first;
-  t.fault = q.fault;
   t.beyond = q.beyond;
   t.begin = 0;
   tile_keys(a.group, a.window, kRows, t);
@@ -111,7 +111,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
   const int tile = unit / a.splits, split = unit % a.splits;
   AttentionTile t;
-  if (a.pairs == 0 || !find_by_length(a, tile, sh.keys, sh.chosen, t)) t = find_tile(a, tile, kRows);
+  const bool report = blockIdx.x == 0;
+  if (a.pairs == 0 || !find_by_length(a, tile, report, sh.keys, sh.chosen, t)) t = find_tile(a, tile, kRows, report);
   if (t.s < 0) return;
   // chunks of one length for all sequences, so that a batch's longest does not outlast the rest
   int chunk = kStep;
@@ -124,7 +125,6 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const KeyChunk c = key_chunk(t, split, a.splits, kStep, chunk);
   if (split >= c.used) return;
   if (tid == 0) sh.bad = t.beyond;
-  if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
   __syncthreads();
 
   // the lane's row: column of every accumulator

@@ -71,12 +71,11 @@ attention_many_kernel(const AttentionArgs a) {
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
   const int tile = a.tiles - 1 - unit / a.splits, split = unit % a.splits;  // long tiles first
-  const AttentionTile t = find_tile(a, tile, kRows);
+  const AttentionTile t = find_tile(a, tile, kRows, blockIdx.x == 0);
   if (t.s < 0) return;
   const KeyChunk c = key_chunk(t, split, a.splits, kChunkStep, kLeastChunk);
   if (split >= c.used) return;
   if (tid == 0) sh.bad = t.beyond, sh.odd[0] = sh.odd[1] = 0;  // odd[n & 3] is cleared while tile n - 2 runs
-  if (t.fault && tid == 0 && head == 0 && split == 0) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
   if (t.beyond && tid == 0) kv_fault(a.kv, QK_KV_FAULT_PAGE);
 
   // the lane's row
@@ -455,7 +454,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
   const int groups = tile_rows / 32, group = static_cast<int>(blockIdx.x) % groups, unit = static_cast<int>(blockIdx.x) / groups;
   const int tile = unit / a.kv.kv_heads, head = unit % a.kv.kv_heads;
-  const AttentionTile t = find_tile(a, tile, tile_rows);
+  const AttentionTile t = find_tile(a, tile, tile_rows, false);
   if (t.s < 0) return;
   const int used = key_chunk(t, 0, a.splits, kChunkStep, kLeastChunk).used;
   const int col = lane & 31, half = lane >> 5, row = t.begin + group * 32 + col;

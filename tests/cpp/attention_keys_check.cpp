@@ -46,6 +46,11 @@ int main() {
     for (int s = 0; s < a.sequences; ++s) {
       const qk::KvSequence q = qk::kv_sequence(a, s);
       CHECK(q.beyond == (context[s] > (1 << 30) || context[s] > room));
+      // a negative context keeps its rows, none of which has a position
+      const bool owned = start[s] >= 0 && start[s + 1] >= start[s] && start[s + 1] <= a.tokens;
+      if (owned) CHECK(q.row == start[s] && q.count == start[s + 1] - start[s]);
+      if (!owned || context[s] < q.count) CHECK(q.fault);
+      if (context[s] < 0) CHECK(q.fault && q.first + q.count <= 0);
       const int seen = qk::kv_keys(q);
       CHECK(seen >= 0 && seen <= room && seen <= 1 << 30);
       for (int begin = 0; begin < q.count * group; begin += tile_rows) {
@@ -54,7 +59,6 @@ int main() {
         t.row = q.row;
         t.count = q.count;
         t.first = q.first;
-        t.fault = q.fault;
         t.beyond = q.beyond;
         t.begin = begin;
         qk::tile_keys(group, window, tile_rows, t);

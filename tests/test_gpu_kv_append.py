@@ -204,3 +204,33 @@ def test_captured_append_serves_new_lengths(gpu):
         a.check()
     graph.destroy()
     stream.destroy()
+
+
+def test_lengths_that_do_not_fit_are_reported_whoever_owns_the_rows(gpu):
+    """A sequence that owns no row, and a negative context, store nothing and are reported."""
+    p = Paged([3, 0], [20, 9], page=8, seed=14)
+    a = Append(gpu, p, 2)
+    p.dev["context"].upload(np.asarray([20, -1], np.int32))
+    a.call()
+    gpu.synchronize()
+    assert p.fault() == gpu.KV_FAULT_LENGTH
+    p.dev["fault"].upload(np.zeros(1, np.uint32))
+    a.check()
+    for context in (-1, -(1 << 31)):
+        p = Paged([2, 3], [20, 9], page=8, seed=15)
+        a = Append(gpu, p, 2)
+        p.dev["context"].upload(np.asarray([20, context], np.int32))
+        before = [p.dev[n].download(np.uint16).reshape(p.k.shape) for n in "kv"]
+        a.call()
+        gpu.synchronize()
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        for n, pool in zip("kv", before):
+            after = p.dev[n].download(np.uint16).reshape(p.k.shape)
+            held = p.table[1, :2]
+            assert np.array_equal(p.seen(after)[held], p.seen(pool)[held])
+    p = Paged([2, 3, 1], [20, 9, 5], page=8, seed=16)
+    a = Append(gpu, p, 2)
+    p.dev["start"].upload(np.asarray([0, 5, 2, 6], np.int32))
+    a.call()
+    gpu.synchronize()
+    assert p.fault() & gpu.KV_FAULT_LENGTH

@@ -529,3 +529,76 @@ def test_a_context_beyond_its_page_table_among_many(gpu):
     assert p.fault() == gpu.KV_FAULT_PAGE
     p.dev["fault"].upload(np.zeros(1, np.uint32))
     a.check(sequences=[s for s in range(70) if s != 9])
+
+
+def _misfits(layout):
+    """(sequence, new, contexts, contexts with a negative one there) of batches in that layout."""
+    if layout == "long":
+        new, contexts = [90, 30, 30], [300, 200, 31]
+    elif layout == "by-length":
+        new, contexts = [1] * 70, [20 + 3 * i for i in range(69)] + [1300]
+    else:
+        new, contexts = [1, 2, 1], [40, 300, 7]
+    last = len(new) - 1
+    for s in (0, last // 2, last):
+        yield s, new, contexts, np.asarray(contexts[:s] + [-1 - s] + contexts[s + 1:], np.int32)
+        yield s, new, contexts, np.asarray(contexts[:s] + [-(1 << 31)] + contexts[s + 1:], np.int32)
+
+
+@pytest.mark.parametrize("layout", ["few", "long", "by-length"])
+def test_negative_contexts_see_nothing_and_are_reported(gpu, layout):
+    for s, new, contexts, lengths in _misfits(layout):
+        print(f"[case] attention {layout} sequence {s} context {lengths[s]}", flush=True)
+        p = Paged(new, contexts, kv_heads=4, dim=64, seed=26)
+        a = Attend(gpu, p, 8)
+        p.dev["context"].upload(lengths)
+        a.call()
+        gpu.synchronize()
+        bits, lse = a.results()
+        rows = slice(p.start[s], p.start[s + 1])
+        assert (bits[rows] == 0).all() and np.isneginf(lse[rows]).all()
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        with pytest.raises(gpu.QKError, match="token_start"):
+            gpu.kv_check(p.cache)
+        a.check(sequences=[i for i in range(len(new)) if i != s])
+
+
+@pytest.mark.parametrize("layout", ["few", "long", "by-length"])
+def test_starts_that_descend_or_pass_the_rows_are_reported(gpu, layout):
+    """Sequences that so own no row have no tile; the word is set all the same."""
+    for s, new, contexts, _ in _misfits(layout):
+        for start_of in ("descends", "passes", "negative"):
+            if s + (start_of != "negative") >= len(new):
+                continue
+            print(f"[case] attention {layout} sequence {s} {start_of}", flush=True)
+            p = Paged(new, contexts, kv_heads=4, dim=64, seed=27)
+            a = Attend(gpu, p, 8)
+            starts = p.start.copy()
+            if start_of == "descends":  # sequence s + 1 ends before it begins
+                starts[s + 1:] = starts[-1]
+                starts[s + 2:] = starts[s]
+            elif start_of == "passes":
+                starts[s + 1:] = p.tokens + 5
+            else:
+                starts[:s + 1] = -1
+            p.dev["start"].upload(starts)
+            a.call()
+            gpu.synchronize()
+            assert p.fault() & gpu.KV_FAULT_LENGTH
+            with pytest.raises(gpu.QKError):
+                gpu.kv_check(p.cache)
+
+
+def test_a_last_sequence_without_rows_is_reported(gpu):
+    """Only its own lengths are wrong: no row of the batch is its."""
+    for new, contexts in (([1, 1, 0], [40, 300, 9]), ([90, 30, 0], [300, 200, 9]), ([1] * 70 + [0], [1300] * 71)):
+        p = Paged(new, contexts, kv_heads=4, dim=64, seed=28)
+        a = Attend(gpu, p, 8)
+        lengths = np.asarray(contexts, np.int32)
+        lengths[-1] = -5
+        p.dev["context"].upload(lengths)
+        a.call()
+        gpu.synchronize()
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        p.dev["fault"].upload(np.zeros(1, np.uint32))
+        a.check()
