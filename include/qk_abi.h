@@ -389,8 +389,10 @@ size_t qk_paged_attention_workspace_size(const qk_kv_cache *cache, const qk_kv_b
                                          int q_type, int64_t q_heads, int64_t window,
                                          int64_t max_context);
 
-/* Synchronises `stream`, then returns QK_ERR_RUNTIME (and clears the word) if
- * a call on this cache met a fault since the last check, else QK_OK. */
+/* Synchronises `stream`, then returns QK_ERR_RUNTIME (and clears what it
+ * reports) if a call on this cache met a fault since the last check, else QK_OK;
+ * the message names each kind that was met. Calls on the cache may be in flight on
+ * other streams: what they set meanwhile is in this report or the next. */
 int qk_kv_check(const qk_kv_cache *cache, qk_stream_t stream);
 
 /* token[r] = an index drawn from logits[r*row_stride + 0 .. vocabulary) for

@@ -132,7 +132,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   *reinterpret_cast<u16x4*>(out + second) = y1;
 }
 
+__global__ void kv_fault_clear_kernel(uint32_t* word, uint32_t bits) { atomicAnd(word, ~bits); }
+
 }  // namespace
+
+hipError_t launch_kv_fault_clear(uint32_t* word, uint32_t bits, hipStream_t stream) {
+  kv_fault_clear_kernel<<<1, 1, 0, stream>>>(word, bits);
+  return hipGetLastError();
+}
 
 hipError_t launch_kv_append(const AppendArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
   const int rows = a.q_heads + 2 * a.kv.kv_heads, per = 256 / (head_dim / 8);

@@ -188,14 +188,18 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
 int qk_kv_check(const qk_kv_cache* cache, qk_stream_t stream) {
   if (!cache) return refuse("cache must be non-null");
   if (!cache->fault) return QK_OK;
+  if (misaligned(cache->fault, 4)) return refuse("the fault word must be 4-byte aligned");
   uint32_t fault = 0;
-  int status = qk_memcpy_d2h(&fault, cache->fault, sizeof(fault), stream);
+  const int status = qk_memcpy_d2h(&fault, cache->fault, sizeof(fault), stream);
   if (status != QK_OK || fault == 0) return status;
-  const uint32_t none = 0;
-  status = qk_memcpy_h2d(cache->fault, &none, sizeof(none), stream);
-  if (status != QK_OK) return status;
-  return refuse(fault & QK_KV_FAULT_PAGE ? "a page id or position outside the cache was met"
-                                         : "token_start or context did not fit the batch",
+  // the bits that were read and no others: a call on another stream may set one meanwhile
+  hipError_t error = qk::launch_kv_fault_clear(cache->fault, fault, as_stream(stream));
+  if (error == hipSuccess) error = hipStreamSynchronize(as_stream(stream));
+  if (error != hipSuccess) return finish(error, "clearing the fault word failed");
+  const bool page = fault & QK_KV_FAULT_PAGE, length = fault & QK_KV_FAULT_LENGTH;
+  return refuse(page && length ? "a page id or position outside the cache was met, and token_start or context did not fit the batch"
+                : page         ? "a page id or position outside the cache was met"
+                               : "token_start or context did not fit the batch",
                 QK_ERR_RUNTIME);
 }
 

@@ -35,6 +35,8 @@ struct AppendArgs {
 };
 hipError_t launch_kv_append(const AppendArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
 
+hipError_t launch_kv_fault_clear(uint32_t* word, uint32_t bits, hipStream_t stream);
+
 struct AttentionArgs {
   KvArgs kv;
   const void* q;

@@ -234,3 +234,60 @@ def test_lengths_that_do_not_fit_are_reported_whoever_owns_the_rows(gpu):
     a.call()
     gpu.synchronize()
     assert p.fault() & gpu.KV_FAULT_LENGTH
+
+
+def test_a_check_names_and_clears_what_it_read(gpu):
+    p = Paged([1], [5], page=8, seed=17).upload(gpu)
+    page, length = gpu.KV_FAULT_PAGE, gpu.KV_FAULT_LENGTH
+    for word, named in ((page, ["page"]), (length, ["token_start"]), (page | length, ["page", "token_start"])):
+        p.dev["fault"].upload(np.asarray([word], np.uint32))
+        with pytest.raises(gpu.QKError) as error:
+            gpu.kv_check(p.cache)
+        for name in ("page", "token_start"):
+            assert (name in str(error.value)) == (name in named)
+        assert p.fault() == 0
+        gpu.kv_check(p.cache)
+
+
+def test_checks_beside_calls_on_another_stream_lose_no_fault(gpu):
+    """Every faulty call is followed by a check on its own stream while checks on
+    another stream run: one of the two reports it."""
+    import threading
+
+    p = Paged([2], [20], page=8, seed=18)
+    p.table[0, 2] = -1
+    a = Append(gpu, p, 2)
+    mine, theirs = gpu.Stream(), gpu.Stream()
+    reports, done = [0], threading.Event()
+
+    def check(stream):
+        try:
+            gpu.kv_check(p.cache, stream)
+        except gpu.QKError:
+            return 1
+        return 0
+
+    def others():
+        while not done.is_set():
+            reports[0] += check(theirs)
+
+    thread = threading.Thread(target=others)
+    thread.start()
+    try:
+        for _ in range(50):
+            before = reports[0]
+            a.call(mine)
+            found = check(mine)
+            mine.synchronize()
+            if not found:  # the other's, on its way at most
+                for _ in range(2000):
+                    if reports[0] > before:
+                        break
+                    done.wait(0.001)
+                assert reports[0] > before
+    finally:
+        done.set()
+        thread.join()
+    for stream in (mine, theirs):
+        stream.synchronize()
+        stream.destroy()

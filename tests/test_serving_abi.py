@@ -185,3 +185,7 @@ def test_attention_workspace_of_windows_and_bounds_of_any_size(qk, tokens):
 
 def test_attention_keys_stay_in_the_page_table(tmp_path):
     _sanitized(tmp_path, "attention_keys_check")
+
+
+def test_a_check_refuses_a_word_out_of_place(qk):
+    assert qk.load().qk_kv_check(cache(qk, fault=P + 2), None) == INVALID
