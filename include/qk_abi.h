@@ -375,7 +375,8 @@ int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float
  * NULL when that is 0), zero-filled once; every call leaves it ready for the
  * next, of this batch or another (the largest that any of a program's batches
  * needs serves them all); calls that may run concurrently need separate ones.
- * Nothing is allocated: the call can be captured. Replaces kernels::attention
+ * Calls whose workgroups do not fit one launch are refused: tokens x q_heads up
+ * to 2^23 always fit. Nothing is allocated: the call can be captured. Replaces kernels::attention
  * (include/Kernels.hpp:66-68, src/cuda/attention.cu:95-110). */
 int qk_paged_attention(const qk_kv_cache *cache, const qk_kv_batch *batch, const void *q,
                        int q_type, int64_t q_stride, int64_t q_heads, float scale, int64_t window,

@@ -176,4 +176,12 @@ inline AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q
   return p;
 }
 
+// Whether the call's launches fit a grid, which has fewer than 2^32 threads.
+inline bool plan_fits(const AttentionPlan& p, int64_t kv_heads, int type, int q_type) {
+  const int64_t units = p.tiles * kv_heads, waves = attention_many_waves(type == QK_TYPE_BF16, q_type == QK_TYPE_F32);
+  const int64_t threads = units * p.splits * (p.few ? 256 : 64 * waves);
+  const int64_t joining = p.few || p.splits == 1 ? 0 : units * (p.rows / 32) * 256;
+  return threads <= UINT32_MAX && joining <= UINT32_MAX;
+}
+
 }  // namespace qk

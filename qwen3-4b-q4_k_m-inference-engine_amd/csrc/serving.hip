@@ -141,9 +141,10 @@ size_t qk_paged_attention_workspace_size(const qk_kv_cache* cache, const qk_kv_b
   if (check_shapes(cache, batch) != QK_OK || check_heads(cache, batch, q_heads, q_type) != QK_OK || window < 0 ||
       max_context < 0)
     return 0;
-  return qk::plan_attention(batch->tokens, batch->sequences, q_heads, cache->kv_heads, static_cast<int>(cache->head_dim),
-                            cache->type, q_type, window, max_context)
-      .bytes;
+  const qk::AttentionPlan plan =
+      qk::plan_attention(batch->tokens, batch->sequences, q_heads, cache->kv_heads, static_cast<int>(cache->head_dim),
+                         cache->type, q_type, window, max_context);
+  return qk::plan_fits(plan, cache->kv_heads, cache->type, q_type) ? plan.bytes : 0;
 }
 
 int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const void* q, int q_type, int64_t q_stride,
@@ -166,6 +167,8 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
   const qk::AttentionPlan plan =
       qk::plan_attention(batch->tokens, batch->sequences, q_heads, cache->kv_heads, static_cast<int>(cache->head_dim),
                          cache->type, q_type, window, max_context);
+  if (!qk::plan_fits(plan, cache->kv_heads, cache->type, q_type))
+    return refuse("attention of so many tokens and heads does not fit one launch");
   const size_t need = plan.bytes;
   if (need != 0 && !workspace) return refuse("attention workspace must be non-null");
   if (workspace_bytes < need) return refuse("attention workspace too small");

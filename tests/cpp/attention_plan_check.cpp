@@ -32,6 +32,7 @@ bool same(const qk::AttentionPlan& a, const qk::AttentionPlan& b) {
 }
 
 void sound(const Call& c, const qk::AttentionPlan& p) {
+  if (c.tokens * c.kv_heads * c.group <= 1 << 23) CHECK(qk::plan_fits(p, c.kv_heads, c.type, c.q_type));
   CHECK(p.tiles >= 1 && p.splits >= 1);
   CHECK(p.rows >= 16 && p.key_groups >= 1);
   // every row has a tile, whichever sequences have them

@@ -189,3 +189,12 @@ def test_attention_keys_stay_in_the_page_table(tmp_path):
 
 def test_a_check_refuses_a_word_out_of_place(qk):
     assert qk.load().qk_kv_check(cache(qk, fault=P + 2), None) == INVALID
+
+
+def test_attention_refuses_more_workgroups_than_a_launch_holds(qk):
+    lib = qk.load()
+    c = cache(qk, kv_heads=4096, token_stride=4096 * 128, page_stride=16 * 4096 * 128)
+    b = batch(qk, sequences=65535, tokens=65535)
+    for q_type in (0, 1):
+        assert lib.qk_paged_attention(c, b, P, q_type, 4096 * 128, 4096, 0.1, 0, 100, P, None, P, 1 << 40, None) == INVALID
+        assert lib.qk_paged_attention_workspace_size(c, b, q_type, 4096, 0, 100) == 0
