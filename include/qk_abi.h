@@ -365,10 +365,12 @@ int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float
  * is out of range, rows of that sequence are NaN (see qk_kv_cache::fault); all of
  * them, and no key is read, where its context is longer than table_stride pages
  * or than 2^30 tokens.
- * Scores, the softmax and the sums are fp32. F32 q: q and the softmax weights
- * meet the cached values as two F16 (three BF16) parts, so the result has
- * fp32's precision; 16-bit q: the weights are rounded to the cache's type for
- * the product with V, the result once at the end.
+ * Scores, the softmax and the sums are fp32. F32 q: q meets the cached keys and
+ * the softmax weights the cached values as two F16 parts (22 bits) or three BF16
+ * ones; 16-bit q: the weights are rounded to the cache's type for the product
+ * with V, the result once at the end. Over an F16 cache weights too small for that
+ * (beside one that takes nearly all of the mass) keep 20 or 11 bits, down to 2^-100
+ * of the row's sum, wherever the row's output does not outweigh what they lack.
  * max_context: the largest context the call may meet, a bound for the split of
  * long contexts over workgroups; longer ones are still right, only slower.
  * workspace: qk_paged_attention_workspace_size bytes, 256-byte aligned (may be

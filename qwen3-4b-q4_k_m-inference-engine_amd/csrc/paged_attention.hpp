@@ -10,11 +10,19 @@
 // the keys in the order that the registers hold them, and V is read in the same
 // order, transposed, by ds_read_b64_tr_b16).
 //
-// Softmax in base 2: weights are 2^(x - M + kLift), x = scale log2(e) q.k. M
-// follows the running maximum only when that grows by more than kSlack
-// (weights stay below 2^(kLift + kSlack) = 2^14, within fp16), which spares
-// nearly all rescalings of the output; kLift keeps weights down to 2^-22 of
-// the largest out of fp16's subnormals. Both cancel in the division by the sum.
+// Softmax in base 2: weights are 2^(x - M + kLift), x = scale log2(e) q.k. M, the
+// row's reference, follows the running maximum only when that grows by more than
+// kSlack (weights stay below 2^(kLift + kSlack), within fp16), which spares
+// nearly all rescalings of the output. Both cancel in the division by the sum.
+//
+// fp16 holds a weight to its last bit down to 2^-14, in two parts to 2^-20 of
+// itself down to 2^-5 (kReach below M), and smaller ones to 2^-25. That is far
+// below what counts in most rows, but not where the large weights' values are near
+// zero, as those of a first token that takes most of the mass are. So where a
+// block of keys over an F16 cache holds smaller weights, and a row's output does not
+// yet outweigh what they may lack (kSound), M sinks and what they lack is
+// added: sums and outputs are fp32 and have the range for it, down to weights of
+// 2^-100 of the row's sum. bf16 has that range itself.
 #pragma once
 
 #include "qk_device.hpp"
@@ -23,7 +31,11 @@
 
 namespace qk {
 
-constexpr float kLift = 8.0f, kSlack = 6.0f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 8.0f : 9.0f;
+constexpr float kSlack = 6.0f;
+template <int NP>  // F16, weights in NP parts
+constexpr float kReach = kLift<false> + (NP > 1 ? 5.0f : 14.0f);
 constexpr float kNoMax = -3.4028234e38f;  // the maximum of no score: no finite score is below it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -62,6 +74,16 @@ __device__ __forceinline__ uint32_t infinite_halves(uint32_t two) {  // bits 15 
 }
 template <bool BF16>
 __device__ __forceinline__ bool any_infinite(u32x4 v) {
+  if constexpr (!BF16) {  // 0 times each: zeros, or a NaN
+    typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+    H2 sum = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t two = v[i];
+      sum = __builtin_elementwise_fma(__builtin_bit_cast(H2, two), H2{}, sum);
+    }
+    return (__builtin_bit_cast(uint32_t, sum) & 0x7FFF7FFFu) != 0;
+  }
   return (infinite_halves<BF16>(v.x) | infinite_halves<BF16>(v.y) | infinite_halves<BF16>(v.z) |
           infinite_halves<BF16>(v.w)) != 0;
 }
@@ -151,6 +173,43 @@ __device__ __forceinline__ AttentionTile find_tile(const AttentionArgs& a, int t
   return t;
 }
 
+// The reference of a row over an F16 cache that has to rise to `most`. Whole numbers,
+// so that rescaling is exact; weights in two parts leave half of the room above
+// for later, larger ones, as more of the smaller ones fit below.
+template <int NP>
+__device__ __forceinline__ float risen(float top, float most) {
+  return most > top + kSlack ? ceilf(most - (NP > 1 ? kSlack / 2 : 0.0f)) : top;
+}
+// What weights of NP fp16 parts lack is at most 2^-25 each where it counts. A
+// row's output outweighs it from kSound times the largest value v on: were all of
+// 2^13 smaller weights short by that, and their values alike, it would be 2^-19
+// (two parts) or 2^-12 of the output.
+template <int NP>
+constexpr float kSound = NP > 1 ? 0x1p7f : 1.0f;
+// Up to which reference a row is sound whose output is `size` at `top`.
+template <int NP>
+__device__ __forceinline__ float sound_to(float top, float size, float largest) {
+  const int spare = __builtin_amdgcn_frexp_expf(size) - 1 - __builtin_amdgcn_frexp_expf(kSound<NP> * largest);
+  return largest == 0.0f ? __builtin_inff() : size == 0.0f ? -__builtin_inff() : top + static_cast<float>(spare);
+}
+// How far the reference of a row sinks that is not sound, its output at most `size`
+// and its sum `sum`: to where it may be, but no further than that what the weights
+// lack (2^-22 or 2^-11 of them) stays within fp16, nor at all beyond 2^112, so that
+// neither later blocks nor the join of 2048 parts leave fp32.
+template <int NP>
+__device__ __forceinline__ int sinking(float size, float sum, float largest) {
+  constexpr int kMost = NP > 1 ? 20 : 12;
+  const int lacks = __builtin_amdgcn_frexp_expf(kSound<NP> * largest) - __builtin_amdgcn_frexp_expf(size) + 3;
+  const int by = size == 0.0f || lacks > kMost ? kMost : lacks < 1 ? 1 : lacks;
+  return by + __builtin_amdgcn_frexp_expf(fmaxf(size, sum)) > 112 ? 0 : by;
+}
+// The larger of two pairs of fp16 values by their sizes, both finite.
+__device__ __forceinline__ uint32_t larger_sizes(uint32_t x, uint32_t y) {
+  typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(U2, x & 0x7FFF7FFFu),
+                                                                 __builtin_bit_cast(U2, y & 0x7FFF7FFFu)));
+}
+
 // The most keys that a row of any sequence sees.
 __device__ __forceinline__ int longest_context(const AttentionArgs& a) {
   const int lane = static_cast<int>(threadIdx.x & 63);
@@ -212,9 +271,10 @@ __device__ __forceinline__ void store_row(void* out, int64_t at, f32x4 y) {
   }
 }
 
-// A row's sum and maximum as its log of the sum of exp.
+// A row's sum and reference as its log of the sum of exp.
+template <bool BF16>
 __device__ __forceinline__ float row_lse(float top, float sum) {
-  return sum == 0.0f ? -__builtin_inff() : (top - kLift) * kLn2 + logf(sum);
+  return sum == 0.0f ? -__builtin_inff() : (top - kLift<BF16>) * kLn2 + logf(sum);
 }
 
 }  // namespace qk

@@ -228,6 +228,108 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   typedef short i16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) i16x4* LdsRow;
 
+  const auto rescale = [&](float to) {
+    const float f = __builtin_amdgcn_exp2f(top - to);
+    top = to;
+    sum *= f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
+  };
+  float sound = -__builtin_inff();  // the reference up to which the row is sound
+  const auto least_full = [&]() __attribute__((always_inline)) {  // scores below have weights that lack bits that count
+    return top > sound ? top - kReach<NP> : -__builtin_inff();
+  };
+  // q.k of the block in ks, scaled
+  const auto scores = [&](f32x4 (&x)[2]) __attribute__((always_inline)) {
+    x[0] = x[1] = f32x4{};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const V8 k = __builtin_bit_cast(V8, load16(ks + i * (16 * 2 * D) + k_chunk<D>(col, 4 * s + grp)));
+#pragma unroll
+        for (int p = 0; p < NP; ++p) x[i] = N::mfma16(k, q[s][p], x[i]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = x[i] * factor;
+  };
+  // No short circuit: a select, not a branch.
+  const auto sees = [&](int key0, int i, int r) __attribute__((always_inline)) {
+    const int key = key0 + 16 * i + 4 * grp + r;
+    return static_cast<bool>(static_cast<int>(key <= last) & static_cast<int>(key >= from));
+  };
+  const auto add_values = [&](const V8 (&w)[NP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      uint8_t* const at = vs + (tr_at ^ (d << 5));
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at + 16 * 2 * D));
+      const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) o[d] = N::mfma16(__builtin_bit_cast(V8, both), w[n], o[d]);
+    }
+  };
+  // Adds what the weights of the block in ks and vs lack to rows that are not sound,
+  // in steps of a sinking reference. Scores and weights are formed anew, the same bits.
+  const auto correct = [&](int key0) __attribute__((always_inline)) {
+    uint32_t sizes = 0;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const u32x4 v = load16(vs + i * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sizes = larger_sizes(sizes, v[e]);
+    }
+    sizes = sizes > sizes << 16 ? sizes >> 16 : sizes & 0xFFFFu;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t other = __shfl_xor(sizes, off);
+      sizes = other > sizes ? other : sizes;
+    }
+    const float largest = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sizes)));
+    float size;
+    const auto judge = [&]() __attribute__((always_inline)) {
+      size = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) size = fmaxf(size, fabsf(o[d][r]) < __builtin_inff() ? fabsf(o[d][r]) : 0.0f);
+      size = swap32_max(swap16_max(size));
+      sound = sound_to<NP>(top, size, largest);
+    };
+    judge();
+    if (!__any(top > sound)) return;
+    f32x4 x[2];
+    scores(x);
+    const float low = least_full();
+    float p[8];
+    bool lacks = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool in = sees(key0, i, r);
+        lacks |= in && x[i][r] < low;
+        p[4 * i + r] = in ? __builtin_amdgcn_exp2f(x[i][r] - (top - kLift<BF16>)) : 0.0f;
+      }
+    lacks = swap32_max(swap16_max(lacks ? 1.0f : 0.0f)) > 0.0f;
+    V8 w[NP];
+    split8<BF16, NP>(p, w);
+    for (int step = 0; step < 8; ++step) {
+      const int by = lacks && top > sound ? sinking<NP>(size, swap32_max(swap16_max(sum)), largest) : 0;
+      if (!__any(by > 0)) break;
+      rescale(top - static_cast<float>(by));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) p[e] -= static_cast<float>(w[n][e]);
+        p[e] = by > 0 ? ldexpf(p[e], by) : 0.0f;
+      }
+      split8<BF16, NP>(p, w);
+      add_values(w);
+      judge();
+    }
+  };
+
   for (int b = wave; b < blocks; b += kWaves) {
     const int key0 = c.lo + b * kBlock;
 #pragma unroll
@@ -238,51 +340,13 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     settle(next);
     load_k(next);
     look_up(next + kWaves);
-    f32x4 x[2] = {};
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const V8 k = __builtin_bit_cast(V8, load16(ks + i * (16 * 2 * D) + k_chunk<D>(col, 4 * s + grp)));
-#pragma unroll
-        for (int p = 0; p < NP; ++p) x[i] = N::mfma16(k, q[s][p], x[i]);
-      }
-    // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
+    f32x4 x[2];
+    scores(x);
     const bool whole = key0 + kBlock - 1 <= all_last && key0 + kBlock <= c.hi && key0 >= all_from;
-    float most = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[i][r] *= factor;
-        if (!whole) {
-          const int key = key0 + 16 * i + 4 * grp + r;
-          x[i][r] = key <= last && key >= from ? x[i][r] : -__builtin_inff();
-        }
-        most = fmaxf(most, x[i][r]);
-      }
-    most = swap32_max(swap16_max(most));
-    if (__any(most > top + kSlack)) {
-      const float to = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      sum *= f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
-    }
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        p[4 * i + r] = __builtin_amdgcn_exp2f(x[i][r] - (top - kLift));
-        sum += p[4 * i + r];
-      }
-    V8 w[NP];
-    split8<BF16, NP>(p, w);
-
-    // values into LDS; those of keys past the end as zeros (their weight is 0)
+    // values into LDS; those of keys past the end as zeros (their weight is 0), and
+    // where a weight may be 0, or its parts of either sign, infinite ones too
     bool odd = false;
-    if (!whole || NP > 1) {  // a weight's parts may be of either sign, or nothing
+    if (!whole || NP > 1 || !BF16) {
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
         if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
@@ -297,15 +361,42 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     }
     load_v(next);
     __builtin_amdgcn_wave_barrier();
+    // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
+    float most = -__builtin_inff(), least = __builtin_inff();
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      uint8_t* const at = vs + (tr_at ^ (d << 5));
-      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at));
-      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at + 16 * 2 * D));
-      const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int n = 0; n < NP; ++n) o[d] = N::mfma16(__builtin_bit_cast(V8, both), w[n], o[d]);
+      for (int r = 0; r < 4; ++r) {
+        if (!whole) {
+          const bool in = sees(key0, i, r);
+          if constexpr (!BF16) least = fminf(least, in ? x[i][r] : __builtin_inff());
+          x[i][r] = in ? x[i][r] : -__builtin_inff();
+        } else if constexpr (!BF16) {
+          least = fminf(least, x[i][r]);
+        }
+        most = fmaxf(most, x[i][r]);
+      }
+    if (__any(most > top + kSlack)) {
+      most = swap32_max(swap16_max(most));
+      if constexpr (BF16) {
+        rescale(fmaxf(top, most));
+      } else {
+        rescale(risen<NP>(top, most));
+      }
     }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[4 * i + r] = __builtin_amdgcn_exp2f(x[i][r] - (top - kLift<BF16>));
+        sum += p[4 * i + r];
+      }
+    V8 w[NP];
+    split8<BF16, NP>(p, w);
+    add_values(w);
+    if constexpr (!BF16)
+      if (__builtin_expect(__any(least < least_full()), 0)) correct(key0);
     __builtin_amdgcn_wave_barrier();
     if (odd) {
       // infinite or NaN values of keys that some rows do not see: 0 times them
@@ -461,7 +552,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       *reinterpret_cast<T2*>(static_cast<T*>(a.out) + at * D + pair(i)) =
           T2{static_cast<T>(y[i] * inv), static_cast<T>(y[i + 1] * inv)};
   }
-  if (a.lse && (tid & 15) == 0) a.lse[at] = row_lse(all, total);
+  if (a.lse && (tid & 15) == 0) a.lse[at] = row_lse<BF16>(all, total);
 }
 
 }  // namespace

@@ -144,18 +144,18 @@ attention_many_kernel(const AttentionArgs a) {
   int32_t page = 0;
   bool listed = true, bad = false;
   const bool looks = wave < kKeys / 64;
-  const auto key_of = [&](int n) { return min(c.lo + n * kKeys + tid, c.hi - 1); };
-  const auto look_up = [&](int n) {
+  const auto key_of = [&](int n) __attribute__((always_inline)) { return min(c.lo + n * kKeys + tid, c.hi - 1); };
+  const auto look_up = [&](int n) __attribute__((always_inline)) {
     if (n < count) page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(n) / a.kv.page_size, listed)];
   };
-  const auto settle = [&](int n) {
+  const auto settle = [&](int n) __attribute__((always_inline)) {
     if (n >= count) return;
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
     sh.place[n & (kRing - 1)][tid] = kv_place(a.kv, ok ? page : 0, key_of(n) % a.kv.page_size, head);
   };
   u32x4 kreg[NL], vreg[NL];
-  const auto load = [&](int n) {
+  const auto load = [&](int n) __attribute__((always_inline)) {
     if (n >= count) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -165,23 +165,26 @@ attention_many_kernel(const AttentionArgs a) {
     }
   };
   // registers -> LDS; values of keys past the end become zeros, and where some
-  // row does not see some key, or its weight has parts (of either sign, or
-  // none), so do infinite ones (odd)
-  const auto store = [&](int n, int buffer) {
+  // row does not see some key, or a weight's parts may be of either sign, or
+  // none, so do infinite ones (odd)
+  const auto store = [&](int n, int buffer) __attribute__((always_inline)) {
     if (n >= count) return;
     const int key0 = c.lo + n * kKeys;
     const bool edge = !(key0 + kKeys - 1 <= tile_last && key0 + kKeys <= c.hi && key0 >= tile_from);
-    if (edge || NP > 1) {
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (key0 + KPL * i + tid / LPK >= c.hi) vreg[i] = u32x4{};
+    }
+    if (edge || NP > 1 || !BF16) {
       bool odd = false;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        if (key0 + KPL * i + tid / LPK >= c.hi) vreg[i] = u32x4{};
-        if (any_infinite<BF16>(vreg[i])) {
-          odd = true;
-          vreg[i] = only_finite<BF16>(vreg[i]);
-        }
+      for (int i = 0; i < NL; ++i) odd |= any_infinite<BF16>(vreg[i]);
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vreg[i] = only_finite<BF16>(vreg[i]);
+        sh.odd[n & 3] = 1;
       }
-      if (odd) sh.odd[n & 3] = 1;
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -217,8 +220,15 @@ attention_many_kernel(const AttentionArgs a) {
       asm("" : "+v"(v_at[d][i]));
     }
 
+  const auto rescale = [&](float to) __attribute__((always_inline)) {
+    const float f = __builtin_amdgcn_exp2f(top - to);
+    top = to;
+    sum *= f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
+  };
   // blocks of 32 keys; `at`: of the block in sh.k and sh.v
-  const auto scores = [&](int at, f32x16& x) {
+  const auto scores = [&](int at, f32x16& x) __attribute__((always_inline)) {
     x = f32x16{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -227,41 +237,13 @@ attention_many_kernel(const AttentionArgs a) {
       for (int p = 0; p < NP; ++p) x = N::mfma32(k, q[s][p], x);
     }
   };
-  // The softmax step of the block whose q.k are in x and the product with its
-  // values; between the two, next to the exponentials, the scores of the next
-  // block into y. Registers 8 g + 4 e + r of x hold key 16 g + 8 e + 4 half + r.
-  const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16* y) __attribute__((always_inline)) {
-    if (!(key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from)) {  // some row does not see some key
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = key0 + (r >> 3) * 16 + (r >> 2 & 1) * 8 + 4 * half + (r & 3);
-        x[r] = key <= last && key >= from ? x[r] : -__builtin_inff();
-      }
-    }
-    float most = -__builtin_inff();
-#pragma unroll
-    for (int r = 0; r < 16; ++r) most = fmaxf(most, x[r]);
-    most = swap32_max(most) * factor;
-    if (__any(most > top + kSlack)) {
-      const float to = fmaxf(top, most), f = __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      sum *= f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
-    }
-    if (y) scores(next_at, *y);
-    const float base = kLift - top;
-    V8 w[2][NP];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * g + e], factor, base));
-        sum += p[e];
-      }
-      split8<BF16, NP>(p, w[g]);
-    }
+  // Registers 8 g + 4 e + r of a block's scores hold key 16 g + 8 e + 4 half + r.
+  // No short circuit: a select, not a branch.
+  const auto sees = [&](int key0, int r) __attribute__((always_inline)) {
+    const int key = key0 + (r >> 3) * 16 + (r >> 2 & 1) * 8 + 4 * half + (r & 3);
+    return static_cast<bool>(static_cast<int>(key <= last) & static_cast<int>(key >= from));
+  };
+  const auto add_values = [&](int at, const V8 (&w)[2][NP]) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -274,9 +256,126 @@ attention_many_kernel(const AttentionArgs a) {
         for (int p = 0; p < NP; ++p) o[d] = N::mfma32(v, w[g][p], o[d]);
       }
   };
+  // The softmax step of the block whose q.k are in x and the product with its
+  // values; between the two, next to the exponentials, the scores of the next
+  // block into y. True where weights may lack bits that count (see correct).
+  float sound = -__builtin_inff();  // the reference up to which the row is sound
+  const auto least_full = [&]() __attribute__((always_inline)) {  // scores below have weights that lack bits that count
+    return top > sound ? top - kReach<NP> : -__builtin_inff();
+  };
+  const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16* y) __attribute__((always_inline)) {
+    float most = -__builtin_inff(), least = __builtin_inff();
+    if (key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        most = fmaxf(most, x[r]);
+        if constexpr (!BF16) least = fminf(least, x[r]);
+      }
+    } else {  // some row does not see some key
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool in = sees(key0, r);
+        if constexpr (!BF16) least = fminf(least, in ? x[r] : __builtin_inff());
+        x[r] = in ? x[r] : -__builtin_inff();
+        most = fmaxf(most, x[r]);
+      }
+    }
+    most *= factor;
+    if (__any(most > top + kSlack)) {
+      most = swap32_max(most);
+      if constexpr (BF16) {
+        rescale(fmaxf(top, most));
+      } else {
+        rescale(risen<NP>(top, most));
+      }
+    }
+    const bool lacks = !BF16 && __any(least * factor < least_full());
+    if (y) scores(next_at, *y);
+    const float base = kLift<BF16> - top;
+    V8 w[2][NP];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * g + e], factor, base));
+        sum += p[e];
+      }
+      split8<BF16, NP>(p, w[g]);
+    }
+    add_values(at, w);
+    return lacks;
+  };
+  // Adds what the weights of a block lack to rows that are not sound, in steps of a
+  // sinking reference. Scores and weights are formed anew, the same bits: registers
+  // to keep them are not to be had. Looking for such weights costs nothing that
+  // shows, this 2 to 5% where scores have a spread of 1.5 (512 tokens over 4096 keys,
+  // F32 q: 83 to 87 us), a quarter at twice that (105) and with a first token that
+  // takes nearly all of the mass (99). In the same place, without asking whether
+  // a row is sound: 277 and 109.
+  const auto correct = [&](int key0, int at) __attribute__((always_inline)) {
+    uint32_t sizes = 0;
+#pragma unroll
+    for (int i = 0; i < 32 * 2 * D / 1024; ++i) {
+      const u32x4 v = load16(sh.v[0] + part * (32 * 2 * D) + at + i * 1024 + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sizes = larger_sizes(sizes, v[e]);
+    }
+    sizes = sizes > sizes << 16 ? sizes >> 16 : sizes & 0xFFFFu;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t other = __shfl_xor(sizes, off);
+      sizes = other > sizes ? other : sizes;
+    }
+    const float largest = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sizes)));
+    float size;
+    const auto judge = [&]() __attribute__((always_inline)) {
+      size = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) size = fmaxf(size, fabsf(o[d][r]) < __builtin_inff() ? fabsf(o[d][r]) : 0.0f);
+      size = swap32_max(size);
+      sound = sound_to<NP>(top, size, largest);
+    };
+    judge();
+    if (!__any(top > sound)) return;
+    f32x16 x;
+    scores(at, x);
+    const float base = kLift<BF16> - top, low = least_full();
+    float p[2][8];
+    bool lacks = false;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool in = sees(key0, r);
+      lacks |= in && x[r] * factor < low;
+      p[r / 8][r % 8] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], factor, base)) : 0.0f;
+    }
+    lacks = swap32_max(lacks ? 1.0f : 0.0f) > 0.0f;
+    V8 w[2][NP];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) split8<BF16, NP>(p[g], w[g]);
+    for (int step = 0; step < 8; ++step) {
+      const int by = lacks && top > sound ? sinking<NP>(size, swap32_max(sum), largest) : 0;
+      if (!__any(by > 0)) break;
+      rescale(top - static_cast<float>(by));
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+          for (int n = 0; n < NP; ++n) p[g][e] -= static_cast<float>(w[g][n][e]);
+          p[g][e] = by > 0 ? ldexpf(p[g][e], by) : 0.0f;
+        }
+        split8<BF16, NP>(p[g], w[g]);
+      }
+      add_values(at, w);
+      judge();
+    }
+  };
   // infinite or NaN values went into the product as zeros (0 times them is no
   // zero); the rows that see them get them here
-  const auto add_infinite = [&](int n) {
+  const auto add_infinite = [&](int n) __attribute__((always_inline)) {
     for (int m = 0; m < kKeys / KG; ++m) {
       const int key = c.lo + n * kKeys + part * 32 + m;
       if (key >= c.hi) break;
@@ -329,9 +428,11 @@ attention_many_kernel(const AttentionArgs a) {
         const auto both = [&](auto buffer) __attribute__((always_inline)) {
           constexpr int at = decltype(buffer)::value * kTile, next = (decltype(buffer)::value + 1) % 3;
           const int key0 = c.lo + n * kKeys;
-          attend(key0, at, x0, at + 32 * 2 * D, &x1);
+          const bool lacks0 = attend(key0, at, x0, at + 32 * 2 * D, &x1);
+          if (__builtin_expect(lacks0, 0)) correct(key0, at);
           advance(n, next);
-          attend(key0 + 32, at + 32 * 2 * D, x1, next * kTile, &x0);
+          const bool lacks1 = attend(key0 + 32, at + 32 * 2 * D, x1, next * kTile, &x0);
+          if (__builtin_expect(lacks1, 0)) correct(key0 + 32, at + 32 * 2 * D);
           if (sh.odd[n & 3]) add_infinite(n);
           return ++n < end;
         };
@@ -348,7 +449,8 @@ attention_many_kernel(const AttentionArgs a) {
         const auto one = [&](auto buffer, f32x16& x, f32x16& y) __attribute__((always_inline)) {
           constexpr int at = decltype(buffer)::value * kTile, next = (decltype(buffer)::value + 1) % 3;
           advance(n, next);
-          attend(c.lo + n * kKeys + 32 * part, at, x, next * kTile, &y);
+          const bool lacks = attend(c.lo + n * kKeys + 32 * part, at, x, next * kTile, &y);
+          if (__builtin_expect(lacks, 0)) correct(c.lo + n * kKeys + 32 * part, at);
           if (sh.odd[n & 3]) add_infinite(n);
           return ++n < end;
         };
@@ -365,7 +467,8 @@ attention_many_kernel(const AttentionArgs a) {
         advance(n, decltype(buffer)::value ^ 1);
         f32x16 x;
         scores(at, x);
-        attend(c.lo + n * kKeys + 32 * part, at, x, 0, nullptr);
+        const bool lacks = attend(c.lo + n * kKeys + 32 * part, at, x, 0, nullptr);
+        if (__builtin_expect(lacks, 0)) correct(c.lo + n * kKeys + 32 * part, at);
         if (sh.odd[n & 3]) add_infinite(n);
         return ++n < end;
       };
@@ -440,7 +543,7 @@ attention_many_kernel(const AttentionArgs a) {
     const int64_t at = out_at * D + (part * kQuads + q) * 8 + 4 * half;
     store_row<BF16, Q32>(a.out, at, y[q] * inv);
   }
-  if (a.lse && half == 0 && part == 0) a.lse[out_at] = row_lse(top, sum);
+  if (a.lse && half == 0 && part == 0) a.lse[out_at] = row_lse<BF16>(top, sum);
 }
 
 // Joins the parts of rows whose keys several workgroups took, 32 rows a
@@ -476,7 +579,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
   for (int q = 0; q < kQuads; ++q) store_row<BF16, Q32>(a.out, out_at * D + (wave * kQuads + q) * 8 + 4 * half, y[q] * inv);
-  if (a.lse && half == 0 && wave == 0) a.lse[out_at] = row_lse(all, total);
+  if (a.lse && half == 0 && wave == 0) a.lse[out_at] = row_lse<BF16>(all, total);
 }
 
 template <int D>

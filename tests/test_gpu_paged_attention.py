@@ -602,3 +602,106 @@ def test_a_last_sequence_without_rows_is_reported(gpu):
         assert p.fault() == gpu.KV_FAULT_LENGTH
         p.dev["fault"].upload(np.zeros(1, np.uint32))
         a.check()
+
+
+class Sinks(Attend):
+    """Attend, with keys that the queries prefer by about `gaps` nats each and whose values are nothing."""
+
+    def __init__(self, qk, p, q_heads, gaps, at, *, noise=0.12, value=0.0, **more):
+        kind, D = p.kind, p.dim
+        u = np.sign(p.rng.standard_normal(D)) / math.sqrt(D)
+        p.k = ref.encode(ref.decode(p.k, kind) * noise, kind)
+        K, V = p.seen(p.k), p.seen(p.v)
+        for s, c in enumerate(p.contexts):
+            for gap, pos in zip(gaps, at):
+                if pos < c:
+                    place = p.table[s, pos // p.page], pos % p.page
+                    K[place] = ref.encode(u * (gap / 8), kind)
+                    V[place] = ref.encode(ref.decode(V[place], kind) * value, kind)
+        super().__init__(qk, p, q_heads, scale=1.0, q_size=1.0, **more)
+        q = ref.decode(self.q, self.q_type)
+        q[:, :q_heads * D] += np.tile(8 * u, q_heads)
+        self.q = ref.encode(q, self.q_type)
+        self.qd.upload(self.q)
+
+
+# where the kernels differ: single tokens, drafts, prompts whose keys lie in one
+# workgroup, in waves of it, in several workgroups
+SINKS = {
+    "single": dict(new=[1, 1], contexts=[300, 47], q_heads=8),
+    "single-parts": dict(new=[1], contexts=[5000], q_heads=8, page=64),
+    "drafts": dict(new=[4, 3], contexts=[700, 33], q_heads=8),
+    "window": dict(new=[3, 90], contexts=[700, 300], q_heads=8, window=250),
+    "prompt": dict(new=[150], contexts=[400], q_heads=8),
+    "prompt-parts": dict(new=[100, 40], contexts=[900, 90], q_heads=8, max_context=6000),
+    "prompt-wide": dict(new=[60], contexts=[330], q_heads=96, kv_heads=96, max_context=700),
+    "prompt-pairs": dict(new=[60], contexts=[330], q_heads=80, kv_heads=80, max_context=400),
+}
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("name", SINKS)
+def test_weights_beside_much_larger_ones_keep_their_precision(gpu, name, types):
+    """Keys that take nearly all of the mass and have values of nothing: the rest
+    of the row, down to 2^-90 of the mass, is all of the result."""
+    kind, q_type = TYPES[types]
+    case = dict(SINKS[name])
+    q_heads, window, bound = case.pop("q_heads"), case.pop("window", 0), case.pop("max_context", None)
+    for i, (gaps, at, value) in enumerate((([10], [0], 0.0), ([14], [0], 1e-6), ([18], [0], 0.0), ([25, 12], [0, 5], 0.0),
+                                           ([12, 30, 45, 20], [2, 130, 61, 64], 0.0), ([55], [33], 0.0),
+                                           ([60, 38, 18], [0, 1, 2], 0.0))):
+        dim = 128 if i % 2 == 0 else 64
+        print(f"[case] attention sinks {name} {types} {gaps} at {at} dim={dim}", flush=True)
+        p = Paged(kind=kind, dim=dim, seed=40 + i, **case)
+        a = Sinks(gpu, p, q_heads, gaps, at, value=value, q_type=q_type, window=window, max_context=bound)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("name", ["single", "drafts", "prompt", "prompt-parts"])
+def test_large_weights_of_small_values_and_the_rest(gpu, name, types):
+    """Values between nothing and those of the rest: what the rest adds is a part
+    of the result, of any size."""
+    kind, q_type = TYPES[types]
+    case = dict(SINKS[name])
+    q_heads, bound = case.pop("q_heads"), case.pop("max_context", None)
+    for i, (gap, at, value) in enumerate(((14, 0, 0.3), (14, 40, 0.05), (14, 0, 2.0 ** -8), (25, 0, 0.05), (25, 33, 2.0 ** -10),
+                                          (40, 0, 2.0 ** -14))):
+        print(f"[case] attention small values {name} {types} {gap} at {at} value={value}", flush=True)
+        p = Paged(kind=kind, dim=128 if i % 2 == 0 else 64, seed=70 + i, **case)
+        a = Sinks(gpu, p, q_heads, [gap], [at], value=value, q_type=q_type, max_context=bound)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("new", [1, 4, 100])
+def test_scores_of_any_spread_keep_their_precision(gpu, new, types):
+    """Weights over tens of powers of two in every block of keys."""
+    kind, q_type = TYPES[types]
+    for i, (size, bound) in enumerate(((4.0, None), (9.0, None), (9.0, 6000), (25.0, None))):
+        print(f"[case] attention spread {size} {types} new={new} bound={bound}", flush=True)
+        p = Paged([new], [new + 400], kind=kind, dim=128 if i % 2 == 0 else 64, seed=50 + i)
+        a = Attend(gpu, p, 8, q_type=q_type, q_size=size, max_context=bound)
+        a.call()
+        gpu.synchronize()
+        a.check()
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_an_infinite_value_of_a_tiny_weight(gpu, types):
+    """Infinity times any weight is infinity, in blocks of keys that all rows see too."""
+    kind, q_type = TYPES[types]
+    for new, contexts, bound in (([1], [600], None), ([100], [600], None), ([100], [600], 6000)):
+        for gap, at in ((0, 0), (14, 0), (20, 33), (30, 0), (35, 33)):  # 33: in the same 32 keys
+            print(f"[case] attention infinite value {types} new={new} gap={gap} at {at} bound={bound}", flush=True)
+            p = Paged(new, contexts, kind=kind, dim=128, seed=60)
+            p.seen(p.v)[p.table[0, 40 // p.page], 40 % p.page, :, 7] = ref.encode(np.inf, kind)
+            a = Sinks(gpu, p, 8, [gap], [at], q_type=q_type, max_context=bound)
+            a.call()
+            gpu.synchronize()
+            out = ref.decode(a.results()[0], q_type)
+            assert (out[:, :, 7] == np.inf).all() and np.isfinite(np.delete(out, 7, axis=2)).all()
