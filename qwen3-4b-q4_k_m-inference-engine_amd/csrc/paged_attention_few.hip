@@ -239,8 +239,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const auto least_full = [&]() __attribute__((always_inline)) {  // scores below have weights that lack bits that count
     return top > sound ? top - kReach<NP> : -__builtin_inff();
   };
-  // q.k of the block in ks, scaled
+  // q.k of the block in ks, scaled: by products of their own, so that weights formed
+  // of them twice are the same bits
   const auto scores = [&](f32x4 (&x)[2]) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
     x[0] = x[1] = f32x4{};
 #pragma unroll
     for (int s = 0; s < KS; ++s)
