@@ -367,8 +367,9 @@ int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float
  * or than 2^30 tokens.
  * Scores, the softmax and the sums are fp32. F32 q: q meets the cached keys and
  * the softmax weights the cached values as two F16 parts (22 bits) or three BF16
- * ones; 16-bit q: the weights are rounded to the cache's type for the product
- * with V, the result once at the end. Over an F16 cache weights too small for that
+ * ones; 16-bit q: the weights are two such parts where there are few new tokens a
+ * sequence (single ones, drafts), and else rounded to the cache's type for the
+ * product with V; the result once at the end. Over an F16 cache weights too small for that
  * (beside one that takes nearly all of the mass) keep 20 or 11 bits, down to 2^-100
  * of the row's sum, wherever the row's output does not outweigh what they lack.
  * max_context: the largest context the call may meet, a bound for the split of

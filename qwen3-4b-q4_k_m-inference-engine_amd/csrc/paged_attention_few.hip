@@ -87,6 +87,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   typedef typename N::T T;
   typedef typename N::V8 V8;
   constexpr int NP = kParts<BF16, Q32>;
+  // Parts of a weight: two with 16-bit q as well, as the matrix cores are idle nine
+  // tenths of the time (three contexts of 131072, BF16: 153 and 156 us, error of the
+  // result 2.3e-3 and 1.6e-3, half a step).
+  constexpr int NW = NP > 1 ? NP : 2;
   constexpr int KS = D / 32, DT = D / 16;    // k steps of q.k, 16-wide tiles of the output
   constexpr int LPK = D / 8;                 // lanes that load one key's values
   constexpr int VL = kBlock * LPK / 64;      // loads of a block's values
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   };
   float sound = -__builtin_inff();  // the reference up to which the row is sound
   const auto least_full = [&]() __attribute__((always_inline)) {  // scores below have weights that lack bits that count
-    return top > sound ? top - kReach<NP> : -__builtin_inff();
+    return top > sound ? top - kReach<NW> : -__builtin_inff();
   };
   // q.k of the block in ks, scaled: by products of their own, so that weights formed
   // of them twice are the same bits
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     const int key = key0 + 16 * i + 4 * grp + r;
     return static_cast<bool>(static_cast<int>(key <= last) & static_cast<int>(key >= from));
   };
-  const auto add_values = [&](const V8 (&w)[NP]) __attribute__((always_inline)) {
+  const auto add_values = [&](const V8 (&w)[NW]) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       uint8_t* const at = vs + (tr_at ^ (d << 5));
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRow)(at + 16 * 2 * D));
       const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int n = 0; n < NP; ++n) o[d] = N::mfma16(__builtin_bit_cast(V8, both), w[n], o[d]);
+      for (int n = 0; n < NW; ++n) o[d] = N::mfma16(__builtin_bit_cast(V8, both), w[n], o[d]);
     }
   };
   // Adds what the weights of the block in ks and vs lack to rows that are not sound,
@@ -296,7 +300,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
 #pragma unroll
         for (int r = 0; r < 4; ++r) size = fmaxf(size, fabsf(o[d][r]) < __builtin_inff() ? fabsf(o[d][r]) : 0.0f);
       size = swap32_max(swap16_max(size));
-      sound = sound_to<NP>(top, size, largest);
+      sound = sound_to<NW>(top, size, largest);
     };
     judge();
     if (!__any(top > sound)) return;
@@ -314,19 +318,19 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
         p[4 * i + r] = in ? __builtin_amdgcn_exp2f(x[i][r] - (top - kLift<BF16>)) : 0.0f;
       }
     lacks = swap32_max(swap16_max(lacks ? 1.0f : 0.0f)) > 0.0f;
-    V8 w[NP];
-    split8<BF16, NP>(p, w);
+    V8 w[NW];
+    split8<BF16, NW>(p, w);
     for (int step = 0; step < 8; ++step) {
-      const int by = lacks && top > sound ? sinking<NP>(size, swap32_max(swap16_max(sum)), largest) : 0;
+      const int by = lacks && top > sound ? sinking<NW>(size, swap32_max(swap16_max(sum)), largest) : 0;
       if (!__any(by > 0)) break;
       rescale(top - static_cast<float>(by));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) p[e] -= static_cast<float>(w[n][e]);
+        for (int n = 0; n < NW; ++n) p[e] -= static_cast<float>(w[n][e]);
         p[e] = by > 0 ? ldexpf(p[e], by) : 0.0f;
       }
-      split8<BF16, NP>(p, w);
+      split8<BF16, NW>(p, w);
       add_values(w);
       judge();
     }
@@ -348,14 +352,12 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     // values into LDS; those of keys past the end as zeros (their weight is 0), and
     // where a weight may be 0, or its parts of either sign, infinite ones too
     bool odd = false;
-    if (!whole || NP > 1 || !BF16) {
 #pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
-        odd |= any_infinite<BF16>(vreg[i]);
-      }
-      odd = __any(odd);
+    for (int i = 0; i < VL; ++i) {
+      if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
+      odd |= any_infinite<BF16>(vreg[i]);
     }
+    odd = __any(odd);
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       const int key = KPL * i + lane / LPK;
@@ -383,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       if constexpr (BF16) {
         rescale(fmaxf(top, most));
       } else {
-        rescale(risen<NP>(top, most));
+        rescale(risen<NW>(top, most));
       }
     }
     float p[8];
@@ -394,8 +396,8 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
         p[4 * i + r] = __builtin_amdgcn_exp2f(x[i][r] - (top - kLift<BF16>));
         sum += p[4 * i + r];
       }
-    V8 w[NP];
-    split8<BF16, NP>(p, w);
+    V8 w[NW];
+    split8<BF16, NW>(p, w);
     add_values(w);
     if constexpr (!BF16)
       if (__builtin_expect(__any(least < least_full()), 0)) correct(key0);

@@ -705,3 +705,28 @@ def test_an_infinite_value_of_a_tiny_weight(gpu, types):
             gpu.synchronize()
             out = ref.decode(a.results()[0], q_type)
             assert (out[:, :, 7] == np.inf).all() and np.isfinite(np.delete(out, 7, axis=2)).all()
+
+
+@pytest.mark.parametrize("types", ["f16-f16", "bf16-bf16"])
+@pytest.mark.parametrize("name", ["decode", "decode-long", "drafts"])
+def test_single_tokens_round_once(gpu, name, types):
+    """Few new tokens, 16-bit q: the result is within half a step of the type, and
+    what weights of two parts (2^-16 of BF16, 2^-20 of F16) and the sums are off by."""
+    kind, q_type = TYPES[types]
+    case = dict(CASES[name])
+    q_heads = case.pop("q_heads")
+    for dim in (64, 128):
+        p = Paged(kind=kind, dim=dim, seed=80 + dim, **case)
+        a = Attend(gpu, p, q_heads, q_type=q_type)
+        a.call()
+        gpu.synchronize()
+        got, step = ref.decode(a.results()[0], q_type), ref.HALF_STEP[q_type]
+        for s, (n, c) in enumerate(zip(p.new, p.contexts)):
+            rows = slice(p.start[s], p.start[s] + n)
+            q = ref.decode(a.q[rows].reshape(n, q_heads, dim), q_type)
+            K, V = (ref.decode(p.rows(s, pool), kind) for pool in (p.k, p.v))
+            out, _, weight, reach = ref.attention(q, K, V, c - n, float(a.scale), 0)
+            e = ((dim / 4 + 6) * reach + 4) * U + (2.0 ** -16 if kind == BF16 else 2.0 ** -20)
+            off = (2 * e + (64 + math.sqrt(c)) * U)[..., None] * weight
+            off = off + step * (np.abs(out) + off) + ref.TINY[q_type]
+            assert (np.abs(got[rows] - out) <= off).all(), s
