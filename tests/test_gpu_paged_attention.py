@@ -730,3 +730,18 @@ def test_single_tokens_round_once(gpu, name, types):
             off = (2 * e + (64 + math.sqrt(c)) * U)[..., None] * weight
             off = off + step * (np.abs(out) + off) + ref.TINY[q_type]
             assert (np.abs(got[rows] - out) <= off).all(), s
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_single_tokens_beside_a_long_chunk(gpu, types):
+    """A chunk of a prompt among decode rows in one call: one kernel takes both."""
+    kind, q_type = TYPES[types]
+    for new, contexts, bound in (([1] * 40 + [300] + [1] * 23, [5 + 31 * i for i in range(40)] + [700] + [400] * 23, 1300),
+                                 ([200] + [1] * 9, [260] + [3000] + [90] * 8, 4000)):
+        print(f"[case] attention singles and a chunk {types} {len(new)} sequences", flush=True)
+        p = Paged(new, contexts, kv_heads=2, kind=kind, dim=64, seed=90 + len(new))
+        a = Attend(gpu, p, 8, q_type=q_type, max_context=bound)
+        a.call()
+        a.call()
+        gpu.synchronize()
+        a.check()
