@@ -410,8 +410,10 @@ int qk_kv_check(const qk_kv_cache *cache, qk_stream_t stream);
  * argmax. NaN and -inf are never drawn; 0xFFFFFFFF if a row has nothing else;
  * of +inf logits each weighs 1 and the rest nothing. probability (NULL, or
  * float[rows]) receives the drawn token's share of the kept sum (0 if none).
- * Weights are 64-bit, their sums exact in fixed point, so a result does not
- * depend on the order of any sum. vocabulary in [1, 2^24]; row_stride >= vocabulary.
+ * Weights are 64-bit exponentials rounded to multiples of 2^-44 of the largest
+ * (above 2^18 logits coarser, 2^-38 at 2^24; what rounds to nothing is not drawn),
+ * their sums exact, so a result does not depend on the order of any sum.
+ * vocabulary in [1, 2^24]; row_stride >= vocabulary.
  * workspace: qk_sample_workspace_size bytes, 256-byte aligned (may be NULL
  * when that is 0), zero-filled once; every call leaves it ready for the next, of
  * this batch or another; calls that may run concurrently need separate ones.

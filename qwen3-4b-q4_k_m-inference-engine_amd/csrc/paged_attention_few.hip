@@ -10,7 +10,7 @@
 // wave are in flight under the arithmetic.
 // Loads take whole rows (256 bytes a key, 16 lanes) and are marked as not used
 // again: this card's plain reads reach 6.4 TB/s, those 7.2. 64 sequences of up to
-// 8192 keys, 1.06 GB: 175 us (6.1 TB/s), 3 of 131072: 154 (5.7); before the
+// 8192 keys, 1.06 GB: 175 us (6.1 TB/s), 3 of 131072: 156 (5.6); before the
 // sequences were taken by length 225, and 263 with keys loaded straight into the
 // operand's layout (64 bytes of a row an instruction).
 #include "paged_attention.hpp"

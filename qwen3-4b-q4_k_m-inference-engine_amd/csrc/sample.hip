@@ -27,7 +27,7 @@
 // its own and scaled once per band, in 64-bit floating point. Bands only say
 // where to look; no result depends on their width.
 // Measured: one row of 151936, top-k 20 and top-p 0.95: 15 us; 200 rows: greedy 24
-// (5.0 TB/s), top-k 20 37, filters of their own (a fifth without top-k) 82.
+// (5.0 TB/s), top-k 20 37, filters of their own (a fifth without top-k) 80.
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -36,7 +36,7 @@ namespace qk {
 namespace {
 
 constexpr int kThreads = 1024;     // of the draw
-constexpr int kBins = 2048;        // of a digit; of a band, half as many
+constexpr int kBins = 2048;        // of a digit
 constexpr int kScanThreads = 256;
 constexpr int kBands = 128;
 constexpr int kList = 512;         // most listed logits of a chunk
