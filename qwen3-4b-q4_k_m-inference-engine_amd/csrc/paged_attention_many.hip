@@ -256,13 +256,13 @@ attention_many_kernel(const AttentionArgs a) {
         for (int p = 0; p < NP; ++p) o[d] = N::mfma32(v, w[g][p], o[d]);
       }
   };
-  // The softmax step of the block whose q.k are in x and the product with its
-  // values; between the two, next to the exponentials, the scores of the next
-  // block into y. True where weights may lack bits that count (see correct).
   float sound = -__builtin_inff();  // the reference up to which the row is sound
   const auto least_full = [&]() __attribute__((always_inline)) {  // scores below have weights that lack bits that count
     return top > sound ? top - kReach<NP> : -__builtin_inff();
   };
+  // The softmax step of the block whose q.k are in x and the product with its
+  // values; between the two, next to the exponentials, the scores of the next
+  // block into y. True where weights may lack bits that count (see correct).
   const auto attend = [&](int key0, int at, f32x16& x, int next_at, f32x16* y) __attribute__((always_inline)) {
     float most = -__builtin_inff(), least = __builtin_inff();
     if (key0 + 31 <= wave_last && key0 + 32 <= c.hi && key0 >= wave_from) {
