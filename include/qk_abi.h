@@ -34,6 +34,7 @@ enum qk_status {
 enum qk_type {
     QK_TYPE_F32 = 0,
     QK_TYPE_F16 = 1,
+    QK_TYPE_Q4_1 = 3, /* caches only */
     QK_TYPE_Q4_K = 12,
     QK_TYPE_Q6_K = 14,
     QK_TYPE_BF16 = 30 /* caches and attention rows only */
@@ -278,11 +279,19 @@ int qk_matmul_argmax(const float *x, const void *w, int type, int64_t K, int64_t
  * ------------------------------------------------------------------------- */
 
 /* One layer's cache: `pages` pages of `page_size` tokens (any size from 1 to
- * 65536), keys in k and values in v, both F16 or BF16 (`type`) and laid out
+ * 65536), keys in k and values in v, both F16, BF16 or Q4_1 (`type`) and laid out
  * alike: the head_dim values of token slot t of page p and head h start at
  * p*page_stride + t*token_stride + h*head_stride (elements; multiples of 8, so
  * that every row is 16-byte aligned; tokens outside heads or heads outside
  * tokens). head_dim is 64 or 128.
+ * Q4_1: a row is head_dim/32 blocks of 20 bytes (80 bytes for 128 values): F16 d,
+ * F16 m, then 16 bytes of codes, byte j with the code of value j in bits 0..3 and
+ * of value j + 16 in bits 4..7, as in GGUF files; a code c stands for d*c + m, rounded
+ * once to F16. Strides still count values (multiples of 32, each 32 of them 20
+ * bytes); q and rows read out are F32 or F16. Written by qk_kv_append: m is the least
+ * value rounded to F16, d the rest of the block's range over 15, rounded to F16
+ * towards zero, codes the nearest (at most d/2 off, and what d and m lack to their
+ * roundings). A block with a NaN, or with a value beyond F16's range, is NaN as a whole.
  * fault: NULL, or a device word that the calls on this cache OR bits into (the
  * caller clears it once): QK_KV_FAULT_PAGE, a page id outside [0, pages) or a
  * position beyond the sequence's page table was met; QK_KV_FAULT_LENGTH,
@@ -351,6 +360,23 @@ int qk_kv_append(const qk_kv_cache *cache, const qk_kv_batch *batch, const float
                  int64_t q_stride, const float *k, int64_t k_stride, const float *v,
                  int64_t v_stride, int64_t q_heads, const qk_rope *rope, void *q_out, int q_type,
                  qk_stream_t stream);
+
+/* qk_kv_append for sequences that have lost tokens (qk_kv_evict): seen[sequences]
+ * (device; NULL: the contexts) counts the tokens that a sequence has had, up to and
+ * with its new ones, so that its new token i of n is rotated for position
+ * seen - n + i, wherever in the cache it goes (context - n + i, as ever). */
+int qk_kv_append_at(const qk_kv_cache *cache, const qk_kv_batch *batch, const int32_t *seen,
+                    const float *q, int64_t q_stride, const float *k, int64_t k_stride,
+                    const float *v, int64_t v_stride, int64_t q_heads, const qk_rope *rope,
+                    void *q_out, int q_type, qk_stream_t stream);
+
+/* The cached rows of the batch's new tokens out of their pages: k_out and v_out
+ * [tokens x kv_heads x head_dim] (either may be NULL) of out_type, F32 or the
+ * cache's type (F16 for Q4_1); exact in both. With token_start of whole contexts
+ * it reads whole sequences. Rows that no sequence owns are left alone; rows whose
+ * page id or position is out of range are NaN (see qk_kv_cache::fault). */
+int qk_kv_rows(const qk_kv_cache *cache, const qk_kv_batch *batch, void *k_out, void *v_out,
+               int out_type, qk_stream_t stream);
 
 /* out [tokens x q_heads x head_dim] = softmax(scale * q . K^T) . V for the new
  * tokens over their sequences' cached tokens: a token at position t sees the

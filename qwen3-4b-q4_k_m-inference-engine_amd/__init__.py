@@ -32,11 +32,13 @@ QK_ERR_OUT_OF_MEMORY = 4
 
 TYPE_F32 = 0
 TYPE_F16 = 1
+TYPE_Q4_1 = 3
 TYPE_Q4_K = 12
 TYPE_Q6_K = 14
 TYPE_BF16 = 30
 KV_FAULT_PAGE = 1
 KV_FAULT_LENGTH = 2
+Q4_1_VALUES, Q4_1_BYTES = 32, 20  # of a cache's block
 SUPERBLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210}
 QK = 256
 Q8_BLOCK_BYTES = 48
@@ -111,6 +113,9 @@ _SIGNATURES = {
                          _size, _c_void_p],
     "qk_kv_append": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
                      _i64, _i64, ctypes.POINTER(Rope), _c_void_p, _int, _c_void_p],
+    "qk_kv_append_at": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+                        _c_void_p, _i64, _i64, ctypes.POINTER(Rope), _c_void_p, _int, _c_void_p],
+    "qk_kv_rows": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _c_void_p, _int, _c_void_p],
     "qk_paged_attention": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _int, _i64, _i64, _float,
                            _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
     "qk_paged_attention_workspace_size": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _int, _i64, _i64, _i64],
@@ -512,6 +517,18 @@ def kv_append(cache: KVCache, batch: KVBatch, q, q_stride: int, k, k_stride: int
     """qk_kv_append: keys and values of the new tokens into their pages, q and k normed and rotated on the way."""
     check(load().qk_kv_append(cache, batch, _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride, q_heads, rope,
                               _ptr(q_out), q_type, _stream_ptr(stream)))
+
+
+def kv_append_at(cache: KVCache, batch: KVBatch, seen, q, q_stride: int, k, k_stride: int, v, v_stride: int,
+                 q_heads: int, rope: Rope | None, q_out, q_type: int, stream=None) -> None:
+    """qk_kv_append_at: kv_append, positions counted by `seen` where tokens were evicted."""
+    check(load().qk_kv_append_at(cache, batch, _ptr(seen), _ptr(q), q_stride, _ptr(k), k_stride, _ptr(v), v_stride,
+                                 q_heads, rope, _ptr(q_out), q_type, _stream_ptr(stream)))
+
+
+def kv_rows(cache: KVCache, batch: KVBatch, k_out, v_out, out_type: int, stream=None) -> None:
+    """qk_kv_rows: the new tokens' cached keys and values as rows of F32 or of the cache's 16-bit type."""
+    check(load().qk_kv_rows(cache, batch, _ptr(k_out), _ptr(v_out), out_type, _stream_ptr(stream)))
 
 
 def paged_attention_workspace_size(cache: KVCache, batch: KVBatch, q_type: int, q_heads: int, window: int,

@@ -16,6 +16,10 @@
 // Memory bounds long prompts: 4096 tokens of 32 + 2 x 8 heads of 128, 184 MB, 38 us
 // (4.8 TB/s, a copy's rate); launch and three dependent reads (lengths, page id,
 // values) a decode step: one token 2.7 us, 64 3.9.
+//
+// Q4_1 caches: a finished row goes through LDS, from where each lane takes four
+// values and the four 16 further on, the codes of one dword, four lanes a block.
+#include "q4_1.hpp"
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -31,10 +35,49 @@ __device__ __forceinline__ uint16_t narrow(float v) {
     return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
 
-template <int D, bool BF16, bool Q32>
+// A row's lane of a Q4_1 cache: x0 its values 4 u .. of block `u / 4`, x1 the ones 16
+// on, u = lane of the block. The block's d and m are rounded first (d towards zero,
+// so that no value leaves F16), and the codes go by them. fp32, as the row is: a value
+// that near a border between two codes may come out as the other one.
+__device__ __forceinline__ void store_q4(uint8_t* row, int u, f32x4 x0, f32x4 x1) {
+  float low = fminf(fminf(fminf(x0[0], x0[1]), fminf(x0[2], x0[3])), fminf(fminf(x1[0], x1[1]), fminf(x1[2], x1[3])));
+  float high = fmaxf(fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3])), fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3])));
+  float zeros = 0.0f;  // or NaN, if a value is NaN or infinite
+#pragma unroll
+  for (int i = 0; i < 4; ++i) zeros += 0.0f * x0[i] + 0.0f * x1[i];
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    low = fminf(low, __shfl_xor(low, off));
+    high = fmaxf(high, __shfl_xor(high, off));
+    zeros += __shfl_xor(zeros, off);
+  }
+  const _Float16 m = static_cast<_Float16>(low);
+  const float base = static_cast<float>(m), span = fmaxf(high - base, 0.0f) / 15.0f;
+  _Float16 d = static_cast<_Float16>(span);
+  uint32_t d_bits = __builtin_bit_cast(uint16_t, d);
+  if (static_cast<float>(d) > span) --d_bits;
+  const float step = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d_bits)));
+  const float inverse = step == 0.0f ? 0.0f : 1.0f / step;
+  const float top = static_cast<float>(static_cast<_Float16>(high));
+  const bool broken = !(zeros == 0.0f) || fabsf(base) == __builtin_inff() || fabsf(top) == __builtin_inff();
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = static_cast<uint32_t>(fminf(fmaxf(rintf((x0[i] - base) * inverse), 0.0f), 15.0f));
+    const uint32_t hi = static_cast<uint32_t>(fminf(fmaxf(rintf((x1[i] - base) * inverse), 0.0f), 15.0f));
+    codes |= (lo | hi << 4) << (8 * i);
+  }
+  uint8_t* block = row + (u >> 2) * kQ4Bytes;
+  *reinterpret_cast<uint32_t*>(block + 4 + 4 * (u & 3)) = broken ? 0u : codes;
+  if ((u & 3) == 0)
+    *reinterpret_cast<uint32_t*>(block) = broken ? 0x7E007E00u : d_bits | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, m)) << 16;
+}
+
+template <int D, bool BF16, bool Q32, bool Q4>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   constexpr int L = D / 8;  // lanes a row
   __shared__ float cosine[D / 2], sine[D / 2];
+  __shared__ __attribute__((aligned(16))) float finished[Q4 ? 256 * 8 : 4];  // a Q4_1 cache's rows
   const int tid = static_cast<int>(threadIdx.x);
   const int token = static_cast<int>(blockIdx.x);
   const int row = static_cast<int>(blockIdx.y) * (256 / L) + tid / L;
@@ -63,7 +106,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   if (token < seq.row || token >= seq.row + seq.count) return;  // no sequence owns this row
   const int position = seq.first + (token - seq.row);
   if (tid < a.dims / 2) {
-    const double turns = position * (exp2(a.turns_log2 * tid) * 0.15915494309189535);
+    // where tokens were evicted, a token's position is not its place in the cache
+    const int64_t angle = a.seen ? static_cast<int64_t>(a.seen[s]) - a.kv.context[s] + position : position;
+    const double turns = static_cast<double>(angle) * (exp2(a.turns_log2 * tid) * 0.15915494309189535);
     const float part = static_cast<float>(turns - floor(turns));
     float sn, cs;
     sincospif(2.0f * part, &sn, &cs);
@@ -109,7 +154,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     *reinterpret_cast<f32x4*>(out + second) = x1;
     return;
   }
-  uint16_t* out;
+  uint16_t* out = nullptr;
+  int64_t place = 0;
   if (is_q) {
     out = static_cast<uint16_t*>(a.q_out) + (static_cast<int64_t>(token) * a.q_heads + head) * D;
   } else {
@@ -119,7 +165,21 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
       if (u == 0) kv_fault(a.kv, position < 0 ? QK_KV_FAULT_LENGTH : QK_KV_FAULT_PAGE);
       return;
     }
-    out = (is_k ? a.kv.k : a.kv.v) + kv_place(a.kv, page, position - entry * a.kv.page_size, head);
+    place = kv_place(a.kv, page, position - entry * a.kv.page_size, head);
+    out = (is_k ? a.kv.k : a.kv.v) + place;
+  }
+  if constexpr (Q4) {
+    if (!is_q) {  // all of a row's lanes, which lie in one wave, come here
+      float* row_values = finished + tid / L * D;
+      *reinterpret_cast<f32x4*>(row_values + first) = x0;
+      *reinterpret_cast<f32x4*>(row_values + second) = x1;
+      __builtin_amdgcn_wave_barrier();
+      const int at = (u >> 2) * kQ4Values + 4 * (u & 3);
+      x0 = *reinterpret_cast<const f32x4*>(row_values + at);
+      x1 = *reinterpret_cast<const f32x4*>(row_values + at + 16);
+      store_q4(reinterpret_cast<uint8_t*>(is_k ? a.kv.k : a.kv.v) + q4_bytes(place), u, x0, x1);
+      return;
+    }
   }
   typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
   u16x4 y0, y1;
@@ -146,13 +206,16 @@ hipError_t launch_kv_append(const AppendArgs& a, int type, int head_dim, int q_t
   const dim3 grid(static_cast<uint32_t>(a.kv.tokens), static_cast<uint32_t>((rows + per - 1) / per));
   const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
   auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a); };
+  const bool q4 = type == QK_TYPE_Q4_1;
   if (head_dim == 128)
-    bf16 ? (q32 ? go(kv_append_kernel<128, true, true>) : go(kv_append_kernel<128, true, false>))
-         : (q32 ? go(kv_append_kernel<128, false, true>) : go(kv_append_kernel<128, false, false>));
+    bf16 ? (q32 ? go(kv_append_kernel<128, true, true, false>) : go(kv_append_kernel<128, true, false, false>))
+    : q4 ? (q32 ? go(kv_append_kernel<128, false, true, true>) : go(kv_append_kernel<128, false, false, true>))
+         : (q32 ? go(kv_append_kernel<128, false, true, false>) : go(kv_append_kernel<128, false, false, false>));
   else
-    bf16 ? (q32 ? go(kv_append_kernel<64, true, true>) : go(kv_append_kernel<64, true, false>))
-         : (q32 ? go(kv_append_kernel<64, false, true>) : go(kv_append_kernel<64, false, false>));
-  note("kv_append_kernel", static_cast<int64_t>(grid.x) * grid.y, head_dim, bf16, q32);
+    bf16 ? (q32 ? go(kv_append_kernel<64, true, true, false>) : go(kv_append_kernel<64, true, false, false>))
+    : q4 ? (q32 ? go(kv_append_kernel<64, false, true, true>) : go(kv_append_kernel<64, false, false, true>))
+         : (q32 ? go(kv_append_kernel<64, false, true, false>) : go(kv_append_kernel<64, false, false, false>));
+  note("kv_append_kernel", static_cast<int64_t>(grid.x) * grid.y, head_dim, bf16, q32, q4);
   return hipGetLastError();
 }
 

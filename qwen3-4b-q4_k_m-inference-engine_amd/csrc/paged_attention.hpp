@@ -25,6 +25,7 @@
 // 2^-100 of the row's sum. bf16 has that range itself.
 #pragma once
 
+#include "q4_1.hpp"
 #include "qk_device.hpp"
 #include "qk_launch.hpp"
 #include "serving.hpp"
@@ -96,6 +97,23 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
     if ((v[i] >> 16 & Num<BF16>::kOne) == Num<BF16>::kOne) v[i] &= 0x0000FFFFu;
   }
   return v;
+}
+
+// A lane's piece of a cached row: 16 bytes of 16-bit values, or half a block's
+// codes. `place`: the row's, in 16-bit values or, of Q4_1 blocks, in bytes.
+__device__ __forceinline__ void load_cached(u32x4& piece, const uint16_t* pool, int64_t place, int unit) {
+  piece = stream_load16(pool + place + 8 * unit);
+}
+__device__ __forceinline__ void load_cached(Q4Piece& piece, const uint16_t* pool, int64_t place, int unit) {
+  piece = q4_load(reinterpret_cast<const uint8_t*>(pool) + place, unit);
+}
+// Value i of that row.
+template <class T, bool Q4>
+__device__ __forceinline__ float cached_value(const uint16_t* pool, int64_t place, int i) {
+  if constexpr (Q4)
+    return static_cast<float>(q4_value(reinterpret_cast<const uint8_t*>(pool) + place, i));
+  else
+    return static_cast<float>(__builtin_bit_cast(T, pool[place + i]));
 }
 
 // Parts of an fp32 value: 16-bit q is its own only part; F32 is two fp16 parts

@@ -13,6 +13,8 @@
 // 8192 keys, 1.06 GB: 175 us (6.1 TB/s), 3 of 131072: 156 (5.6); before the
 // sequences were taken by length 225, and 263 with keys loaded straight into the
 // operand's layout (64 bytes of a row an instruction).
+#include <type_traits>
+
 #include "paged_attention.hpp"
 
 namespace qk {
@@ -81,7 +83,7 @@ __device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile,
   return true;
 }
 
-template <int D, bool BF16, bool Q32>
+template <int D, bool BF16, bool Q32, bool Q4>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionArgs a) {
   typedef Num<BF16> N;
   typedef typename N::T T;
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   // result 2.3e-3 and 1.6e-3, half a step).
   constexpr int NW = NP > 1 ? NP : 2;
   constexpr int KS = D / 32, DT = D / 16;    // k steps of q.k, 16-wide tiles of the output
-  constexpr int LPK = D / 8;                 // lanes that load one key's values
+  constexpr int LPK = Q4 ? D / 16 : D / 8;   // lanes that load one key's values
   constexpr int VL = kBlock * LPK / 64;      // loads of a block's values
   constexpr int KPL = 64 / LPK;              // keys a load
   struct Shared {
@@ -155,23 +157,24 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const auto look_up = [&](int b) {
     page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(b) / a.kv.page_size, listed)];
   };
-  u32x4 kreg[VL], vreg[VL];
+  std::conditional_t<Q4, Q4Piece, u32x4> kreg[VL], vreg[VL];
   const auto settle = [&](int b) {  // page id -> place of block b
     const int key = key_of(b);
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
-    sh.place[wave][b / kWaves & 1][lane & 31] = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
+    const int64_t place = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
+    sh.place[wave][b / kWaves & 1][lane & 31] = Q4 ? q4_bytes(place) : place;
     __builtin_amdgcn_wave_barrier();
   };
   const auto load_k = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      kreg[i] = stream_load16(a.kv.k + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
+      load_cached(kreg[i], a.kv.k, sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK], lane % LPK);
   };
   const auto load_v = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      vreg[i] = stream_load16(a.kv.v + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
+      load_cached(vreg[i], a.kv.v, sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK], lane % LPK);
   };
   if (wave < blocks) {
     look_up(wave);
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const auto correct = [&](int key0) __attribute__((always_inline)) {
     uint32_t sizes = 0;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
+    for (int i = 0; i < kBlock * 2 * D / 1024; ++i) {
       const u32x4 v = load16(vs + i * 1024 + lane * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sizes = larger_sizes(sizes, v[e]);
@@ -339,7 +342,17 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   for (int b = wave; b < blocks; b += kWaves) {
     const int key0 = c.lo + b * kBlock;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4*>(ks + k_chunk<D>(KPL * i + lane / LPK, lane % LPK)) = kreg[i];
+    for (int i = 0; i < VL; ++i) {
+      const int key = KPL * i + lane / LPK;
+      if constexpr (Q4) {
+        u32x4 low, high;
+        q4_values(kreg[i], low, high);
+        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK))) = low;
+        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK) + 2)) = high;
+      } else {
+        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, lane % LPK)) = kreg[i];
+      }
+    }
     // loads past the last block are of its last key: a branch here would make
     // every wait one for all loads in flight
     const int next = b + kWaves;
@@ -352,17 +365,28 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     // values into LDS; those of keys past the end as zeros (their weight is 0), and
     // where a weight may be 0, or its parts of either sign, infinite ones too
     bool odd = false;
+    constexpr int PL = Q4 ? 2 : 1;  // chunks of a load
+    u32x4 values[VL][PL];
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
-      if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
-      odd |= any_infinite<BF16>(vreg[i]);
+      if constexpr (Q4)
+        q4_values(vreg[i], values[i][0], values[i][1]);
+      else
+        values[i][0] = vreg[i];
+#pragma unroll
+      for (int n = 0; n < PL; ++n) {
+        if (key0 + KPL * i + lane / LPK >= c.hi) values[i][n] = u32x4{};
+        odd |= any_infinite<BF16>(values[i][n]);
+      }
     }
     odd = __any(odd);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int key = KPL * i + lane / LPK;
-      *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, lane % LPK)) = odd ? only_finite<BF16>(vreg[i]) : vreg[i];
-    }
+    for (int i = 0; i < VL; ++i)
+#pragma unroll
+      for (int n = 0; n < PL; ++n) {
+        const int key = KPL * i + lane / LPK, chunk = Q4 ? q4_chunk(lane % LPK) + 2 * n : lane % LPK;
+        *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, chunk)) = odd ? only_finite<BF16>(values[i][n]) : values[i][n];
+      }
     load_v(next);
     __builtin_amdgcn_wave_barrier();
     // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
@@ -408,12 +432,12 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       // to the rows that do see them (any weight times them is themselves)
       for (int j = 0; j < kBlock && key0 + j < c.hi; ++j) {
         const bool sees = key0 + j <= last && key0 + j >= from;
-        const uint16_t* v = a.kv.v + sh.place[wave][b / kWaves & 1][j] + 4 * grp;
+        const int64_t place = sh.place[wave][b / kWaves & 1][j];
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = static_cast<float>(__builtin_bit_cast(T, v[16 * d + r]));
+            const float e = cached_value<T, Q4>(a.kv.v, place, 16 * d + 4 * grp + r);
             if (sees && !(fabsf(e) < __builtin_inff())) o[d][r] += e;
           }
       }
@@ -563,15 +587,17 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
 
 hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(a.tiles) * a.splits * a.kv.kv_heads;
-  const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
+  const bool bf16 = type == QK_TYPE_BF16, q4 = type == QK_TYPE_Q4_1, q32 = q_type == QK_TYPE_F32;
   auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, stream>>>(a); };
   if (head_dim == 128)
-    bf16 ? (q32 ? go(attention_few_kernel<128, true, true>) : go(attention_few_kernel<128, true, false>))
-         : (q32 ? go(attention_few_kernel<128, false, true>) : go(attention_few_kernel<128, false, false>));
+    bf16 ? (q32 ? go(attention_few_kernel<128, true, true, false>) : go(attention_few_kernel<128, true, false, false>))
+    : q4 ? (q32 ? go(attention_few_kernel<128, false, true, true>) : go(attention_few_kernel<128, false, false, true>))
+         : (q32 ? go(attention_few_kernel<128, false, true, false>) : go(attention_few_kernel<128, false, false, false>));
   else
-    bf16 ? (q32 ? go(attention_few_kernel<64, true, true>) : go(attention_few_kernel<64, true, false>))
-         : (q32 ? go(attention_few_kernel<64, false, true>) : go(attention_few_kernel<64, false, false>));
-  note("attention_few_kernel", grid, head_dim, bf16, q32, a.splits > 1);
+    bf16 ? (q32 ? go(attention_few_kernel<64, true, true, false>) : go(attention_few_kernel<64, true, false, false>))
+    : q4 ? (q32 ? go(attention_few_kernel<64, false, true, true>) : go(attention_few_kernel<64, false, false, true>))
+         : (q32 ? go(attention_few_kernel<64, false, true, false>) : go(attention_few_kernel<64, false, false, false>));
+  note("attention_few_kernel", grid, head_dim, bf16, q32, a.splits > 1, q4);
   return hipGetLastError();
 }
 

@@ -37,7 +37,7 @@ __device__ __forceinline__ int tile_chunk(int key, int chunk) {
   return key * (2 * D) + ((chunk ^ tile_swizzle<D>(key)) << 4);
 }
 
-template <int D, bool BF16, bool Q32, int KG>
+template <int D, bool BF16, bool Q32, int KG, bool Q4>
 __global__ __launch_bounds__(64 * attention_many_waves(BF16, Q32), attention_many_waves(BF16, Q32) / 4) void
 attention_many_kernel(const AttentionArgs a) {
   typedef Num<BF16> N;
@@ -49,9 +49,10 @@ attention_many_kernel(const AttentionArgs a) {
   constexpr int kKeys = KG == 1 ? 64 : 32 * KG;  // keys of a tile in LDS
   constexpr int kBuffers = KG == 4 ? 2 : 3;
   constexpr int KS = D / 16, DT = D / 32;   // k steps of q.k, 32-wide tiles of the output
-  constexpr int LPK = D / 8;                // lanes that load one key
+  constexpr int LPK = Q4 ? D / 16 : D / 8;  // lanes that load one key
   constexpr int KPL = 64 * kWaves / LPK;    // keys a load of the workgroup
-  constexpr int NL = kKeys / KPL;           // such loads a tile
+  constexpr int NL = KPL < kKeys ? kKeys / KPL : 1;  // such loads a tile
+  constexpr int PL = Q4 ? 2 : 1;            // 16-byte chunks of a lane's load
   constexpr int kTile = kKeys * 2 * D;      // bytes of a tile's keys, or values
   constexpr int kRing = KG == 4 ? 4 : 8;    // tiles whose places are kept
   struct Shared {
@@ -152,46 +153,73 @@ attention_many_kernel(const AttentionArgs a) {
     if (n >= count) return;
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
-    sh.place[n & (kRing - 1)][tid] = kv_place(a.kv, ok ? page : 0, key_of(n) % a.kv.page_size, head);
+    const int64_t place = kv_place(a.kv, ok ? page : 0, key_of(n) % a.kv.page_size, head);
+    sh.place[n & (kRing - 1)][tid] = Q4 ? q4_bytes(place) : place;
   };
-  u32x4 kreg[NL], vreg[NL];
+  std::conditional_t<Q4, Q4Piece, u32x4> kreg[NL], vreg[NL];
+  const bool loads = KPL <= kKeys || tid / LPK < kKeys;
   const auto load = [&](int n) __attribute__((always_inline)) {
-    if (n >= count) return;
+    if (n >= count || !loads) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int64_t at = sh.place[n & (kRing - 1)][KPL * i + tid / LPK] + 8 * (tid % LPK);
-      kreg[i] = load16(a.kv.k + at);
-      vreg[i] = load16(a.kv.v + at);
+      const int64_t at = sh.place[n & (kRing - 1)][KPL * i + tid / LPK];
+      if constexpr (Q4) {
+        kreg[i] = q4_load<false>(reinterpret_cast<const uint8_t*>(a.kv.k) + at, tid % LPK);
+        vreg[i] = q4_load<false>(reinterpret_cast<const uint8_t*>(a.kv.v) + at, tid % LPK);
+      } else {
+        kreg[i] = load16(a.kv.k + at + 8 * (tid % LPK));
+        vreg[i] = load16(a.kv.v + at + 8 * (tid % LPK));
+      }
     }
   };
   // registers -> LDS; values of keys past the end become zeros, and where some
   // row does not see some key, or a weight's parts may be of either sign, or
   // none, so do infinite ones (odd)
   const auto store = [&](int n, int buffer) __attribute__((always_inline)) {
-    if (n >= count) return;
+    if (n >= count || !loads) return;
     const int key0 = c.lo + n * kKeys;
     const bool edge = !(key0 + kKeys - 1 <= tile_last && key0 + kKeys <= c.hi && key0 >= tile_from);
+    u32x4 keys[NL][PL], values[NL][PL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      if constexpr (Q4) {
+        q4_values(kreg[i], keys[i][0], keys[i][1]);
+        q4_values(vreg[i], values[i][0], values[i][1]);
+      } else {
+        keys[i][0] = kreg[i];
+        values[i][0] = vreg[i];
+      }
+    }
     if (edge) {
 #pragma unroll
       for (int i = 0; i < NL; ++i)
-        if (key0 + KPL * i + tid / LPK >= c.hi) vreg[i] = u32x4{};
+        if (key0 + KPL * i + tid / LPK >= c.hi)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) values[i][p] = u32x4{};
     }
     if (edge || NP > 1 || !BF16) {
       bool odd = false;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) odd |= any_infinite<BF16>(vreg[i]);
+      for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int p = 0; p < PL; ++p) odd |= any_infinite<BF16>(values[i][p]);
       if (odd) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) vreg[i] = only_finite<BF16>(vreg[i]);
+        for (int i = 0; i < NL; ++i)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) values[i][p] = only_finite<BF16>(values[i][p]);
         sh.odd[n & 3] = 1;
       }
     }
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int at = buffer * kTile + tile_chunk<D>(KPL * i + tid / LPK, tid % LPK);
-      *reinterpret_cast<u32x4*>(sh.k[0] + at) = kreg[i];
-      *reinterpret_cast<u32x4*>(sh.v[0] + at) = vreg[i];
-    }
+    for (int i = 0; i < NL; ++i)
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+        const int chunk = Q4 ? q4_chunk(tid % LPK) + 2 * p : tid % LPK;
+        const int at = buffer * kTile + tile_chunk<D>(KPL * i + tid / LPK, chunk);
+        *reinterpret_cast<u32x4*>(sh.k[0] + at) = keys[i][p];
+        *reinterpret_cast<u32x4*>(sh.v[0] + at) = values[i][p];
+      }
   };
 
   f32x16 o[DT] = {};
@@ -379,13 +407,13 @@ attention_many_kernel(const AttentionArgs a) {
     for (int m = 0; m < kKeys / KG; ++m) {
       const int key = c.lo + n * kKeys + part * 32 + m;
       if (key >= c.hi) break;
-      const uint16_t* v = a.kv.v + sh.place[n & (kRing - 1)][part * 32 + m] + 4 * half;
+      const int64_t place = sh.place[n & (kRing - 1)][part * 32 + m];
       const bool sees = key <= last && key >= from;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float e = static_cast<float>(__builtin_bit_cast(T, v[32 * d + (r >> 2) * 8 + (r & 3)]));
+          const float e = cached_value<T, Q4>(a.kv.v, place, 32 * d + (r >> 2) * 8 + 4 * half + (r & 3));
           if (sees && !(fabsf(e) < __builtin_inff())) o[d][r] += e;
         }
     }
@@ -594,16 +622,18 @@ hipError_t launch_join(const AttentionArgs& a, int tile_rows, bool bf16, bool q3
 template <int KG>
 hipError_t launch_groups(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(a.tiles) * a.splits * a.kv.kv_heads;
-  const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
+  const bool bf16 = type == QK_TYPE_BF16, q4 = type == QK_TYPE_Q4_1, q32 = q_type == QK_TYPE_F32;
   const int threads = 64 * attention_many_waves(bf16, q32);
   auto go = [&](auto kernel) { kernel<<<grid, threads, 0, stream>>>(a); };
   if (head_dim == 128)
-    bf16 ? (q32 ? go(attention_many_kernel<128, true, true, KG>) : go(attention_many_kernel<128, true, false, KG>))
-         : (q32 ? go(attention_many_kernel<128, false, true, KG>) : go(attention_many_kernel<128, false, false, KG>));
+    bf16 ? (q32 ? go(attention_many_kernel<128, true, true, KG, false>) : go(attention_many_kernel<128, true, false, KG, false>))
+    : q4 ? (q32 ? go(attention_many_kernel<128, false, true, KG, true>) : go(attention_many_kernel<128, false, false, KG, true>))
+         : (q32 ? go(attention_many_kernel<128, false, true, KG, false>) : go(attention_many_kernel<128, false, false, KG, false>));
   else
-    bf16 ? (q32 ? go(attention_many_kernel<64, true, true, KG>) : go(attention_many_kernel<64, true, false, KG>))
-         : (q32 ? go(attention_many_kernel<64, false, true, KG>) : go(attention_many_kernel<64, false, false, KG>));
-  note("attention_many_kernel", grid, head_dim, bf16, q32, KG, a.splits > 1);
+    bf16 ? (q32 ? go(attention_many_kernel<64, true, true, KG, false>) : go(attention_many_kernel<64, true, false, KG, false>))
+    : q4 ? (q32 ? go(attention_many_kernel<64, false, true, KG, true>) : go(attention_many_kernel<64, false, false, KG, true>))
+         : (q32 ? go(attention_many_kernel<64, false, true, KG, false>) : go(attention_many_kernel<64, false, false, KG, false>));
+  note("attention_many_kernel", grid, head_dim, bf16, q32, KG, a.splits > 1, q4);
   const hipError_t error = hipGetLastError();
   if (error != hipSuccess || a.splits == 1) return error;
   return head_dim == 128 ? launch_join<128>(a, threads / 2 / KG, bf16, q32, stream)

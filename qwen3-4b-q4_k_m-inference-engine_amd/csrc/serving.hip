@@ -5,6 +5,7 @@
 
 #include <cmath>
 
+#include "q4_1.hpp"
 #include "qk_launch.hpp"
 
 namespace {
@@ -23,15 +24,16 @@ hipStream_t as_stream(qk_stream_t s) { return static_cast<hipStream_t>(s); }
 // Lengths and strides of a cache and a batch (pointers: check_pointers).
 int check_shapes(const qk_kv_cache* c, const qk_kv_batch* b) {
   if (!c || !b) return refuse("cache and batch must be non-null");
-  if (c->type != QK_TYPE_F16 && c->type != QK_TYPE_BF16)
-    return refuse("caches are F16 or BF16", QK_ERR_UNSUPPORTED_TYPE);
+  if (c->type != QK_TYPE_F16 && c->type != QK_TYPE_BF16 && c->type != QK_TYPE_Q4_1)
+    return refuse("caches are F16, BF16 or Q4_1", QK_ERR_UNSUPPORTED_TYPE);
   if (c->head_dim != 64 && c->head_dim != 128) return refuse("cache head_dim must be 64 or 128");
   if (c->pages < 1 || c->pages > INT32_MAX || c->page_size < 1 || c->page_size > 65536)
     return refuse("cache needs 1 .. 2^31-1 pages of 1 .. 65536 tokens");
   if (c->kv_heads < 1 || c->kv_heads > 4096) return refuse("cache needs 1 .. 4096 heads");
   const int64_t most = int64_t{1} << 30;
-  if (c->token_stride % 8 != 0 || c->head_stride % 8 != 0 || c->page_stride % 8 != 0)
-    return refuse("cache strides must be multiples of 8 elements");
+  const int64_t unit = c->type == QK_TYPE_Q4_1 ? qk::kQ4Values : 8;
+  if (c->token_stride % unit != 0 || c->head_stride % unit != 0 || c->page_stride % unit != 0)
+    return refuse("cache strides must be multiples of 8 elements, of a Q4_1 cache of 32");
   if (c->token_stride < c->head_dim || c->head_stride < c->head_dim || c->token_stride > most || c->head_stride > most ||
       c->page_stride < 0 || c->page_stride > (int64_t{1} << 40))
     return refuse("cache strides must hold a head's values and stay below 2^30 elements (pages: 2^40)");
@@ -50,10 +52,13 @@ int check_pointers(const qk_kv_cache* c, const qk_kv_batch* b) {
   return QK_OK;
 }
 
+// The 16-bit type that a cache's rows are read as.
+int value_type(const qk_kv_cache* c) { return c->type == QK_TYPE_Q4_1 ? QK_TYPE_F16 : c->type; }
+
 // q heads against the cache's, and q's type.
 int check_heads(const qk_kv_cache* c, const qk_kv_batch* b, int64_t q_heads, int q_type) {
-  if (q_type != QK_TYPE_F32 && q_type != c->type)
-    return refuse("q must be F32 or of the cache's type", QK_ERR_UNSUPPORTED_TYPE);
+  if (q_type != QK_TYPE_F32 && q_type != value_type(c))
+    return refuse("q must be F32 or of the cache's type (F16 for Q4_1)", QK_ERR_UNSUPPORTED_TYPE);
   if (q_heads < 1 || q_heads > 4096 || q_heads % c->kv_heads != 0)
     return refuse("q_heads must be a multiple of the cache's heads, at most 4096");
   if (b->tokens * q_heads > (int64_t{1} << 28)) return refuse("tokens x q_heads must stay within 2^28");
@@ -88,6 +93,12 @@ extern "C" {
 int qk_kv_append(const qk_kv_cache* cache, const qk_kv_batch* batch, const float* q, int64_t q_stride, const float* k,
                  int64_t k_stride, const float* v, int64_t v_stride, int64_t q_heads, const qk_rope* rope, void* q_out,
                  int q_type, qk_stream_t stream) {
+  return qk_kv_append_at(cache, batch, nullptr, q, q_stride, k, k_stride, v, v_stride, q_heads, rope, q_out, q_type, stream);
+}
+
+int qk_kv_append_at(const qk_kv_cache* cache, const qk_kv_batch* batch, const int32_t* seen, const float* q,
+                    int64_t q_stride, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                    int64_t q_heads, const qk_rope* rope, void* q_out, int q_type, qk_stream_t stream) {
   int status = check_shapes(cache, batch);
   if (status != QK_OK) return status;
   if (q_heads != 0) status = check_heads(cache, batch, q_heads, q_type);
@@ -106,6 +117,7 @@ int qk_kv_append(const qk_kv_cache* cache, const qk_kv_batch* batch, const float
     return refuse("q, k and v strides must hold a token's heads");
   status = check_pointers(cache, batch);
   if (status != QK_OK) return status;
+  if (misaligned(seen, 4)) return refuse("batch arrays must be 4-byte aligned");
   if (!k || !v || (q_heads != 0 && (!q || !q_out))) return refuse("append pointers must be non-null");
   if (misaligned(q, 4) || misaligned(k, 4) || misaligned(v, 4) || (q_heads != 0 && misaligned(q_out, 16)))
     return refuse("append inputs must be 4-byte, q_out 16-byte aligned");
@@ -116,6 +128,7 @@ int qk_kv_append(const qk_kv_cache* cache, const qk_kv_batch* batch, const float
     return refuse("q_out may be q only for F32 rows without gaps");
   qk::AppendArgs a{};
   a.kv = kv_args(cache, batch);
+  a.seen = seen;
   a.q = q;
   a.k = k;
   a.v = v;
@@ -186,6 +199,22 @@ int qk_paged_attention(const qk_kv_cache* cache, const qk_kv_batch* batch, const
   return finish(qk::launch_paged_attention(a, plan, cache->type, static_cast<int>(cache->head_dim), q_type, workspace,
                                            as_stream(stream)),
                 "paged attention launch failed");
+}
+
+int qk_kv_rows(const qk_kv_cache* cache, const qk_kv_batch* batch, void* k_out, void* v_out, int out_type,
+               qk_stream_t stream) {
+  int status = check_shapes(cache, batch);
+  if (status != QK_OK) return status;
+  if (out_type != QK_TYPE_F32 && out_type != value_type(cache))
+    return refuse("rows are F32 or of the cache's type (F16 for Q4_1)", QK_ERR_UNSUPPORTED_TYPE);
+  if (batch->tokens == 0 || batch->sequences == 0) return QK_OK;
+  status = check_pointers(cache, batch);
+  if (status != QK_OK) return status;
+  if (!k_out && !v_out) return refuse("rows need somewhere to go");
+  if (misaligned(k_out, 16) || misaligned(v_out, 16)) return refuse("row outputs must be 16-byte aligned");
+  qk::RowsArgs a{kv_args(cache, batch), k_out, v_out};
+  return finish(qk::launch_kv_rows(a, cache->type, static_cast<int>(cache->head_dim), out_type, as_stream(stream)),
+                "cache rows launch failed");
 }
 
 int qk_kv_check(const qk_kv_cache* cache, qk_stream_t stream) {

@@ -21,6 +21,7 @@ __device__ __forceinline__ void kv_fault(const KvArgs& a, uint32_t bit) {
 
 struct AppendArgs {
   KvArgs kv;
+  const int32_t* seen;  // tokens of each sequence for the angles' positions; nullptr: the contexts
   const float* q;
   const float* k;
   const float* v;
@@ -34,6 +35,13 @@ struct AppendArgs {
   int32_t dims, interleaved;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
+
+struct RowsArgs {
+  KvArgs kv;
+  void* k_out;  // either may be nullptr
+  void* v_out;
+};
+hipError_t launch_kv_rows(const RowsArgs& a, int type, int head_dim, int out_type, hipStream_t stream);
 
 hipError_t launch_kv_fault_clear(uint32_t* word, uint32_t bits, hipStream_t stream);
 
