@@ -16,7 +16,7 @@ constexpr int kOrdered = 128;        // most sequences that are taken by length
 
 // How a call is laid out, from host values alone.
 struct AttentionPlan {
-  bool few;              // 16-row tiles (paged_attention_few.hip), else 256 to 32 (paged_attention_many.hip)
+  bool few;              // 16-row tiles (paged_attention_few*.hip; of Q4_1 also 8), else 256 to 32 (paged_attention_many.hip)
   int key_groups;        // of the latter: 1, or 2 or 4 waves that share 32 rows, each with a part of the keys
   int rows;              // rows of a tile: (new token, query head of the key/value head)
   int32_t tiles;         // at most so many tiles
@@ -66,6 +66,8 @@ constexpr int64_t kOrderedKeys = 1024;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
+// Over Q4_1 blocks.
+constexpr int kLeastPartQ4 = 256, kSlotsQ4 = 1024;
 constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
 inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -150,18 +152,25 @@ inline AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q
     ManyRows{rows, tokens, sequences, kv_heads, group, window, max_context, waves_rows, head_dim,
              q_type == QK_TYPE_F32 ? (type == QK_TYPE_BF16 ? 3 : 2) : 1}
         .choose(p.key_groups, splits);
-  const int tile_rows = p.few ? 16 : waves_rows / p.key_groups;
+  // over Q4_1 blocks a tile of few rows leaves the matrix core's other columns to other keys
+  const int few_rows = type != QK_TYPE_Q4_1 || rows > 8 * sequences ? 16 : 8;
+  const int tile_rows = p.few ? few_rows : waves_rows / p.key_groups;
   p.rows = tile_rows;
   const int64_t tiles = tiles_of(tile_rows);
   p.tiles = static_cast<int32_t>(tiles);
   const int64_t units = tiles * kv_heads;
   const bool whole = p.few && keys >= kOrderedKeys && units > kUnits;
-  const bool ordered = whole && rows <= 16 * sequences && sequences <= kOrdered;  // else some sequence has two tiles
+  const bool ordered = whole && rows <= tile_rows * sequences && sequences <= kOrdered;  // else some sequence has two tiles
   if (p.few) splits = whole ? 1 : up(kMostUnits, units);
   p.fill = static_cast<int32_t>(splits);
   if (p.few && !ordered && units <= kMostUnits && splits < up(keys, kGoodPart)) {
     const int64_t most = up(4 * kMostUnits, units);
     splits = up(keys, kGoodPart) < most ? up(keys, kGoodPart) : most;
+  }
+  if (p.few && type == QK_TYPE_Q4_1) {
+    // the kernel cuts contexts into even shares of all keys
+    splits = whole || units > kMostUnits ? 1 : up(kSlotsQ4, units);
+    if (splits > up(keys, kLeastPartQ4)) splits = up(keys, kLeastPartQ4);
   }
   const int64_t least = p.few ? 128 : 256;
   if (splits > up(keys, least)) splits = up(keys, least);

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const RowsArgs a) {
     if constexpr (Q4) {
       // values 8 u .. of the row: the low or the high halves of a piece's codes
       u32x4 low, high;
-      q4_values(q4_load<false>(reinterpret_cast<const uint8_t*>(pool) + q4_bytes(place), (u >> 2) * 2 + (u & 1)), low, high);
+      q4_values(q4_load(reinterpret_cast<const uint8_t*>(pool) + q4_bytes(place), (u >> 2) * 2 + (u & 1)), low, high);
       x = u & 2 ? high : low;
     } else {
       x = load16(pool + place + 8 * u);

@@ -99,15 +99,7 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
   return v;
 }
 
-// A lane's piece of a cached row: 16 bytes of 16-bit values, or half a block's
-// codes. `place`: the row's, in 16-bit values or, of Q4_1 blocks, in bytes.
-__device__ __forceinline__ void load_cached(u32x4& piece, const uint16_t* pool, int64_t place, int unit) {
-  piece = stream_load16(pool + place + 8 * unit);
-}
-__device__ __forceinline__ void load_cached(Q4Piece& piece, const uint16_t* pool, int64_t place, int unit) {
-  piece = q4_load(reinterpret_cast<const uint8_t*>(pool) + place, unit);
-}
-// Value i of that row.
+// Value i of a cached row. `place`: the row's, in 16-bit values or, of Q4_1 blocks, in bytes.
 template <class T, bool Q4>
 __device__ __forceinline__ float cached_value(const uint16_t* pool, int64_t place, int i) {
   if constexpr (Q4)
@@ -148,6 +140,13 @@ __device__ __forceinline__ float swap32_max(float v) {
                                                   false);
   const unsigned a = t[0], b = t[1];
   return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// Which entry of its page table a key lies in, key / page_size, for keys below 2^30:
+// the high half of a product with page_factor (launch_paged_attention).
+__device__ __forceinline__ int page_entry(const AttentionArgs& a, int key) {
+  const uint32_t high = __umulhi(static_cast<uint32_t>(key), a.page_factor);
+  return a.kv.page_size == 1 ? key : static_cast<int>(high >> a.page_shift);
 }
 
 // Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
@@ -243,6 +242,33 @@ __device__ __forceinline__ int longest_context(const AttentionArgs& a) {
     most = other > most ? other : most;
   }
   return __builtin_amdgcn_readfirstlane(a.window > 0 && most > a.window ? a.window : most);
+}
+
+// The tiles of `tile_rows` rows, the keys of all of them, and of the longest one.
+struct KeyCounts {
+  int64_t all;
+  int tiles, longest;
+};
+__device__ __forceinline__ KeyCounts count_keys(const AttentionArgs& a, int tile_rows) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  KeyCounts c = {};
+  for (int s = lane; s < a.kv.sequences; s += 64) {
+    const KvSequence q = kv_sequence(a.kv, s);
+    int keys = kv_keys(q);
+    keys = a.window > 0 && keys > a.window ? a.window : keys;
+    const int tiles = (q.count * a.group + tile_rows - 1) / tile_rows;
+    c.tiles += tiles;
+    c.all += static_cast<int64_t>(tiles) * keys;
+    c.longest = keys > c.longest ? keys : c.longest;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    c.all += __shfl_xor(c.all, off);
+    c.tiles += __shfl_xor(c.tiles, off);
+    const int other = __shfl_xor(c.longest, off);
+    c.longest = other > c.longest ? other : c.longest;
+  }
+  return c;
 }
 
 // Values that another workgroup of the launch reads: coherent at agent scope,

@@ -13,14 +13,12 @@
 // 8192 keys, 1.06 GB: 175 us (6.1 TB/s), 3 of 131072: 156 (5.6); before the
 // sequences were taken by length 225, and 263 with keys loaded straight into the
 // operand's layout (64 bytes of a row an instruction).
-#include <type_traits>
-
-#include "paged_attention.hpp"
+#include "paged_attention_few.hpp"
 
 namespace qk {
 namespace {
 
-constexpr int kRows = 16, kBlock = 32, kWaves = 4, kStep = kBlock * kWaves;
+constexpr int kRows = 16, kWaves = 4, kStep = kBlock * kWaves;
 
 // 16-byte chunks of V rows in LDS are permuted so that the eight keys which one
 // pass of a transposing read touches lie in different banks.
@@ -36,54 +34,7 @@ __device__ __forceinline__ int k_chunk(int key, int chunk) {
   return key * (2 * D) + ((chunk ^ (D == 128 ? key & 15 : key >> 1 & 7)) << 4);
 }
 
-// Tiles by the length of their sequences' contexts, where no sequence has more
-// than one (false otherwise): the `pairs` longest in the first round of
-// workgroups, one a compute unit, the next ones in the second, which the card
-// places on the same units in the same order, from the shortest up; then the
-// rest. Each unit's two contexts so have about the same length together: 64
-// sequences of up to 8192 keys, uneven, 225 us as they come, 175 paired. Every
-// workgroup ranks the lengths itself, a thread a sequence.
-__device__ __forceinline__ bool find_by_length(const AttentionArgs& a, int tile, bool report, int32_t (&keys)[kOrdered],
-                                               int32_t& chosen, AttentionTile& t) {
-  const int s = static_cast<int>(threadIdx.x);
-  int mine = -1;
-  bool single = true;
-  if (s < a.kv.sequences) {
-    const KvSequence q = kv_sequence(a.kv, s);
-    if (report && q.fault) kv_fault(a.kv, QK_KV_FAULT_LENGTH);
-    single = q.count * a.group <= kRows;
-    if (q.count > 0) {
-      mine = kv_keys(q);
-      mine = a.window > 0 && mine > a.window ? a.window : mine;
-    }
-  }
-  if (s < kOrdered) keys[s] = mine;
-  if (s == 0) chosen = -1;
-  const int tiles = __syncthreads_count(mine >= 0);
-  if (!__syncthreads_and(single)) return false;
-  int rank = 0;
-  for (int i = 0; i < a.kv.sequences; i += 4) {
-    const i32x4 other = *reinterpret_cast<const i32x4*>(&keys[i]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) rank += other[e] > mine || (other[e] == mine && i + e < s);
-  }
-  const int second = 2 * a.pairs < tiles ? 2 * a.pairs : tiles;
-  const int wanted = tile < a.pairs || tile >= second ? tile : second - 1 - (tile - a.pairs);
-  if (mine >= 0 && rank == wanted) chosen = s;
-  __syncthreads();
-  t.s = __builtin_amdgcn_readfirstlane(chosen);
-  if (t.s < 0) return true;
-  const KvSequence q = kv_sequence(a.kv, t.s);
-  t.row = q.row;
-  t.count = q.count;
-  t.first = q.first;
-  t.beyond = q.beyond;
-  t.begin = 0;
-  tile_keys(a.group, a.window, kRows, t);
-  return true;
-}
-
-template <int D, bool BF16, bool Q32, bool Q4>
+template <int D, bool BF16, bool Q32>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionArgs a) {
   typedef Num<BF16> N;
   typedef typename N::T T;
@@ -94,10 +45,10 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   // result 2.3e-3 and 1.6e-3, half a step).
   constexpr int NW = NP > 1 ? NP : 2;
   constexpr int KS = D / 32, DT = D / 16;    // k steps of q.k, 16-wide tiles of the output
-  constexpr int LPK = Q4 ? D / 16 : D / 8;   // lanes that load one key's values
+  constexpr int LPK = D / 8;                 // lanes that load one key's values
   constexpr int VL = kBlock * LPK / 64;      // loads of a block's values
   constexpr int KPL = 64 / LPK;              // keys a load
-  struct Shared {
+  struct Shared : FewShared {
     union {
       struct {
         uint8_t k[kWaves][kBlock * 2 * D];
@@ -107,18 +58,13 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     };
     int64_t place[kWaves][2][kBlock];
     float top[kWaves][kRows], sum[kWaves][kRows];
-    __attribute__((aligned(16))) int32_t keys[kOrdered];
-    int32_t chosen;
-    uint32_t bad, arrived;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
   const int tile = unit / a.splits, split = unit % a.splits;
-  AttentionTile t;
-  const bool report = blockIdx.x == 0;
-  if (a.pairs == 0 || !find_by_length(a, tile, report, sh.keys, sh.chosen, t)) t = find_tile(a, tile, kRows, report);
+  const AttentionTile t = few_tile<kRows>(a, tile, sh);
   if (t.s < 0) return;
   // chunks of one length for all sequences, so that a batch's longest does not outlast the rest
   int chunk = kStep;
@@ -157,24 +103,23 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const auto look_up = [&](int b) {
     page = a.kv.page_table[kv_table_at(a.kv, t.s, key_of(b) / a.kv.page_size, listed)];
   };
-  std::conditional_t<Q4, Q4Piece, u32x4> kreg[VL], vreg[VL];
+  u32x4 kreg[VL], vreg[VL];
   const auto settle = [&](int b) {  // page id -> place of block b
     const int key = key_of(b);
     const bool ok = listed && page >= 0 && page < a.kv.pages;
     bad |= !ok;
-    const int64_t place = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
-    sh.place[wave][b / kWaves & 1][lane & 31] = Q4 ? q4_bytes(place) : place;
+    sh.place[wave][b / kWaves & 1][lane & 31] = kv_place(a.kv, ok ? page : 0, key % a.kv.page_size, head);
     __builtin_amdgcn_wave_barrier();
   };
   const auto load_k = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      load_cached(kreg[i], a.kv.k, sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK], lane % LPK);
+      kreg[i] = stream_load16(a.kv.k + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
   };
   const auto load_v = [&](int b) {
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      load_cached(vreg[i], a.kv.v, sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK], lane % LPK);
+      vreg[i] = stream_load16(a.kv.v + sh.place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
   };
   if (wave < blocks) {
     look_up(wave);
@@ -283,7 +228,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   const auto correct = [&](int key0) __attribute__((always_inline)) {
     uint32_t sizes = 0;
 #pragma unroll
-    for (int i = 0; i < kBlock * 2 * D / 1024; ++i) {
+    for (int i = 0; i < VL; ++i) {
       const u32x4 v = load16(vs + i * 1024 + lane * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sizes = larger_sizes(sizes, v[e]);
@@ -342,17 +287,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
   for (int b = wave; b < blocks; b += kWaves) {
     const int key0 = c.lo + b * kBlock;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int key = KPL * i + lane / LPK;
-      if constexpr (Q4) {
-        u32x4 low, high;
-        q4_values(kreg[i], low, high);
-        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK))) = low;
-        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK) + 2)) = high;
-      } else {
-        *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, lane % LPK)) = kreg[i];
-      }
-    }
+    for (int i = 0; i < VL; ++i) *reinterpret_cast<u32x4*>(ks + k_chunk<D>(KPL * i + lane / LPK, lane % LPK)) = kreg[i];
     // loads past the last block are of its last key: a branch here would make
     // every wait one for all loads in flight
     const int next = b + kWaves;
@@ -365,28 +300,17 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
     // values into LDS; those of keys past the end as zeros (their weight is 0), and
     // where a weight may be 0, or its parts of either sign, infinite ones too
     bool odd = false;
-    constexpr int PL = Q4 ? 2 : 1;  // chunks of a load
-    u32x4 values[VL][PL];
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
-      if constexpr (Q4)
-        q4_values(vreg[i], values[i][0], values[i][1]);
-      else
-        values[i][0] = vreg[i];
-#pragma unroll
-      for (int n = 0; n < PL; ++n) {
-        if (key0 + KPL * i + lane / LPK >= c.hi) values[i][n] = u32x4{};
-        odd |= any_infinite<BF16>(values[i][n]);
-      }
+      if (key0 + KPL * i + lane / LPK >= c.hi) vreg[i] = u32x4{};
+      odd |= any_infinite<BF16>(vreg[i]);
     }
     odd = __any(odd);
 #pragma unroll
-    for (int i = 0; i < VL; ++i)
-#pragma unroll
-      for (int n = 0; n < PL; ++n) {
-        const int key = KPL * i + lane / LPK, chunk = Q4 ? q4_chunk(lane % LPK) + 2 * n : lane % LPK;
-        *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, chunk)) = odd ? only_finite<BF16>(values[i][n]) : values[i][n];
-      }
+    for (int i = 0; i < VL; ++i) {
+      const int key = KPL * i + lane / LPK;
+      *reinterpret_cast<u32x4*>(vs + v_chunk<D>(key, lane % LPK)) = odd ? only_finite<BF16>(vreg[i]) : vreg[i];
+    }
     load_v(next);
     __builtin_amdgcn_wave_barrier();
     // softmax of 32 keys: registers r of tile i hold key 16 i + 4 grp + r
@@ -432,12 +356,12 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
       // to the rows that do see them (any weight times them is themselves)
       for (int j = 0; j < kBlock && key0 + j < c.hi; ++j) {
         const bool sees = key0 + j <= last && key0 + j >= from;
-        const int64_t place = sh.place[wave][b / kWaves & 1][j];
+        const uint16_t* v = a.kv.v + sh.place[wave][b / kWaves & 1][j] + 4 * grp;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = cached_value<T, Q4>(a.kv.v, place, 16 * d + 4 * grp + r);
+            const float e = static_cast<float>(__builtin_bit_cast(T, v[16 * d + r]));
             if (sees && !(fabsf(e) < __builtin_inff())) o[d][r] += e;
           }
       }
@@ -587,17 +511,15 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttentionAr
 
 hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(a.tiles) * a.splits * a.kv.kv_heads;
-  const bool bf16 = type == QK_TYPE_BF16, q4 = type == QK_TYPE_Q4_1, q32 = q_type == QK_TYPE_F32;
+  const bool bf16 = type == QK_TYPE_BF16, q32 = q_type == QK_TYPE_F32;
   auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, stream>>>(a); };
   if (head_dim == 128)
-    bf16 ? (q32 ? go(attention_few_kernel<128, true, true, false>) : go(attention_few_kernel<128, true, false, false>))
-    : q4 ? (q32 ? go(attention_few_kernel<128, false, true, true>) : go(attention_few_kernel<128, false, false, true>))
-         : (q32 ? go(attention_few_kernel<128, false, true, false>) : go(attention_few_kernel<128, false, false, false>));
+    bf16 ? (q32 ? go(attention_few_kernel<128, true, true>) : go(attention_few_kernel<128, true, false>))
+         : (q32 ? go(attention_few_kernel<128, false, true>) : go(attention_few_kernel<128, false, false>));
   else
-    bf16 ? (q32 ? go(attention_few_kernel<64, true, true, false>) : go(attention_few_kernel<64, true, false, false>))
-    : q4 ? (q32 ? go(attention_few_kernel<64, false, true, true>) : go(attention_few_kernel<64, false, false, true>))
-         : (q32 ? go(attention_few_kernel<64, false, true, false>) : go(attention_few_kernel<64, false, false, false>));
-  note("attention_few_kernel", grid, head_dim, bf16, q32, a.splits > 1, q4);
+    bf16 ? (q32 ? go(attention_few_kernel<64, true, true>) : go(attention_few_kernel<64, true, false>))
+         : (q32 ? go(attention_few_kernel<64, false, true>) : go(attention_few_kernel<64, false, false>));
+  note("attention_few_kernel", grid, head_dim, bf16, q32, a.splits > 1);
   return hipGetLastError();
 }
 

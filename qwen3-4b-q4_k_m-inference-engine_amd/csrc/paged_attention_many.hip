@@ -164,8 +164,8 @@ attention_many_kernel(const AttentionArgs a) {
     for (int i = 0; i < NL; ++i) {
       const int64_t at = sh.place[n & (kRing - 1)][KPL * i + tid / LPK];
       if constexpr (Q4) {
-        kreg[i] = q4_load<false>(reinterpret_cast<const uint8_t*>(a.kv.k) + at, tid % LPK);
-        vreg[i] = q4_load<false>(reinterpret_cast<const uint8_t*>(a.kv.v) + at, tid % LPK);
+        kreg[i] = q4_load(reinterpret_cast<const uint8_t*>(a.kv.k) + at, tid % LPK);
+        vreg[i] = q4_load(reinterpret_cast<const uint8_t*>(a.kv.v) + at, tid % LPK);
       } else {
         kreg[i] = load16(a.kv.k + at + 8 * (tid % LPK));
         vreg[i] = load16(a.kv.v + at + 8 * (tid % LPK));

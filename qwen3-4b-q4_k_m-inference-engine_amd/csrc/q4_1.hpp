@@ -6,7 +6,8 @@
 //
 // The codes become F16 without a conversion: a nibble under the exponent of 1024
 // (bits 0 .. 3) or of 64 (bits 4 .. 7) is 1024 + c or 64 + c, less that is c,
-// exactly, and one packed fma gives the value. 14 instructions for eight values.
+// exactly, and one packed fma gives the value: 14 instructions for eight values in
+// their order, 13 in any.
 #pragma once
 
 #include "qk_device.hpp"
@@ -27,41 +28,51 @@ struct Q4Piece {
   u32x2_q4 codes;
   uint32_t dm;
 };
-// Piece `unit` of a row: block unit / 2, half unit % 2. STREAM: it is not read again.
-template <bool STREAM = true>
+// Piece `unit` of a row: block unit / 2, half unit % 2.
 __device__ __forceinline__ Q4Piece q4_load(const uint8_t* row, int unit) {
   const uint8_t* block = row + (unit >> 1) * kQ4Bytes;
-  const uint32_t* dm = reinterpret_cast<const uint32_t*>(block);
-  const u32x2_a4* codes = reinterpret_cast<const u32x2_a4*>(block + 4 + 8 * (unit & 1));
-  if constexpr (STREAM) return {__builtin_nontemporal_load(codes), __builtin_nontemporal_load(dm)};
-  return {*codes, *dm};
+  return {*reinterpret_cast<const u32x2_a4*>(block + 4 + 8 * (unit & 1)), *reinterpret_cast<const uint32_t*>(block)};
 }
 // Where its values lie in a row, in chunks of eight: this one, and two on.
 __device__ __forceinline__ int q4_chunk(int unit) { return 4 * (unit >> 1) + (unit & 1); }
 
 typedef _Float16 half2_q4 __attribute__((ext_vector_type(2)));
 
+// Codes as F16: `two` holds one in bits 0 .. 3 of each half, or in bits 4 .. 7. The
+// exponents come from a register that the compiler does not see through: with two
+// constants an and and an or would be two instructions.
+struct Q4Exponents {
+  uint32_t low = 0x64006400u, high = 0x54005400u;  // of 1024 and of 64
+  __device__ __forceinline__ Q4Exponents() { asm("" : "+v"(low), "+v"(high)); }
+};
+__device__ __forceinline__ half2_q4 q4_low(uint32_t two, const Q4Exponents& e) {
+  return __builtin_bit_cast(half2_q4, (two & 0x000F000Fu) | e.low) +
+         half2_q4{static_cast<_Float16>(-1024.0f), static_cast<_Float16>(-1024.0f)};
+}
+__device__ __forceinline__ half2_q4 q4_high(uint32_t two, const Q4Exponents& e) {
+  return __builtin_bit_cast(half2_q4, (two & 0x00F000F0u) | e.high) +
+         half2_q4{static_cast<_Float16>(-64.0f), static_cast<_Float16>(-64.0f)};
+}
+
 // Eight values of four bytes of codes: their low halves' to `low`, their high halves' to `high`.
-__device__ __forceinline__ void q4_values4(uint32_t codes, half2_q4 d, half2_q4 m, uint32_t (&low)[2], uint32_t (&high)[2]) {
-  const half2_q4 off_low = {static_cast<_Float16>(-1024.0f), static_cast<_Float16>(-1024.0f)};
-  const half2_q4 off_high = {static_cast<_Float16>(-64.0f), static_cast<_Float16>(-64.0f)};
+__device__ __forceinline__ void q4_values4(uint32_t codes, half2_q4 d, half2_q4 m, const Q4Exponents& e, uint32_t (&low)[2],
+                                           uint32_t (&high)[2]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t two = __builtin_amdgcn_perm(0u, codes, i == 0 ? 0x0C010C00u : 0x0C030C02u);  // bytes 2 i and 2 i + 1
-    const half2_q4 lo = __builtin_bit_cast(half2_q4, (two & 0x000F000Fu) | 0x64006400u) + off_low;
-    const half2_q4 hi = __builtin_bit_cast(half2_q4, (two & 0x00F000F0u) | 0x54005400u) + off_high;
-    low[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(lo, d, m));
-    high[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(hi, d, m));
+    low[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q4_low(two, e), d, m));
+    high[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q4_high(two, e), d, m));
   }
 }
 // The sixteen values of a piece: chunks q4_chunk(unit) and q4_chunk(unit) + 2.
 __device__ __forceinline__ void q4_values(const Q4Piece& p, u32x4& low, u32x4& high) {
   const half2_q4 dm = __builtin_bit_cast(half2_q4, p.dm);
   const half2_q4 d = {dm.x, dm.x}, m = {dm.y, dm.y};
+  const Q4Exponents e;
   uint32_t l[2], h[2];
-  q4_values4(p.codes.x, d, m, l, h);
+  q4_values4(p.codes.x, d, m, e, l, h);
   low.x = l[0], low.y = l[1], high.x = h[0], high.y = h[1];
-  q4_values4(p.codes.y, d, m, l, h);
+  q4_values4(p.codes.y, d, m, e, l, h);
   low.z = l[0], low.w = l[1], high.z = h[0], high.w = h[1];
 }
 // Value i of a row.

@@ -56,6 +56,8 @@ struct AttentionArgs {
   float* lse;
   // the plan's part (launch_paged_attention)
   int32_t tiles, splits, fill;
+  uint32_t page_factor;  // for page_entry
+  int32_t page_shift;
   int32_t pairs;      // tiles of a round of workgroups, one a compute unit, if sequences are taken by length; else 0
   uint32_t* arrived;  // [tiles x kv_heads], zero between calls
   float* sums;        // [tiles x kv_heads x splits x rows] (maximum, sum) pairs
@@ -65,6 +67,7 @@ struct AttentionArgs {
 hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, int type, int head_dim, int q_type,
                                   void* workspace, hipStream_t stream);
 hipError_t launch_attention_few(const AttentionArgs& a, int type, int head_dim, int q_type, hipStream_t stream);
+hipError_t launch_attention_few_q4(const AttentionArgs& a, int tile_rows, int head_dim, int q_type, hipStream_t stream);
 hipError_t launch_attention_many(const AttentionArgs& a, int key_groups, int type, int head_dim, int q_type, hipStream_t stream);
 
 struct SampleArgs {
