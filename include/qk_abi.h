@@ -419,6 +419,67 @@ size_t qk_paged_attention_workspace_size(const qk_kv_cache *cache, const qk_kv_b
                                          int q_type, int64_t q_heads, int64_t window,
                                          int64_t max_context);
 
+/* What an eviction goes by, of every slot of a cache and key/value head: weight is
+ * the attention weight that its token has gathered, position the token's own (both
+ * device, [pages x kv_heads x page_size], a page's and head's slots side by side). No
+ * value in them needs to be set before qk_kv_weigh has met the token. */
+typedef struct qk_kv_weights {
+    float *weight;
+    int32_t *position;
+} qk_kv_weights;
+
+/* Adds to every cached token of the batch's sequences the softmax weight that the
+ * new tokens' queries give it, for each key/value head the sum over them and its
+ * query heads: weight[j] += sum of exp(scale * q_i . k_j - lse_i) over the tokens i
+ * that see j (j <= i). The new tokens' own slots begin anew with this call: their
+ * weight is the sum alone, their position is set (seen[sequences], device: see
+ * qk_kv_append_at; NULL: the contexts). q, its type and strides as
+ * qk_paged_attention's, without a window; lse [tokens x q_heads] as that call wrote
+ * it. Rows whose lse is -inf or NaN give nothing, nor does a weight that is NaN. fp32
+ * sums in an order that the arguments alone decide. A page may belong to one sequence
+ * of the call only. Keys on a page that is none get nothing; a sequence longer than
+ * max_context by as much as does not fit, or than its page table, is left alone (both
+ * reported, see qk_kv_cache::fault).
+ * workspace: qk_kv_weigh_workspace_size bytes, 256-byte aligned (NULL when that is 0),
+ * whatever it holds; calls that may run concurrently need separate ones. Nothing is
+ * allocated: the call can be captured. No counterpart in the reference. */
+int qk_kv_weigh(const qk_kv_cache *cache, const qk_kv_batch *batch, const int32_t *seen,
+                const void *q, int q_type, int64_t q_stride, int64_t q_heads, float scale,
+                const float *lse, int64_t max_context, const qk_kv_weights *weights,
+                void *workspace, size_t workspace_bytes, qk_stream_t stream);
+
+/* Workspace bytes of qk_kv_weigh (0 for arguments that it rejects). */
+size_t qk_kv_weigh_workspace_size(const qk_kv_cache *cache, const qk_kv_batch *batch, int q_type,
+                                  int64_t q_heads, int64_t max_context);
+
+/* Cuts every sequence s whose context exceeds keep[s] (> 0) to keep[s] tokens, in
+ * place, for each key/value head on its own: those with position >= seen[s] -
+ * recent[s] stay, and of the others the ones with the most weight (ties, and latest
+ * tokens beyond the budget: the first slot first; NaN last). What stays before slot
+ * keep[s] stays where it is; the i-th one past it moves, with its key, value, weight
+ * and position, to the i-th slot that is left. Slots from keep[s] on then hold nothing
+ * of the sequence (their pages may serve others). context_out[s] (device, not the
+ * batch's context, so that every layer's cache can be cut by the same lengths)
+ * receives min(context, keep), or the context where nothing was cut.
+ * Later steps pass context_out as context and count `seen` on; attention sees kept
+ * tokens as it did, as long as it has no window (which would count slots).
+ * keep, recent, seen: device arrays of `sequences` (seen NULL: the contexts). The
+ * batch's token_start and tokens are not looked at. A page may belong to one
+ * sequence of the call only. Sequences with a page that is none, or longer than
+ * max_context or their page table, stay as they are and are reported (see
+ * qk_kv_cache::fault).
+ * workspace: qk_kv_evict_workspace_size bytes, 256-byte aligned, whatever it holds;
+ * calls that may run concurrently need separate ones. Nothing is allocated: the call
+ * can be captured. No counterpart in the reference. */
+int qk_kv_evict(const qk_kv_cache *cache, const qk_kv_batch *batch, const int32_t *seen,
+                const qk_kv_weights *weights, const int32_t *keep, const int32_t *recent,
+                int64_t max_context, int32_t *context_out, void *workspace, size_t workspace_bytes,
+                qk_stream_t stream);
+
+/* Workspace bytes of qk_kv_evict (0 for arguments that it rejects). */
+size_t qk_kv_evict_workspace_size(const qk_kv_cache *cache, const qk_kv_batch *batch,
+                                  int64_t max_context);
+
 /* Synchronises `stream`, then returns QK_ERR_RUNTIME (and clears what it
  * reports) if a call on this cache met a fault since the last check, else QK_OK;
  * the message names each kind that was met. Calls on the cache may be in flight on

@@ -72,6 +72,12 @@ class KVBatch(ctypes.Structure):
                 ("page_table", _c_void_p), ("table_stride", _i64)]
 
 
+class KVWeights(ctypes.Structure):
+    """qk_kv_weights: what the slots' tokens have gathered, and their positions."""
+
+    _fields_ = [("weight", _c_void_p), ("position", _c_void_p)]
+
+
 class Rope(ctypes.Structure):
     """qk_rope: head norms and rotation of q and k."""
 
@@ -119,6 +125,12 @@ _SIGNATURES = {
     "qk_paged_attention": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _int, _i64, _i64, _float,
                            _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
     "qk_paged_attention_workspace_size": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _int, _i64, _i64, _i64],
+    "qk_kv_weigh": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, _c_void_p, _int, _i64, _i64, _float,
+                    _c_void_p, _i64, ctypes.POINTER(KVWeights), _c_void_p, _size, _c_void_p],
+    "qk_kv_weigh_workspace_size": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _int, _i64, _i64],
+    "qk_kv_evict": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _c_void_p, ctypes.POINTER(KVWeights), _c_void_p,
+                    _c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p],
+    "qk_kv_evict_workspace_size": [ctypes.POINTER(KVCache), ctypes.POINTER(KVBatch), _i64],
     "qk_kv_check": [ctypes.POINTER(KVCache), _c_void_p],
     "qk_sample": [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                   _c_void_p, _c_void_p, _size, _c_void_p],
@@ -161,6 +173,7 @@ _RESTYPES = {"qk_last_error": ctypes.c_char_p, "qk_last_launch": ctypes.c_char_p
              "qk_matmul_workspace_size": _size,
              "qk_argmax_workspace_size": _size, "qk_ffn_workspace_size": _size,
              "qk_paged_attention_workspace_size": _size, "qk_sample_workspace_size": _size,
+             "qk_kv_weigh_workspace_size": _size, "qk_kv_evict_workspace_size": _size,
              "qk_ffn_gate_up_workspace_size": _size, "qk_matmul_segments_workspace_size": _size}
 
 _LIB = None
@@ -541,6 +554,28 @@ def paged_attention(cache: KVCache, batch: KVBatch, q, q_type: int, q_stride: in
     """qk_paged_attention: the new tokens' attention over their cached contexts."""
     check(load().qk_paged_attention(cache, batch, _ptr(q), q_type, q_stride, q_heads, scale, window, max_context,
                                     _ptr(out), _ptr(lse), _ptr(workspace), workspace_bytes, _stream_ptr(stream)))
+
+
+def kv_weigh_workspace_size(cache: KVCache, batch: KVBatch, q_type: int, q_heads: int, max_context: int) -> int:
+    return load().qk_kv_weigh_workspace_size(cache, batch, q_type, q_heads, max_context)
+
+
+def kv_weigh(cache: KVCache, batch: KVBatch, seen, q, q_type: int, q_stride: int, q_heads: int, scale: float, lse,
+             max_context: int, weights: KVWeights, workspace, workspace_bytes: int, stream=None) -> None:
+    """qk_kv_weigh: the softmax weight that cached tokens get from the new ones, added to what they have gathered."""
+    check(load().qk_kv_weigh(cache, batch, _ptr(seen), _ptr(q), q_type, q_stride, q_heads, scale, _ptr(lse), max_context,
+                             weights, _ptr(workspace), workspace_bytes, _stream_ptr(stream)))
+
+
+def kv_evict_workspace_size(cache: KVCache, batch: KVBatch, max_context: int) -> int:
+    return load().qk_kv_evict_workspace_size(cache, batch, max_context)
+
+
+def kv_evict(cache: KVCache, batch: KVBatch, seen, weights: KVWeights, keep, recent, max_context: int, context_out,
+             workspace, workspace_bytes: int, stream=None) -> None:
+    """qk_kv_evict: every sequence cut to its latest tokens and those with the most weight, in place."""
+    check(load().qk_kv_evict(cache, batch, _ptr(seen), weights, _ptr(keep), _ptr(recent), max_context, _ptr(context_out),
+                             _ptr(workspace), workspace_bytes, _stream_ptr(stream)))
 
 
 def kv_check(cache: KVCache, stream=None) -> None:

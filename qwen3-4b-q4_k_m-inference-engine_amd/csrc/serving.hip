@@ -65,6 +65,25 @@ int check_heads(const qk_kv_cache* c, const qk_kv_batch* b, int64_t q_heads, int
   return QK_OK;
 }
 
+int check_weights(const qk_kv_weights* w) {
+  if (!w || !w->weight || !w->position) return refuse("weights must be non-null");
+  if (misaligned(w->weight, 4) || misaligned(w->position, 4)) return refuse("weights must be 4-byte aligned");
+  return QK_OK;
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need != 0 && !workspace) return refuse("workspace must be non-null");
+  if (bytes < need) return refuse("workspace too small");
+  if (misaligned(workspace, 256)) return refuse("workspace must be 256-byte aligned");
+  return QK_OK;
+}
+
+// Slots that a list and a grid hold.
+bool evict_fits(const qk_kv_cache* c, const qk_kv_batch* b, int64_t max_context) {
+  const int64_t units = b->sequences * c->kv_heads;
+  return max_context <= qk::kMostPositions && units <= (int64_t{1} << 21) && units * max_context <= (int64_t{1} << 32);
+}
+
 KvArgs kv_args(const qk_kv_cache* c, const qk_kv_batch* b) {
   KvArgs a;
   a.k = static_cast<uint16_t*>(c->k);
@@ -215,6 +234,85 @@ int qk_kv_rows(const qk_kv_cache* cache, const qk_kv_batch* batch, void* k_out, 
   qk::RowsArgs a{kv_args(cache, batch), k_out, v_out};
   return finish(qk::launch_kv_rows(a, cache->type, static_cast<int>(cache->head_dim), out_type, as_stream(stream)),
                 "cache rows launch failed");
+}
+
+size_t qk_kv_weigh_workspace_size(const qk_kv_cache* cache, const qk_kv_batch* batch, int q_type, int64_t q_heads,
+                                  int64_t max_context) {
+  if (check_shapes(cache, batch) != QK_OK || check_heads(cache, batch, q_heads, q_type) != QK_OK || max_context < 0) return 0;
+  const qk::WeighPlan plan = qk::plan_weigh(batch->tokens, batch->sequences, q_heads, cache->kv_heads, max_context);
+  return qk::weigh_fits(plan, batch->sequences, cache->kv_heads) ? plan.bytes : 0;
+}
+
+int qk_kv_weigh(const qk_kv_cache* cache, const qk_kv_batch* batch, const int32_t* seen, const void* q, int q_type,
+                int64_t q_stride, int64_t q_heads, float scale, const float* lse, int64_t max_context,
+                const qk_kv_weights* weights, void* workspace, size_t workspace_bytes, qk_stream_t stream) {
+  int status = check_shapes(cache, batch);
+  if (status == QK_OK) status = check_heads(cache, batch, q_heads, q_type);
+  if (status != QK_OK) return status;
+  if (max_context < 0) return refuse("weigh max_context must not be negative");
+  if (!std::isfinite(scale)) return refuse("weigh scale must be finite");
+  if (batch->tokens == 0 || batch->sequences == 0) return QK_OK;
+  if (q_stride < q_heads * cache->head_dim || q_stride > (int64_t{1} << 40)) return refuse("weigh q_stride must hold a token's heads");
+  if (q_stride % (q_type == QK_TYPE_F32 ? 4 : 8) != 0) return refuse("weigh q rows must be 16-byte aligned");
+  status = check_pointers(cache, batch);
+  if (status == QK_OK) status = check_weights(weights);
+  if (status != QK_OK) return status;
+  if (!q || !lse) return refuse("weigh pointers must be non-null");
+  if (misaligned(q, 16) || misaligned(lse, 4) || misaligned(seen, 4)) return refuse("weigh q must be 16-byte, lse and seen 4-byte aligned");
+  const qk::WeighPlan plan = qk::plan_weigh(batch->tokens, batch->sequences, q_heads, cache->kv_heads, max_context);
+  if (!qk::weigh_fits(plan, batch->sequences, cache->kv_heads))
+    return refuse("weights of so many sequences, heads and keys do not fit one launch");
+  status = check_workspace(workspace, workspace_bytes, plan.bytes);
+  if (status != QK_OK) return status;
+  qk::WeighArgs a{};
+  a.kv = kv_args(cache, batch);
+  a.seen = seen;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.q_heads = static_cast<int32_t>(q_heads);
+  a.group = static_cast<int32_t>(q_heads / cache->kv_heads);
+  a.scale = scale;
+  a.lse = lse;
+  a.weight = weights->weight;
+  a.position = weights->position;
+  return finish(qk::launch_kv_weigh(a, plan, cache->type, static_cast<int>(cache->head_dim), q_type, workspace, as_stream(stream)),
+                "weigh launch failed");
+}
+
+size_t qk_kv_evict_workspace_size(const qk_kv_cache* cache, const qk_kv_batch* batch, int64_t max_context) {
+  if (check_shapes(cache, batch) != QK_OK || batch->sequences == 0 || max_context < 1 || !evict_fits(cache, batch, max_context))
+    return 0;
+  return qk::evict_workspace(batch->sequences, cache->kv_heads, max_context);
+}
+
+int qk_kv_evict(const qk_kv_cache* cache, const qk_kv_batch* batch, const int32_t* seen, const qk_kv_weights* weights,
+                const int32_t* keep, const int32_t* recent, int64_t max_context, int32_t* context_out, void* workspace,
+                size_t workspace_bytes, qk_stream_t stream) {
+  int status = check_shapes(cache, batch);
+  if (status != QK_OK) return status;
+  if (max_context < 1) return refuse("evict max_context must be positive");
+  if (batch->sequences == 0) return QK_OK;
+  if (!evict_fits(cache, batch, max_context)) return refuse("eviction of so many sequences, heads and tokens does not fit one launch");
+  status = check_pointers(cache, batch);
+  if (status == QK_OK) status = check_weights(weights);
+  if (status != QK_OK) return status;
+  if (!keep || !recent || !context_out) return refuse("evict pointers must be non-null");
+  if (misaligned(keep, 4) || misaligned(recent, 4) || misaligned(context_out, 4) || misaligned(seen, 4))
+    return refuse("evict arrays must be 4-byte aligned");
+  if (context_out == batch->context) return refuse("evict context_out must not be the batch's context");
+  status = check_workspace(workspace, workspace_bytes, qk::evict_workspace(batch->sequences, cache->kv_heads, max_context));
+  if (status != QK_OK) return status;
+  qk::EvictArgs a{};
+  a.kv = kv_args(cache, batch);
+  a.seen = seen;
+  a.keep = keep;
+  a.recent = recent;
+  a.weight = weights->weight;
+  a.position = weights->position;
+  a.context_out = context_out;
+  a.width = static_cast<int32_t>(max_context);
+  return finish(qk::launch_kv_evict(a, cache->type, static_cast<int>(cache->head_dim), workspace, as_stream(stream)),
+                "evict launch failed");
 }
 
 int qk_kv_check(const qk_kv_cache* cache, qk_stream_t stream) {

@@ -10,6 +10,7 @@
 #include "attention_plan.hpp"
 #include "kv_index.hpp"
 #include "qk_abi.h"
+#include "weigh_plan.hpp"
 
 namespace qk {
 
@@ -42,6 +43,41 @@ struct RowsArgs {
   void* v_out;
 };
 hipError_t launch_kv_rows(const RowsArgs& a, int type, int head_dim, int out_type, hipStream_t stream);
+
+struct WeighArgs {
+  KvArgs kv;
+  const int32_t* seen;  // tokens of each sequence, for the new ones' positions; nullptr: the contexts
+  const void* q;
+  int64_t q_stride;
+  int32_t q_heads, group;
+  float scale;
+  const float* lse;
+  float* weight;      // [pages x kv_heads x page_size], as position
+  int32_t* position;
+  // the plan's part (launch_kv_weigh)
+  int32_t key_parts, part_keys, row_parts, most_keys;
+  float* parts;
+};
+hipError_t launch_kv_weigh(WeighArgs a, const WeighPlan& plan, int type, int head_dim, int q_type, void* workspace,
+                           hipStream_t stream);
+
+struct EvictArgs {
+  KvArgs kv;  // token_start is not looked at
+  const int32_t* seen;
+  const int32_t* keep;
+  const int32_t* recent;
+  float* weight;
+  int32_t* position;
+  int32_t* context_out;
+  int32_t width;  // the longest context that the workspace has room for
+  // launch_kv_evict's part
+  uint32_t* moves;  // [sequences x kv_heads]
+  uint32_t* ranks;  // [sequences x kv_heads x width]
+  int32_t* lists;   // [sequences x kv_heads x 2 x half of width]: places, then sources
+  int32_t move_parts, unit_values, unit_bytes;
+};
+hipError_t launch_kv_evict(EvictArgs a, int type, int head_dim, void* workspace, hipStream_t stream);
+size_t evict_workspace(int64_t sequences, int64_t kv_heads, int64_t width);
 
 hipError_t launch_kv_fault_clear(uint32_t* word, uint32_t bits, hipStream_t stream);
 
