@@ -35,6 +35,17 @@ __device__ __forceinline__ uint16_t narrow(float v) {
     return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
 
+// a c + b n. EACH: every product rounded by itself, so that the codes of a Q4_1 cache do
+// not depend on which of them the compiler fuses.
+template <bool EACH>
+__device__ __forceinline__ float turned(float a, float c, float b, float n) {
+  if constexpr (EACH) {
+#pragma clang fp contract(off)
+    return a * c + b * n;
+  }
+  return a * c + b * n;
+}
+
 // A row's lane of a Q4_1 cache: x0 its values 4 u .. of block `u / 4`, x1 the ones 16
 // on, u = lane of the block. The block's d and m are rounded first (d towards zero,
 // so that no value leaves F16), and the codes go by them. fp32, as the row is: a value
@@ -109,11 +120,18 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     // where tokens were evicted, a token's position is not its place in the cache
     const int64_t angle = a.seen ? static_cast<int64_t>(a.seen[s]) - a.kv.context[s] + position : position;
     const double turns = static_cast<double>(angle) * (exp2(a.turns_log2 * tid) * 0.15915494309189535);
-    const float part = static_cast<float>(turns - floor(turns));
-    float sn, cs;
-    sincospif(2.0f * part, &sn, &cs);
-    cosine[tid] = cs;
-    sine[tid] = sn;
+    if constexpr (Q4) {  // codes are decided by the last bits of what is stored
+      double sn, cs;
+      sincospi(2.0 * (turns - floor(turns)), &sn, &cs);
+      cosine[tid] = static_cast<float>(cs);
+      sine[tid] = static_cast<float>(sn);
+    } else {
+      const float part = static_cast<float>(turns - floor(turns));
+      float sn, cs;
+      sincospif(2.0f * part, &sn, &cs);
+      cosine[tid] = cs;
+      sine[tid] = sn;
+    }
   }
   __syncthreads();
   if (row >= rows) return;
@@ -121,9 +139,18 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   const float* norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
   if (norm) {
     float sum = 0.0f;
+    if constexpr (Q4) {
+      double squares = 0.0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sum));
-    sum = row_lanes_sum<L>(sum);
+      for (int i = 0; i < 4; ++i) squares += static_cast<double>(x0[i]) * x0[i] + static_cast<double>(x1[i]) * x1[i];
+#pragma unroll
+      for (int off = 1; off < L; off <<= 1) squares += __shfl_xor(squares, off);
+      sum = static_cast<float>(squares);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sum));
+      sum = row_lanes_sum<L>(sum);
+    }
     const float inv = rsqrtf(sum * (1.0f / D) + a.eps);
     x0 = x0 * inv * *reinterpret_cast<const f32x4_a4*>(norm + first);
     x1 = x1 * inv * *reinterpret_cast<const f32x4_a4*>(norm + second);
@@ -133,18 +160,18 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float c = cosine[4 * u + i], n = sine[4 * u + i], b = x0[i];
-        x0[i] = b * c - x1[i] * n;
-        x1[i] = x1[i] * c + b * n;
+        x0[i] = turned<Q4>(b, c, x1[i], -n);
+        x1[i] = turned<Q4>(x1[i], c, b, n);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float c0 = cosine[4 * u + i], n0 = sine[4 * u + i], b0 = x0[2 * i];
         const float c1 = cosine[4 * u + 2 + i], n1 = sine[4 * u + 2 + i], b1 = x1[2 * i];
-        x0[2 * i] = b0 * c0 - x0[2 * i + 1] * n0;
-        x0[2 * i + 1] = x0[2 * i + 1] * c0 + b0 * n0;
-        x1[2 * i] = b1 * c1 - x1[2 * i + 1] * n1;
-        x1[2 * i + 1] = x1[2 * i + 1] * c1 + b1 * n1;
+        x0[2 * i] = turned<Q4>(b0, c0, x0[2 * i + 1], -n0);
+        x0[2 * i + 1] = turned<Q4>(x0[2 * i + 1], c0, b0, n0);
+        x1[2 * i] = turned<Q4>(b1, c1, x1[2 * i + 1], -n1);
+        x1[2 * i + 1] = turned<Q4>(x1[2 * i + 1], c1, b1, n1);
       }
     }
   }

@@ -17,9 +17,12 @@ namespace qk {
 namespace {
 
 constexpr int kRankKeys = 1024;  // slots of a workgroup that ranks
-constexpr int kThreads = 1024;   // of one that selects
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kAhead = 4;  // of one that selects; loads of four ranks in flight
 constexpr int kBits = 11, kBins = 1 << kBits, kCopies = 4;  // of a digit; copies of the counts, against collisions
 constexpr uint32_t kLatest = 0xFFFFFFFFu;
+
+// Ranks of a (sequence, head) begin at 16 bytes each.
+__host__ __device__ constexpr int64_t rank_stride(int64_t width) { return (width + 3) & ~int64_t{3}; }
 
 // A sequence's context and budget, or a budget of all where nothing is to be done.
 struct Cut {
@@ -51,7 +54,7 @@ __global__ __launch_bounds__(256) void kv_evict_rank_kernel(const EvictArgs a) {
   const Cut c = cut_of(a, s);
   if (c.keep == c.context) return;
   const int64_t seen = a.seen ? a.seen[s] : c.context, from = seen - (a.recent[s] > 0 ? a.recent[s] : 0);
-  uint32_t* ranks = a.ranks + static_cast<int64_t>(unit) * a.width;
+  uint32_t* ranks = a.ranks + static_cast<int64_t>(unit) * rank_stride(a.width);
   for (int slot = part * kRankKeys + static_cast<int>(threadIdx.x); slot < min(c.context, (part + 1) * kRankKeys); slot += 256) {
     const int entry = slot / a.kv.page_size, page = kv_page(a.kv, s, entry);
     uint32_t rank = 0;
@@ -64,7 +67,7 @@ __global__ __launch_bounds__(256) void kv_evict_rank_kernel(const EvictArgs a) {
 }
 
 // Sums over the workgroup's threads before the calling one, and of all.
-__device__ __forceinline__ int before_mine(int mine, int (&waves)[kThreads / 64 + 1], int& all) {
+__device__ __forceinline__ int before_mine(int mine, int (&waves)[kWaves], int& all) {
   const int lane = static_cast<int>(threadIdx.x & 63), wave = static_cast<int>(threadIdx.x >> 6);
   int run = mine;
 #pragma unroll
@@ -76,7 +79,7 @@ __device__ __forceinline__ int before_mine(int mine, int (&waves)[kThreads / 64 
   if (lane == 63) waves[wave] = run;
   __syncthreads();
   int before = 0, total = 0;
-  for (int w = 0; w < kThreads / 64; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     before += w < wave ? waves[w] : 0;
     total += waves[w];
   }
@@ -84,10 +87,25 @@ __device__ __forceinline__ int before_mine(int mine, int (&waves)[kThreads / 64 
   return before + run - mine;
 }
 
+// The same of a number a wave, for all of its lanes.
+__device__ __forceinline__ int before_wave(int mine, int (&waves)[kWaves], int& all) {
+  const int wave = static_cast<int>(threadIdx.x >> 6);
+  __syncthreads();  // of the call before
+  if ((threadIdx.x & 63) == 0) waves[wave] = mine;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? waves[w] : 0;
+    all += waves[w];
+  }
+  return before;
+}
+
 __global__ __launch_bounds__(kThreads) void kv_evict_select_kernel(const EvictArgs a) {
   __shared__ uint32_t counts[kCopies][kBins];
-  __shared__ int waves[kThreads / 64 + 1];
-  __shared__ uint32_t digit_found, above_found;
+  __shared__ int waves[kWaves];
+  __shared__ uint32_t digit_found, above_found, alike_found;
   const int tid = static_cast<int>(threadIdx.x);
   const int unit = static_cast<int>(blockIdx.x), s = unit / a.kv.kv_heads, head = unit % a.kv.kv_heads;
   const Cut c = cut_of(a, s);
@@ -106,7 +124,9 @@ __global__ __launch_bounds__(kThreads) void kv_evict_select_kernel(const EvictAr
     a.moves[unit] = 0;
   }
   if (bad || c.keep == c.context) return;
-  const uint32_t* ranks = a.ranks + static_cast<int64_t>(unit) * a.width;
+  const uint32_t* ranks = a.ranks + static_cast<int64_t>(unit) * rank_stride(a.width);
+
+  const int last_four = (c.context - 1) & ~3;  // what four loads past the end take instead
 
   // the rank that the keep-th stands at, digit by digit; `wanted` of those that share the digits so far
   uint32_t prefix = 0;
@@ -116,10 +136,16 @@ __global__ __launch_bounds__(kThreads) void kv_evict_select_kernel(const EvictAr
     shift -= bits;
     for (int i = tid; i < kCopies * kBins; i += kThreads) (&counts[0][0])[i] = 0;
     __syncthreads();
-    for (int i = tid; i < c.context; i += kThreads) {
-      const uint32_t rank = ranks[i];
-      if (shift + bits == 32 || rank >> (shift + bits) == prefix)
-        atomicAdd(&counts[tid >> 6 & (kCopies - 1)][rank >> shift & ((1u << bits) - 1)], 1u);
+    for (int base = 4 * tid; base < c.context; base += 4 * kAhead * kThreads) {
+      u32x4 rank[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) rank[k] = load16(ranks + min(base + 4 * k * kThreads, last_four));
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (base + 4 * k * kThreads + j < c.context && (shift + bits == 32 || rank[k][j] >> (shift + bits) == prefix))
+            atomicAdd(&counts[tid >> 6 & (kCopies - 1)][rank[k][j] >> shift & ((1u << bits) - 1)], 1u);
     }
     __syncthreads();
     // bins from the highest down, two a thread
@@ -139,6 +165,7 @@ __global__ __launch_bounds__(kThreads) void kv_evict_select_kernel(const EvictAr
       if (above < wanted && above + here >= wanted) {
         digit_found = static_cast<uint32_t>(high - k);
         above_found = static_cast<uint32_t>(above);
+        alike_found = static_cast<uint32_t>(here);
       }
       above += here;
     }
@@ -147,26 +174,101 @@ __global__ __launch_bounds__(kThreads) void kv_evict_select_kernel(const EvictAr
     wanted -= static_cast<int>(above_found);
   }
 
-  // slots in runs, one a thread: ties with that rank stay from the first slot on
-  const int run = (c.context + kThreads - 1) / kThreads, lo = min(tid * run, c.context), hi = min(lo + run, c.context);
-  int ties = 0, all;
-  for (int i = lo; i < hi; ++i) ties += ranks[i] == prefix;
-  const int ties_before = before_mine(ties, waves, all);
-  int free_places = 0, sources = 0;
+  // Slots in runs, one a wave, four a lane at a time: those that stay and lie past the
+  // budget, and the places that others leave before it, numbered in the order of the
+  // slots. Of slots with that last rank the first `wanted` stay.
+  constexpr int kTurn = 4 * 64;
+  const int lane = tid & 63, run = (c.context + kTurn * kWaves - 1) / (kTurn * kWaves) * kTurn;
+  const int lo = (tid >> 6) * run, hi = min(lo + run, c.context);
   const auto walk = [&](auto&& at) {
-    int tie = ties_before;
-    for (int i = lo; i < hi; ++i) {
-      const uint32_t rank = ranks[i];
-      const bool stays = rank > prefix || (rank == prefix && tie < wanted);
-      tie += rank == prefix;
-      if (stays != (i < c.keep)) at(i, stays);
+    for (int base = lo + 4 * lane; base - 4 * lane < hi; base += kTurn * kAhead) {
+      u32x4 rank[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) rank[k] = load16(ranks + min(base + kTurn * k, last_four));
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) at(base + kTurn * k, rank[k]);
     }
   };
-  walk([&](int, bool stays) { stays ? ++sources : ++free_places; });
-  int place_at = before_mine(free_places, waves, all), source_at = before_mine(sources, waves, all);
+  const uint64_t lower = (uint64_t{1} << lane) - 1;
+  // of four flags a lane: how many in the lanes before this one, and in all
+  const auto count = [&](const bool (&flag)[4], int& in_all) {
+    int before = 0;
+    in_all = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t lanes = __ballot(flag[j]);
+      before += __builtin_popcountll(lanes & lower);
+      in_all += __builtin_popcountll(lanes);
+    }
+    return before;
+  };
+  int all, ties_before = 0;
+  const bool in_order = static_cast<int>(alike_found) > wanted;
+  if (in_order) {
+    int ties = 0;
+    walk([&](int at, const u32x4& rank) {
+      bool alike[4];
+      int in_all;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) alike[j] = at + j < hi && rank[j] == prefix;
+      count(alike, in_all);
+      ties += in_all;
+    });
+    ties_before = before_wave(ties, waves, all);
+  }
+  int tie = ties_before;
+  const auto staying = [&](int at, const u32x4& rank, bool (&stays)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) stays[j] = at + j < hi && rank[j] >= prefix;
+    if (!in_order) return;
+    bool alike[4];
+    int in_all;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) alike[j] = at + j < hi && rank[j] == prefix;
+    int before = tie + count(alike, in_all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      stays[j] &= !alike[j] || before < wanted;
+      before += alike[j];
+    }
+    tie += in_all;
+  };
+  const auto moving = [&](int at, const u32x4& rank, bool (&leaves)[4], bool (&moves)[4]) {
+    bool stays[4];
+    staying(at, rank, stays);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      leaves[j] = at + j < hi && !stays[j] && at + j < c.keep;
+      moves[j] = stays[j] && at + j >= c.keep;
+    }
+  };
+  int free_places = 0, sources = 0;
+  walk([&](int at, const u32x4& rank) {
+    bool leaves[4], moves[4];
+    int in_all;
+    moving(at, rank, leaves, moves);
+    count(leaves, in_all);
+    free_places += in_all;
+    count(moves, in_all);
+    sources += in_all;
+  });
+  int place_at = before_wave(free_places, waves, all), source_at = before_wave(sources, waves, all);
   const int most = (a.width + 1) / 2;
   int32_t* const places = a.lists + static_cast<int64_t>(unit) * 2 * most;
-  walk([&](int i, bool stays) { stays ? places[most + source_at++] = i : places[place_at++] = i; });
+  tie = ties_before;
+  walk([&](int at, const u32x4& rank) {
+    bool leaves[4], moves[4];
+    int places_here, sources_here;
+    moving(at, rank, leaves, moves);
+    int place = place_at + count(leaves, places_here), source = source_at + count(moves, sources_here);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (leaves[j]) places[place++] = at + j;
+      if (moves[j]) places[most + source++] = at + j;
+    }
+    place_at += places_here;
+    source_at += sources_here;
+  });
   if (tid == 0) a.moves[unit] = static_cast<uint32_t>(all);
 }
 
@@ -210,7 +312,7 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(const EvictArgs a) {
 
 size_t evict_workspace(int64_t sequences, int64_t kv_heads, int64_t width) {
   const int64_t units = sequences * kv_heads;
-  return static_cast<size_t>(((units * 4 + 255) & ~int64_t{255}) + units * width * 4 + units * 2 * ((width + 1) / 2) * 4);
+  return static_cast<size_t>(((units * 4 + 255) & ~int64_t{255}) + units * rank_stride(width) * 4 + units * 2 * ((width + 1) / 2) * 4);
 }
 
 hipError_t launch_kv_evict(EvictArgs a, int type, int head_dim, void* workspace, hipStream_t stream) {
@@ -218,7 +320,7 @@ hipError_t launch_kv_evict(EvictArgs a, int type, int head_dim, void* workspace,
   char* ws = static_cast<char*>(workspace);
   a.moves = reinterpret_cast<uint32_t*>(ws);
   a.ranks = reinterpret_cast<uint32_t*>(ws + ((units * 4 + 255) & ~int64_t{255}));
-  a.lists = reinterpret_cast<int32_t*>(a.ranks + units * a.width);
+  a.lists = reinterpret_cast<int32_t*>(a.ranks + units * rank_stride(a.width));
   const bool q4 = type == QK_TYPE_Q4_1;
   a.unit_values = q4 ? kQ4Values : 1;
   a.unit_bytes = q4 ? kQ4Bytes : 2;

@@ -42,10 +42,10 @@ __device__ __forceinline__ int64_t weight_of_key(const WeighArgs& a, int s, int 
   return weight_place(a, kv_page(a.kv, s, entry), key - entry * a.kv.page_size, head);
 }
 // What a new token's slot held before is of another token: its weight begins here.
-__device__ __forceinline__ void add_weight(const WeighArgs& a, const KvSequence& q, int s, int key, int64_t at, float sum,
-                                           bool first_time) {
+__device__ __forceinline__ void add_weight(const WeighArgs& a, const KvSequence& q, int s, int key, int64_t at, float old,
+                                           float sum, bool first_time) {
   const bool is_new = key >= q.first;
-  a.weight[at] = (is_new && first_time ? 0.0f : a.weight[at]) + sum;
+  a.weight[at] = (is_new && first_time ? 0.0f : old) + sum;
   if (is_new && first_time) a.position[at] = (a.seen ? a.seen[s] - a.kv.context[s] : 0) + key;
 }
 
@@ -77,14 +77,19 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
   typedef Num<BF16> N;
   typedef typename N::V8 V8;
   constexpr int NP = kParts<BF16, Q32>, KS = D / 32;
-  constexpr int LPK = Q4 ? D / 16 : D / 8, KPL = 64 / LPK, NL = kBlock / KPL;  // lanes a key, keys a load, loads a block
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds[kWaves][kBlock * 2 * D];
+  constexpr int LPK = D / 8, KPL = 64 / LPK, NL = Q4 ? 2 : kBlock / KPL;  // lanes a key, keys a load, loads a block
+  __shared__ __attribute__((aligned(16))) uint8_t k_lds[kWaves][Q4 ? 16 : kBlock * 2 * D];
   __shared__ int64_t place[kWaves][2][kBlock];
   __shared__ float factors[kWaves][16], logs[kWaves][16];
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = static_cast<int>(blockIdx.x) % a.kv.kv_heads, unit = static_cast<int>(blockIdx.x) / a.kv.kv_heads;
-  const int s = unit / a.key_parts, part = unit % a.key_parts;
+  // Workgroups go to the eight XCDs in turn: the heads of a unit to the same one where
+  // their rows share lines of memory (see paged_attention_few_q4.hip).
+  const int heads = a.kv.kv_heads, block = static_cast<int>(blockIdx.x);
+  const bool shared = Q4 && a.kv.head_stride < a.kv.token_stride;
+  const int eight = block / (8 * heads), within = block - eight * 8 * heads, side = min(8, a.kv.sequences * a.key_parts - 8 * eight);
+  const int head = shared ? within / side : block % heads, unit = shared ? 8 * eight + within - head * side : block / heads;
+  const int part = unit / a.kv.sequences, s = unit - part * a.kv.sequences;  // the last parts are empty where contexts are short
   KvSequence seq;
   int keys;
   if (!weigh_keys(a, s, head == 0 && part == 0, seq, keys)) return;
@@ -104,25 +109,29 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
     const auto look_up = [&](int b) {
       page = a.kv.page_table[kv_table_at(a.kv, s, key_of(b) / a.kv.page_size, listed)];
     };
-    int64_t at = 0, next_at = 0;  // of the lane's key's weight
+    // Of the lane's key's weight, and what is there. That is loaded with the block's keys,
+    // before them: a load at the end of a block would have to wait for the next one's.
+    int64_t at = 0, next_at = 0;
+    float old = 0.0f, next_old = 0.0f;
     const auto settle = [&](int b) {
       const bool ok = listed && page >= 0 && page < a.kv.pages;
       bad |= !ok;
       const int slot = key_of(b) % a.kv.page_size;
       next_at = weight_place(a, ok ? page : -1, slot, head);
+      next_old = a.weight[next_at < 0 ? 0 : next_at];
       const int64_t to = kv_place(a.kv, ok ? page : 0, slot, head);
       place[wave][b / kWaves & 1][lane & 31] = Q4 ? q4_bytes(to) : to;
       __builtin_amdgcn_wave_barrier();
     };
-    std::conditional_t<Q4, Q4Piece, u32x4> reg[NL];
+    // 16-bit rows as whole rows, through LDS; of Q4_1 ones each lane takes the quarter that it multiplies
+    std::conditional_t<Q4, Q4Quarter<KS>, u32x4> reg[NL];
     const auto load = [&](int b) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int64_t from = place[wave][b / kWaves & 1][KPL * i + lane / LPK];
         if constexpr (Q4)
-          reg[i] = q4_load(reinterpret_cast<const uint8_t*>(a.kv.k) + from, lane % LPK);
+          reg[i] = q4_load_quarter<KS>(reinterpret_cast<const uint8_t*>(a.kv.k) + place[wave][b / kWaves & 1][16 * i + col], grp);
         else
-          reg[i] = stream_load16(a.kv.k + from + 8 * (lane % LPK));
+          reg[i] = stream_load16(a.kv.k + place[wave][b / kWaves & 1][KPL * i + lane / LPK] + 8 * (lane % LPK));
       }
     };
     look_up(wave);
@@ -138,38 +147,49 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
       const bool live = row < rows;
       const int token = seq.row + (live ? row / a.group : 0), h = head * a.group + (live ? row % a.group : 0);
       float factor = a.scale * kLog2e;
-      const int64_t from = token * a.q_stride + static_cast<int64_t>(h) * D + 8 * grp;
+      const int64_t from = token * a.q_stride + static_cast<int64_t>(h) * D;
+      // the first of step k's values 4 i .. 4 i + 3
+      const auto quad_at = [&](int k, int i) { return Q4 ? q4_quarter_value<KS>(grp, k) + 16 * i : 32 * k + 8 * grp + 4 * i; };
+      // which of those is its e-th
+      const auto value_at = [](int e) { return Q4 ? q4_pair_value(e) % 16 + (e & 2 ? 4 : 0) : e; };
       if constexpr (Q32) {
         float x[KS][8];
         float most = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + from + 32 * k + i);
+          for (int i = 0; i < 2; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + from + quad_at(k, i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              x[k][i + j] = live ? v[j] : 0.0f;
-              most = fmaxf(most, fabsf(x[k][i + j]));
+              x[k][4 * i + j] = live ? v[j] : 0.0f;
+              most = fmaxf(most, fabsf(x[k][4 * i + j]));
             }
           }
+        int e = 0;
         if constexpr (!BF16) {
           most = swap32_max(swap16_max(most));
           const bool scaled = most > 0.0f && most < __builtin_inff();
-          const int e = scaled ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;  // the row's largest in [2^13, 2^14)
+          e = scaled ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;  // the row's largest in [2^13, 2^14)
           factor = ldexpf(factor, -e);
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[k][i] = ldexpf(x[k][i], e);
         }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) split8<BF16, NP>(x[k], q[k]);
+        for (int k = 0; k < KS; ++k) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = ldexpf(x[k][value_at(i)], e);
+          split8<BF16, NP>(y, q[k]);
+        }
       } else {
+        typedef typename N::T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const u32x4 v = load16(static_cast<const uint16_t*>(a.q) + from + 32 * k);
-          q[k][0] = __builtin_bit_cast(V8, live ? v : u32x4{});
+          T4 v[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            v[i] = *reinterpret_cast<const T4*>(static_cast<const typename N::T*>(a.q) + from + quad_at(k, i));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[k][0][i] = live ? v[value_at(i) / 4][value_at(i) % 4] : static_cast<typename N::T>(0.0f);
         }
       }
       if (grp == 0) {
@@ -185,35 +205,42 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
     const int any_sees = seq.first + (end_row - 1) / a.group;
 
     uint8_t* const ks = k_lds[wave];
+    const Q4Exponents exponents;
     for (int b = wave; b < blocks; b += kWaves) {
       const int key0 = lo + b * kBlock;
+      f32x4 x[2] = {};
+      if constexpr (Q4) {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int key = KPL * i + lane / LPK;
-        if constexpr (Q4) {
-          u32x4 low, high;
-          q4_values(reg[i], low, high);
-          *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK))) = low;
-          *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, q4_chunk(lane % LPK) + 2)) = high;
-        } else {
-          *reinterpret_cast<u32x4*>(ks + k_chunk<D>(key, lane % LPK)) = reg[i];
-        }
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const half2_q4 dm = __builtin_bit_cast(half2_q4, reg[i].dm);
+            half2_q4 pairs[4];
+            q4_pairs(reg[i].codes[k], half2_q4{dm.x, dm.x}, half2_q4{dm.y, dm.y}, exponents, pairs);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) x[i] = N::mfma16(q[k][p], __builtin_bit_cast(V8, pairs), x[i]);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4*>(ks + k_chunk<D>(KPL * i + lane / LPK, lane % LPK)) = reg[i];
       }
       at = next_at;
+      old = next_old;
       // past the last block loads are of its last key: a path around them would make every wait one for all loads
       settle(b + kWaves);
       load(b + kWaves);
       look_up(b + 2 * kWaves);
       __builtin_amdgcn_wave_barrier();
-      f32x4 x[2] = {};
+      if constexpr (!Q4) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const V8 key = __builtin_bit_cast(V8, load16(ks + i * (16 * 2 * D) + k_chunk<D>(col, 4 * k + grp)));
+          for (int i = 0; i < 2; ++i) {
+            const V8 key = __builtin_bit_cast(V8, load16(ks + i * (16 * 2 * D) + k_chunk<D>(col, 4 * k + grp)));
 #pragma unroll
-          for (int p = 0; p < NP; ++p) x[i] = N::mfma16(q[k][p], key, x[i]);
-        }
+            for (int p = 0; p < NP; ++p) x[i] = N::mfma16(q[k][p], key, x[i]);
+          }
+      }
       float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -228,7 +255,7 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
       }
       const int key = key0 + lane;
       if (lane < kBlock && key < hi && at >= 0 && (key <= any_sees || begin == 0))
-        add_weight(a, seq, s, key, at, lane < 16 ? sum[0] : sum[1], begin == 0);
+        add_weight(a, seq, s, key, at, old, lane < 16 ? sum[0] : sum[1], begin == 0);
       __builtin_amdgcn_wave_barrier();
     }
   }
@@ -400,7 +427,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_weigh_many_kernel(const Wei
       a.parts[(static_cast<int64_t>(row_part) * a.kv.sequences * a.kv.kv_heads + unit_at) * width + key] = sum[g];
     } else {
       const int64_t at = weight_of_key(a, s, key, head);
-      if (at >= 0) add_weight(a, seq, s, key, at, sum[g], true);
+      if (at >= 0) add_weight(a, seq, s, key, at, a.weight[at], sum[g], true);
     }
   }
   if (__any(bad) && lane == 0) kv_fault(a.kv, QK_KV_FAULT_PAGE);
@@ -418,7 +445,7 @@ __global__ __launch_bounds__(256) void kv_weigh_join_kernel(const WeighArgs a) {
   for (int p = 0; p < a.row_parts; ++p)
     sum += a.parts[(static_cast<int64_t>(p) * a.kv.sequences * a.kv.kv_heads + unit_at) * width + key];
   const int64_t at = weight_of_key(a, s, key, head);
-  if (at >= 0) add_weight(a, seq, s, key, at, sum, true);
+  if (at >= 0) add_weight(a, seq, s, key, at, a.weight[at], sum, true);
 }
 
 }  // namespace

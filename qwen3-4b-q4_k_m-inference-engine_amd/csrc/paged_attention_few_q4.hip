@@ -49,12 +49,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
   constexpr int NB = 2, kSets = NB / kGroups;  // blocks a wave and turn, a group and turn
   static_assert(NB * kBlock == 64, "a turn's keys are looked up a lane each");
   constexpr int kRow = D / 8 + D / 32;      // dwords of a row in LDS: codes, then d and m of each block
-  typedef uint32_t Codes __attribute__((ext_vector_type(KS)));
-  typedef Codes Codes_a4 __attribute__((aligned(4)));
-  struct Piece {  // of one key: a lane's codes, and their block's d and m
-    Codes codes;
-    uint32_t dm;
-  };
+  typedef Q4Quarter<KS> Piece;  // of one key
   struct Shared : FewShared {
     union {
       uint32_t v[kWaves][NB][kBlock * kRow];
@@ -127,15 +122,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
     sh.place[wave][turn & 1][lane] = q4_bytes(kv_place(a.kv, ok ? page : 0, slot, head));
     __builtin_amdgcn_wave_barrier();
   };
-  // the lane's block of a row, and its codes there
-  const int block_at = (D == 128 ? grp : grp >> 1) * kQ4Bytes, codes_at = block_at + 4 + (D == 128 ? 0 : 8 * (grp & 1));
   Piece kreg[NB][2], vreg[NB][2];  // [block][key / 16]
   const auto load = [&](const uint16_t* pool, int turn, int n, Piece (&to)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* at = reinterpret_cast<const uint8_t*>(pool) + sh.place[wave][turn & 1][n * kBlock + 16 * i + col];
-      to[i].codes = *reinterpret_cast<const Codes_a4*>(at + codes_at);
-      to[i].dm = *reinterpret_cast<const uint32_t*>(at + block_at);
+      to[i] = q4_load_quarter<KS>(at, grp);
     }
   };
   // q as it lies in memory: of step s the dword's low halves' values, and its high halves'
@@ -144,12 +136,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
   Q4 q_low[KS], q_high[KS];
   if (wave < blocks) look_up(0);
   {
-    const Q* from_q = static_cast<const Q*>(a.q) + token * a.q_stride + static_cast<int64_t>(h) * D +
-                      (D == 128 ? 32 * grp : 32 * (grp >> 1) + 8 * (grp & 1));
+    const Q* from_q = static_cast<const Q*>(a.q) + token * a.q_stride + static_cast<int64_t>(h) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      q_low[s] = *reinterpret_cast<const Q4*>(from_q + 4 * s);
-      q_high[s] = *reinterpret_cast<const Q4*>(from_q + 4 * s + 16);
+      q_low[s] = *reinterpret_cast<const Q4*>(from_q + q4_quarter_value<KS>(grp, s));
+      q_high[s] = *reinterpret_cast<const Q4*>(from_q + q4_quarter_value<KS>(grp, s) + 16);
     }
   }
   if (wave < blocks) {
@@ -159,11 +150,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
     for (int n = 0; n < NB; ++n) load(a.kv.k, 0, n, kreg[n]);
   }
 
-  // q, in parts: eight values of step s in the order of a dword's unpacked codes, 0 2 16 18 1 3 17 19
+  // q, in parts: eight values of step s in the order of a dword's unpacked codes
   V8 q[KS][NP];
   float factor = a.scale * kLog2e;
   {
-    const auto in_order = [&](int s, int i) { return live ? (i & 2 ? q_high : q_low)[s][2 * (i & 1) + (i >> 2)] : static_cast<Q>(0.0f); };
+    const auto in_order = [&](int s, int i) { return live ? (i & 2 ? q_high : q_low)[s][q4_pair_value(i) & 15] : static_cast<Q>(0.0f); };
     if constexpr (Q32) {
       float most = 0.0f;
 #pragma unroll
@@ -264,11 +255,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
       for (int i = 0; i < 2; ++i) {
         const half2_q4 dm = __builtin_bit_cast(half2_q4, k[i].dm);
         const half2_q4 d = {dm.x, dm.x}, m = {dm.y, dm.y};
-        const uint32_t w = k[i].codes[s];
-        const half2_q4 k4[4] = {__builtin_elementwise_fma(q4_low(w, exponents), d, m),
-                                __builtin_elementwise_fma(q4_high(w, exponents), d, m),
-                                __builtin_elementwise_fma(q4_low(w >> 8, exponents), d, m),
-                                __builtin_elementwise_fma(q4_high(w >> 8, exponents), d, m)};
+        half2_q4 k4[4];
+        q4_pairs(k[i].codes[s], d, m, exponents, k4);
         const V8 key = __builtin_bit_cast(V8, k4);
 #pragma unroll
         for (int p = 0; p < NP; ++p) y[i] = N::mfma16(key, q[s][p], y[i]);
@@ -444,7 +432,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t* const to = sh.v[wave][n] + (16 * i + col) * kRow;
-        *reinterpret_cast<Codes*>(to + v_to) = vreg[n][i].codes;
+        *reinterpret_cast<typename Piece::Codes*>(to + v_to) = vreg[n][i].codes;
         to[v_dm] = vreg[n][i].dm;  // of D = 64 two lanes write the same
         const half2_q4 dm = __builtin_bit_cast(half2_q4, vreg[n][i].dm);
         zeros = __builtin_fmaf16(dm.y, 0.0f, zeros);  // values lie between m and 15 d + m

@@ -54,6 +54,42 @@ __device__ __forceinline__ half2_q4 q4_high(uint32_t two, const Q4Exponents& e) 
          half2_q4{static_cast<_Float16>(-64.0f), static_cast<_Float16>(-64.0f)};
 }
 
+// Eight values of a dword of codes as four pairs, of bytes 0 and 2 and then 1 and 3, low
+// halves first: values 0 2 16 18 1 3 17 19 from the dword's first on.
+__device__ __forceinline__ void q4_pairs(uint32_t codes, half2_q4 d, half2_q4 m, const Q4Exponents& e, half2_q4 (&out)[4]) {
+  out[0] = __builtin_elementwise_fma(q4_low(codes, e), d, m);
+  out[1] = __builtin_elementwise_fma(q4_high(codes, e), d, m);
+  out[2] = __builtin_elementwise_fma(q4_low(codes >> 8, e), d, m);
+  out[3] = __builtin_elementwise_fma(q4_high(codes >> 8, e), d, m);
+}
+// Where the i-th of those lies.
+__host__ __device__ constexpr int q4_pair_value(int i) { return 2 * (i & 1) + (i & 2 ? 16 : 0) + (i >> 2); }
+
+// A lane's share of a row that four lanes load: a quarter of its codes, KS = D / 32
+// dwords of one block, and that block's d and m.
+template <int KS>
+struct Q4Quarter {
+  typedef uint32_t Codes __attribute__((ext_vector_type(KS)));
+  Codes codes;
+  uint32_t dm;
+};
+template <int KS>
+__device__ __forceinline__ int q4_quarter_block(int quarter) {
+  return KS == 4 ? quarter : quarter >> 1;
+}
+template <int KS>
+__device__ __forceinline__ Q4Quarter<KS> q4_load_quarter(const uint8_t* row, int quarter) {
+  typedef typename Q4Quarter<KS>::Codes Codes_a4 __attribute__((aligned(4)));
+  const uint8_t* block = row + q4_quarter_block<KS>(quarter) * kQ4Bytes;
+  return {*reinterpret_cast<const Codes_a4*>(block + 4 + (KS == 4 ? 0 : 8 * (quarter & 1))),
+          *reinterpret_cast<const uint32_t*>(block)};
+}
+// Where the values of its dword s begin in the row.
+template <int KS>
+__device__ __forceinline__ int q4_quarter_value(int quarter, int s) {
+  return (KS == 4 ? 32 * quarter : 32 * (quarter >> 1) + 8 * (quarter & 1)) + 4 * s;
+}
+
 // Eight values of four bytes of codes: their low halves' to `low`, their high halves' to `high`.
 __device__ __forceinline__ void q4_values4(uint32_t codes, half2_q4 d, half2_q4 m, const Q4Exponents& e, uint32_t (&low)[2],
                                            uint32_t (&high)[2]) {

@@ -72,7 +72,7 @@ struct EvictArgs {
   int32_t width;  // the longest context that the workspace has room for
   // launch_kv_evict's part
   uint32_t* moves;  // [sequences x kv_heads]
-  uint32_t* ranks;  // [sequences x kv_heads x width]
+  uint32_t* ranks;  // [sequences x kv_heads x width, up to a multiple of 4]
   int32_t* lists;   // [sequences x kv_heads x 2 x half of width]: places, then sources
   int32_t move_parts, unit_values, unit_bytes;
 };

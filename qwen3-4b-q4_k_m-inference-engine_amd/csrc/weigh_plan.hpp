@@ -38,7 +38,7 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   p.row_parts = 1;
   if (p.few) {
     // a few workgroups for each compute unit; 128 keys are one block for each of four waves
-    int64_t parts = up(8 * kUnits, units);
+    int64_t parts = up(16 * kUnits, units);
     if (parts > up(max_context, 128)) parts = up(max_context, 128);
     p.part_keys = static_cast<int32_t>(up(up(max_context, parts), 128) * 128);
     p.key_parts = static_cast<int32_t>(up(max_context, p.part_keys));
