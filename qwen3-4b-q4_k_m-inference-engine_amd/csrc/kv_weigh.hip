@@ -83,13 +83,16 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
   __shared__ float factors[kWaves][16], logs[kWaves][16];
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // Workgroups go to the eight XCDs in turn: the heads of a unit to the same one where
-  // their rows share lines of memory (see paged_attention_few_q4.hip).
+  // Workgroups go to the eight XCDs in turn. Where there are many, the first parts of all
+  // contexts come first, as later ones are empty where contexts are short, and the
+  // heads of one whose Q4_1 rows share lines of memory go to the same XCD: 64 sequences
+  // of up to 8192 keys 75 us, a context and head at a time 85; 16 of them 36 and 26.
   const int heads = a.kv.kv_heads, block = static_cast<int>(blockIdx.x);
-  const bool shared = Q4 && a.kv.head_stride < a.kv.token_stride;
+  const bool many = a.kv.sequences * heads > static_cast<int>(weigh::kUnits);
+  const bool shared = Q4 && many && a.kv.head_stride < a.kv.token_stride;
   const int eight = block / (8 * heads), within = block - eight * 8 * heads, side = min(8, a.kv.sequences * a.key_parts - 8 * eight);
   const int head = shared ? within / side : block % heads, unit = shared ? 8 * eight + within - head * side : block / heads;
-  const int part = unit / a.kv.sequences, s = unit - part * a.kv.sequences;  // the last parts are empty where contexts are short
+  const int s = many ? unit % a.kv.sequences : unit / a.key_parts, part = many ? unit / a.kv.sequences : unit % a.key_parts;
   KvSequence seq;
   int keys;
   if (!weigh_keys(a, s, head == 0 && part == 0, seq, keys)) return;
