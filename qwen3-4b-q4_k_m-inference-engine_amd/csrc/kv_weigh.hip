@@ -276,7 +276,7 @@ __device__ __forceinline__ int q_chunk(int row, int chunk) {
 }
 
 template <int D, int KIND, bool Q32>
-__global__ __launch_bounds__(64 * kWaves, 2) void kv_weigh_many_kernel(const WeighArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 3) void kv_weigh_many_kernel(const WeighArgs a) {
   constexpr bool BF16 = KIND == QK_TYPE_BF16, Q4 = KIND == QK_TYPE_Q4_1;
   typedef Num<BF16> N;
   typedef typename N::V8 V8;
@@ -405,19 +405,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_weigh_many_kernel(const Wei
 #pragma unroll
           for (int g = 0; g < 2; ++g) x[g] = N::mfma32(q, k[g][i], x[g]);
         }
-      const bool whole = tile * kTileRows >= (key0 + kKeysAWave - 1 - seq.first) * a.group;
+      const auto add = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {  // registers 4 r4 .. hold rows 8 r4 + 4 half ..
-        const f32x4 factor = *reinterpret_cast<const f32x4*>(&factors[buffer][8 * r4 + 4 * half]);
-        const f32x4 log2_sum = *reinterpret_cast<const f32x4*>(&logs[buffer][8 * r4 + 4 * half]);
+        for (int r4 = 0; r4 < 4; ++r4) {  // registers 4 r4 .. hold rows 8 r4 + 4 half ..
+          const f32x4 factor = *reinterpret_cast<const f32x4*>(&factors[buffer][8 * r4 + 4 * half]);
+          const f32x4 log2_sum = *reinterpret_cast<const f32x4*>(&logs[buffer][8 * r4 + 4 * half]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float w = weight_of(x[g][4 * r4 + r], factor[r], log2_sum[r]);
-            sum[g] += whole || tile * kTileRows + 8 * r4 + 4 * half + r >= least_row[g] ? w : 0.0f;
-          }
-      }
+            for (int r = 0; r < 4; ++r) {
+              const float w = weight_of(x[g][4 * r4 + r], factor[r], log2_sum[r]);
+              const bool seen = !decltype(masked)::value || tile * kTileRows + 8 * r4 + 4 * half + r >= least_row[g];
+              sum[g] += seen ? w : 0.0f;
+            }
+        }
+      };
+      // does every row of the tile see every key of the wave?
+      if (tile * kTileRows >= (key0 + kKeysAWave - 1 - seq.first) * a.group)
+        add(std::false_type{});
+      else
+        add(std::true_type{});
     }
   }
 #pragma unroll

@@ -47,7 +47,7 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   p.part_keys = kHeldKeys;
   p.key_parts = static_cast<int32_t>(up(max_context, kHeldKeys));
   // Rows are shared out where keys alone do not occupy the card, eight tiles of 32 rows at least.
-  int64_t parts = up(4 * kUnits, units * p.key_parts);
+  int64_t parts = up(8 * kUnits, units * p.key_parts);
   const int64_t most = up(rows, 256 * sequences), each = units * p.key_parts * kHeldKeys * static_cast<int64_t>(sizeof(float));
   if (parts > most) parts = most;
   if (parts * each > kMostBytes) parts = kMostBytes / each;
