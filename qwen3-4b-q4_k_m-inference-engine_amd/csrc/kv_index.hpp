@@ -94,6 +94,23 @@ QK_HD int32_t kv_page(const KvArgs& a, int s, int32_t entry) {
   return ok && page >= 0 && page < a.pages ? page : -1;
 }
 
+// key / page_size of keys below 2^30 as the high half of a product: with 2^l the least
+// power of two that page_size does not exceed, ceil(2^(30 + l) / page_size) is below 2^31
+// and gives the quotient in its bits from 30 + l on; doubled, from 31 + l on.
+struct PageDivision {
+  uint32_t factor;
+  int32_t shift;  // below the high half; -1: pages of one token
+};
+QK_HD PageDivision page_division(int32_t page_size) {
+  int bits = 0;
+  while ((int64_t{1} << bits) < page_size) ++bits;
+  return {static_cast<uint32_t>(2 * (((uint64_t{1} << (30 + bits)) + page_size - 1) / page_size)), bits - 1};
+}
+QK_HD int32_t page_entry(const PageDivision& d, int32_t key) {
+  const uint32_t high = static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(key)) * d.factor >> 32);
+  return d.shift < 0 ? key : static_cast<int32_t>(high >> d.shift);
+}
+
 // Element offset of (page, slot, head); page in [0, pages), slot in [0, page_size).
 QK_HD int64_t kv_place(const KvArgs& a, int32_t page, int32_t slot, int32_t head) {
   return page * a.page_stride + static_cast<int64_t>(slot) * a.token_stride + static_cast<int64_t>(head) * a.head_stride;

@@ -9,11 +9,7 @@ hipError_t launch_paged_attention(AttentionArgs a, const AttentionPlan& plan, in
   a.splits = plan.splits;
   a.fill = plan.fill;
   a.pairs = plan.pairs;
-  // of l bits of page_size - 1: ceil(2^(30 + l) / page_size), which is below 2^31, doubled
-  int bits = 0;
-  while (int64_t{1} << bits < a.kv.page_size) ++bits;
-  a.page_factor = static_cast<uint32_t>(2 * (((uint64_t{1} << (30 + bits)) + a.kv.page_size - 1) / a.kv.page_size));
-  a.page_shift = bits - 1;
+  a.pages = page_division(a.kv.page_size);
   char* ws = static_cast<char*>(workspace);
   a.arrived = reinterpret_cast<uint32_t*>(ws);
   a.sums = reinterpret_cast<float*>(ws + plan.sums_at);

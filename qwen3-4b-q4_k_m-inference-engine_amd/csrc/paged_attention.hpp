@@ -142,13 +142,6 @@ __device__ __forceinline__ float swap32_max(float v) {
   return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
-// Which entry of its page table a key lies in, key / page_size, for keys below 2^30:
-// the high half of a product with page_factor (launch_paged_attention).
-__device__ __forceinline__ int page_entry(const AttentionArgs& a, int key) {
-  const uint32_t high = __umulhi(static_cast<uint32_t>(key), a.page_factor);
-  return a.kv.page_size == 1 ? key : static_cast<int>(high >> a.page_shift);
-}
-
 // Sequence by sequence, ceil(rows / tile_rows) tiles each: wave-parallel running
 // sums of the tile counts until they pass `tile`. Where `report`, lengths that do
 // not fit are reported, of all sequences: one without rows has no tile.

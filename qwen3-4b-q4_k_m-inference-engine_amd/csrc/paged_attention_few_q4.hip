@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
     return key < c.hi ? key : c.hi - 1;
   };
   const auto look_up = [&](int turn) {
-    entry = page_entry(a, key_of(turn));
+    entry = page_entry(a.pages, key_of(turn));
     page = a.kv.page_table[kv_table_at(a.kv, t.s, entry, listed)];
   };
   const auto settle = [&](int turn) {  // page ids -> places

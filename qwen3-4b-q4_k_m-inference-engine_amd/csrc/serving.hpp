@@ -92,8 +92,7 @@ struct AttentionArgs {
   float* lse;
   // the plan's part (launch_paged_attention)
   int32_t tiles, splits, fill;
-  uint32_t page_factor;  // for page_entry
-  int32_t page_shift;
+  PageDivision pages;
   int32_t pairs;      // tiles of a round of workgroups, one a compute unit, if sequences are taken by length; else 0
   uint32_t* arrived;  // [tiles x kv_heads], zero between calls
   float* sums;        // [tiles x kv_heads x splits x rows] (maximum, sum) pairs
