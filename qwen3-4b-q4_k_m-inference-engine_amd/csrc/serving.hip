@@ -299,7 +299,8 @@ int qk_kv_evict(const qk_kv_cache* cache, const qk_kv_batch* batch, const int32_
   if (!keep || !recent || !context_out) return refuse("evict pointers must be non-null");
   if (misaligned(keep, 4) || misaligned(recent, 4) || misaligned(context_out, 4) || misaligned(seen, 4))
     return refuse("evict arrays must be 4-byte aligned");
-  if (context_out == batch->context) return refuse("evict context_out must not be the batch's context");
+  if (context_out == batch->context || context_out == keep || context_out == recent || context_out == seen)
+    return refuse("evict context_out must be an array of its own");
   status = check_workspace(workspace, workspace_bytes, qk::evict_workspace(batch->sequences, cache->kv_heads, max_context));
   if (status != QK_OK) return status;
   qk::EvictArgs a{};

@@ -125,6 +125,15 @@ def test_evict_refusals(qk):
     assert size(wide, batch(qk, sequences=65535), 1000) == 0
 
 
+@pytest.mark.parametrize("name", ["seen", "keep", "recent"])
+def test_evict_writes_lengths_beside_what_it_reads(qk, name):
+    """Other workgroups still read those arrays when the first lengths are written."""
+    arrays = {"seen": 4 * P, "keep": 5 * P, "recent": 6 * P}
+    status = qk.load().qk_kv_evict(cache(qk), batch(qk), arrays["seen"], weights(qk), arrays["keep"], arrays["recent"], 100,
+                                   arrays[name], P, 1 << 40, None)
+    assert status == INVALID and b"own" in qk.load().qk_last_error()
+
+
 def test_the_weights_structure_matches_the_header(qk, tmp_path):
     lines = [f"_Static_assert(sizeof(qk_kv_weights) == {ctypes.sizeof(qk.KVWeights)}, \"size\");"]
     for field, _ in qk.KVWeights._fields_:
