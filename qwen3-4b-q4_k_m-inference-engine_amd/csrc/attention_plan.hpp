@@ -66,7 +66,11 @@ constexpr int64_t kOrderedKeys = 1024;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
-// Over Q4_1 blocks.
+// Over Q4_1 blocks contexts are cut into even shares of all keys, four workgroups a
+// compute unit, which hide one another's starts, and parts of 256 keys, two turns of
+// four waves, at least (us). Half as many workgroups: 32 sequences of up to 8192 keys 95
+// and 109, three of up to 131072 83 to 86 and 93, but 16 of up to 8192 54 and 50.
+// Parts of 512 keys: one sequence of 1000 16 and 17, of 2000 18.2 and 20.8, of 4096 15.6 and 17.6.
 constexpr int kLeastPartQ4 = 256, kSlotsQ4 = 1024;
 constexpr size_t kCounterBytes = kMostUnits * sizeof(uint32_t);
 
@@ -152,7 +156,9 @@ inline AttentionPlan plan_attention(int64_t tokens, int64_t sequences, int64_t q
     ManyRows{rows, tokens, sequences, kv_heads, group, window, max_context, waves_rows, head_dim,
              q_type == QK_TYPE_F32 ? (type == QK_TYPE_BF16 ? 3 : 2) : 1}
         .choose(p.key_groups, splits);
-  // over Q4_1 blocks a tile of few rows leaves the matrix core's other columns to other keys
+  // Over Q4_1 blocks a tile of up to 8 rows leaves the matrix core's other columns to
+  // other keys (us; single tokens of 32 heads over 8: one over 131072 77, in 16 rows 82, over 4096
+  // 15.6 and 18.0; 16 over up to 8192 53.7 and 56.3; 64, where memory bounds it, 114 and 115).
   const int few_rows = type != QK_TYPE_Q4_1 || rows > 8 * sequences ? 16 : 8;
   const int tile_rows = p.few ? few_rows : waves_rows / p.key_groups;
   p.rows = tile_rows;

@@ -3,11 +3,14 @@
 // budget move into the places that the others leave before it. Attention does not ask
 // for an order of keys that were rotated when they were stored.
 //
-// Three launches: every token's rank as 32 bits; of each (sequence, head) the rank that
+// Launches: every token's rank as 32 bits; of each (sequence, head) the rank that
 // the budget ends at, by a search digit by digit in one workgroup, and the list of
 // moves, in the order of the slots; the moves. Sources lie past the budget and
-// places before it, so moves do not meet. Moving bounds it, and for few long
-// sequences the search, which one compute unit does for each head.
+// places before it, so moves do not meet. The search bounds it, which one compute unit
+// does for each head: loads of ranks and dependent steps through LDS counters, of which
+// there are copies, since the ranks of like weights fall together. 32 sequences of up to 2304
+// cut to 2048: ranks 6 us, search 18, moves 8 (8 heads of 128, F16); one of 65536 cut to
+// 8192 in Q4_1: 8, 54 and 9.
 #include "q4_1.hpp"
 #include "qk_device.hpp"
 #include "qk_launch.hpp"

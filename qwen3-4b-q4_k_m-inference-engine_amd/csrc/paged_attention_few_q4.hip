@@ -1,9 +1,9 @@
 // Paged attention for few rows a sequence over Q4_1 blocks: a third of an F16
 // cache's bytes, and the unpacking that comes with them.
 //
-// As in paged_attention_few.hip the waves of a workgroup, eight here, share nothing while
-// they run and take blocks of 32 keys in turn. Codes stay packed up to the registers
-// that the matrix cores read:
+// As in paged_attention_few.hip the four waves of a workgroup share nothing while
+// they run and take blocks of 32 keys in turn, here two a turn. Codes stay packed up to
+// the registers that the matrix cores read:
 // - A key's row goes straight into the lanes that need it. Lane (key, grp) of the A
 //   operand takes the grp-th quarter of the row, so that the 20 bytes it loads are one
 //   block of 32 values (D = 128; half a block at D = 64) with its d and m, and step s of
@@ -17,7 +17,19 @@
 //   lie in different banks.
 // A value is one packed fma of an exact code: the F16 number that the block stands
 // for, so all of the F16 kernel's arithmetic holds as it is there.
-// Loads are issued two blocks ahead, page ids four.
+// Rows of K and page ids are loaded a turn ahead, V's at the turn's start, under the
+// products of q.k. No load is marked as not used again: where a token's heads lie side
+// by side a head's 80 bytes are part of a line whose rest another workgroup reads (64
+// tokens over up to 8192: 327 us so marked, 205 without). For the same reason the heads of
+// a tile run in the same XCD where contexts are whole.
+// What a rare row needs (a score that is no number, weights below what fp16 holds)
+// is in careful(), which fetches its operands again: kept in registers for it they
+// spill. Registers, not waves, are short: 4 waves of up to 256.
+//
+// 64 tokens over up to 8192: 112 us, of that the F16 cache takes 175; codes unpacked
+// into LDS first took 190. Three over up to 131072 (F16 q): 83 to 87, and 156. The kernel then
+// reads 3 TB/s, 5 in the middle of long parts: 320 to 410 vector operations a block of 32
+// keys, the unpacking's among them, take as long as its 5 KB from HBM.
 #include <type_traits>
 
 #include "paged_attention_few.hpp"

@@ -37,7 +37,10 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   p.few = rows <= 64 * sequences;
   p.row_parts = 1;
   if (p.few) {
-    // a few workgroups for each compute unit; 128 keys are one block for each of four waves
+    // Sixteen workgroups for each compute unit, eight of which run at once: contexts are
+  // uneven (us: 64 sequences of up to 8192 keys 75, by a quarter as many workgroups
+  // 100; but 8 such sequences 22 and 19, one of 32768 20 and 17.5). 128 keys are one block for
+  // each of four waves.
     int64_t parts = up(16 * kUnits, units);
     if (parts > up(max_context, 128)) parts = up(max_context, 128);
     p.part_keys = static_cast<int32_t>(up(up(max_context, parts), 128) * 128);
@@ -46,7 +49,10 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   }
   p.part_keys = kHeldKeys;
   p.key_parts = static_cast<int32_t>(up(max_context, kHeldKeys));
-  // Rows are shared out where keys alone do not occupy the card, eight tiles of 32 rows at least.
+  // Rows are shared out where keys alone do not occupy the card, eight tiles of 32 rows
+  // at least. A prompt has few blocks of keys, and the first ones are seen by the most rows
+  // (us: two prompts of up to 2047, 28 heads over 4: 43 to 49, undivided 532). Where keys
+  // are many, rows stay whole (63 new tokens over 32768: 1024 workgroups, 49 to 57).
   int64_t parts = up(8 * kUnits, units * p.key_parts);
   const int64_t most = up(rows, 256 * sequences), each = units * p.key_parts * kHeldKeys * static_cast<int64_t>(sizeof(float));
   if (parts > most) parts = most;
