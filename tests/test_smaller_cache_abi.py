@@ -6,6 +6,8 @@ import ctypes
 import pathlib
 import subprocess
 
+import pytest
+
 from test_serving_abi import (BAD_BATCHES, BAD_CACHES, INVALID, P, UNSUPPORTED, _sanitized, batch, cache, rope)
 
 ROOT = pathlib.Path(__file__).resolve().parents[1]
