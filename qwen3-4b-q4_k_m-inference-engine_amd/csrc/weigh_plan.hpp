@@ -37,11 +37,12 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   p.few = rows <= 64 * sequences;
   p.row_parts = 1;
   if (p.few) {
-    // Sixteen workgroups for each compute unit, eight of which run at once: contexts are
-  // uneven (us: 64 sequences of up to 8192 keys 75, by a quarter as many workgroups
-  // 100; but 8 such sequences 22 and 19, one of 32768 20 and 17.5). 128 keys are one block for
-  // each of four waves.
-    int64_t parts = up(16 * kUnits, units);
+    // Sixteen workgroups for each compute unit where contexts are many and uneven (us:
+    // 64 sequences of up to 8192 keys and 8 heads in Q4_1 75, by four each 100; 32 of them 46 and 52, in
+    // F16 76 and 90). Four each for few, where a start costs more than it balances (8 of
+    // 8192 22 by sixteen and 19, in F16 27 and 21; one of 131072 43 and 38.5). 128 keys are one block
+    // for each of four waves.
+    int64_t parts = up((units > kUnits / 4 ? 16 : 4) * kUnits, units);
     if (parts > up(max_context, 128)) parts = up(max_context, 128);
     p.part_keys = static_cast<int32_t>(up(up(max_context, parts), 128) * 128);
     p.key_parts = static_cast<int32_t>(up(max_context, p.part_keys));
