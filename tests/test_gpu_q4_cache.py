@@ -409,3 +409,13 @@ def test_a_page_far_into_a_large_pool(gpu):
         assert np.array_equal(out.download(np.uint16).reshape(2, H, D), p.rows(0, pool)[-2:])
     for b in big.values():
         b.free()
+
+
+@pytest.mark.parametrize("bound", [0, 1, 300, 1 << 62])
+@pytest.mark.parametrize("q_type", Q_TYPES)
+def test_contexts_beyond_the_bound(gpu, bound, q_type):
+    """max_context shares the work out; results do not depend on it."""
+    for new, contexts, window in (([1], [2500], 0), ([1, 1, 1], [3000, 40, 1300], 0), ([2, 5], [1500, 700], 600)):
+        print(f"[case] attention q4_1 bound={bound} {q_type} {contexts} window={window}", flush=True)
+        p = Paged4(new, contexts, kv_heads=2, dim=128, seed=len(contexts))
+        attend(gpu, p, 8, q_type=Q_TYPES[q_type], max_context=bound, window=window)
