@@ -298,9 +298,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const half2_q4 dm = __builtin_bit_cast(half2_q4, sh.v[wave][n][(16 * i + col) * kRow + v_dm]);
-        const float low = fabsf(static_cast<float>(dm.y));
-        const float high = fabsf(static_cast<float>(__builtin_fmaf16(static_cast<_Float16>(15.0f), dm.x, dm.y)));
-        most = fmaxf(most, fmaxf(low < __builtin_inff() ? low : 0.0f, high < __builtin_inff() ? high : 0.0f));
+        const float d = fabsf(static_cast<float>(dm.x)), low = fabsf(static_cast<float>(dm.y));
+        // in fp32: where code 15 leaves F16, lower codes may stand for any value of it
+        const float high = fminf(fabsf(__builtin_fmaf(15.0f, static_cast<float>(dm.x), static_cast<float>(dm.y))), 65504.0f);
+        const bool any = d < __builtin_inff() && low < __builtin_inff();  // else no value of the block is finite
+        most = fmaxf(most, any ? fmaxf(low, high) : 0.0f);
       }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off));

@@ -336,6 +336,34 @@ def test_weights_beside_much_larger_ones_keep_their_precision(gpu, q_type):
         a.check()
 
 
+@pytest.mark.parametrize("q_type", Q_TYPES)
+def test_weights_keep_their_precision_over_blocks_whose_largest_code_leaves_f16(gpu, q_type):
+    """The same where the other tokens' blocks are not the append's: code 15, which none of them
+    holds, would stand for an infinity, and what they do hold is near F16's largest value."""
+    for new, contexts in (([1, 1], [1000, 333]), ([3, 2], [400, 90]), ([40], [700])):
+        for dim in (64, 128):
+            print(f"[case] attention q4_1 large blocks {contexts} {q_type} dim={dim}", flush=True)
+            p = Paged4(new, contexts, dim=dim, seed=7)
+            blocks = p.v4.reshape(-1, 20)
+            blocks[:, 4:] = p.rng.integers(0, 11, (len(blocks), 16)) | p.rng.integers(0, 11, (len(blocks), 16)) << 4
+            d = np.where(p.rng.random(len(blocks)) < 0.5, 6000.0, -6000.0).astype(np.float16)
+            blocks[:, :4] = np.stack([d, np.zeros_like(d)], -1).view(np.uint8)
+            a = Attend(gpu, p, 4, q_type=Q_TYPES[q_type])
+            for s in range(len(new)):
+                p.seen(p.v4)[p.table[s, 0], 0] = 0
+                q = ref.decode(a.q, a.q_type)[p.start[s], :4 * dim].reshape(4, dim)
+                for h in range(2):  # a key along the first of the head's queries, 25 nats ahead
+                    k = q[2 * h] / (q[2 * h] @ q[2 * h]) * 25.0 / abs(float(a.scale))
+                    p.seen(p.k4)[p.table[s, 0], 0, h] = q4_ref.blocks_of(k.astype(np.float32)[None])[0]
+            p.settle()
+            assert np.isfinite(ref.decode(p.v, F16)).all()
+            p.dev["k"].upload(p.k4)
+            p.dev["v"].upload(p.v4)
+            a.call()
+            gpu.synchronize()
+            a.check()
+
+
 def test_bad_pages_are_reported_and_reach_no_other_sequence(gpu):
     for new, contexts in (([1, 1, 1], [40, 40, 40]), ([30, 30, 30], [40, 40, 40])):
         p = Paged4(new, contexts, page=8, dim=128, seed=16)
