@@ -459,7 +459,8 @@ size_t qk_kv_weigh_workspace_size(const qk_kv_cache *cache, const qk_kv_batch *b
  * keep[s] stays where it is; the i-th one past it moves, with its key, value, weight
  * and position, to the i-th slot that is left. Slots from keep[s] on then hold nothing
  * of the sequence (their pages may serve others). context_out[s] (device, an
- * array of its own, so that every layer's cache can be cut by the same lengths)
+ * array of its own, refused where it shares an entry with context, keep, recent, seen or
+ * page_table, so that every layer's cache can be cut by the same lengths)
  * receives min(context, keep), or the context where nothing was cut.
  * Later steps pass context_out as context and count `seen` on; attention sees kept
  * tokens as it did, as long as it has no window (which would count slots).

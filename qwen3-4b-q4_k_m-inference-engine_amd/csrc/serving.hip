@@ -78,6 +78,12 @@ int check_workspace(const void* workspace, size_t bytes, size_t need) {
   return QK_OK;
 }
 
+// Whether `n` and `m` 32-bit entries from a and b on share any.
+bool overlap(const int32_t* a, uint64_t n, const int32_t* b, uint64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && (x < y ? y - x < 4 * n : x - y < 4 * m);
+}
+
 // Slots that a list and a grid hold.
 bool evict_fits(const qk_kv_cache* c, const qk_kv_batch* b, int64_t max_context) {
   const int64_t units = b->sequences * c->kv_heads;
@@ -299,7 +305,11 @@ int qk_kv_evict(const qk_kv_cache* cache, const qk_kv_batch* batch, const int32_
   if (!keep || !recent || !context_out) return refuse("evict pointers must be non-null");
   if (misaligned(keep, 4) || misaligned(recent, 4) || misaligned(context_out, 4) || misaligned(seen, 4))
     return refuse("evict arrays must be 4-byte aligned");
-  if (context_out == batch->context || context_out == keep || context_out == recent || context_out == seen)
+  // workgroups of other heads still read those when the first lengths are written
+  const uint64_t n = static_cast<uint64_t>(batch->sequences), stride = static_cast<uint64_t>(batch->table_stride);
+  const uint64_t table = stride < (uint64_t{1} << 40) ? n * stride : n << 40;  // no address space holds more
+  if (overlap(context_out, n, batch->context, n) || overlap(context_out, n, keep, n) || overlap(context_out, n, recent, n) ||
+      overlap(context_out, n, seen, n) || overlap(context_out, n, batch->page_table, table))
     return refuse("evict context_out must be an array of its own");
   status = check_workspace(workspace, workspace_bytes, qk::evict_workspace(batch->sequences, cache->kv_heads, max_context));
   if (status != QK_OK) return status;

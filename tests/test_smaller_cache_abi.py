@@ -136,6 +136,34 @@ def test_evict_writes_lengths_beside_what_it_reads(qk, name):
     assert status == INVALID and b"own" in qk.load().qk_last_error()
 
 
+@pytest.mark.parametrize("name,entries", [("context", 9), ("seen", 9), ("keep", 9), ("recent", 9), ("page_table", 9 * 4)])
+def test_evict_lengths_may_not_overlap_what_it_reads(qk, name, entries):
+    """Not by one entry at either end; side by side they may lie (and the workspace is looked at then)."""
+    arrays = {"context": 3 * P, "seen": 4 * P, "keep": 5 * P, "recent": 6 * P, "page_table": 7 * P}
+    b = batch(qk, sequences=9, context=arrays["context"], page_table=arrays["page_table"], table_stride=4)
+
+    def call(out):
+        status = qk.load().qk_kv_evict(cache(qk), b, arrays["seen"], weights(qk), arrays["keep"], arrays["recent"], 100, out,
+                                       P, 0, None)
+        return status, qk.load().qk_last_error()
+
+    for out in (arrays[name], arrays[name] + 4, arrays[name] - 4, arrays[name] + 4 * (entries - 1), arrays[name] - 4 * 8):
+        status, message = call(out)
+        assert status == INVALID and b"own" in message, (out - arrays[name], message)
+    for out in (arrays[name] + 4 * entries, arrays[name] - 4 * 9):
+        status, message = call(out)
+        assert status == INVALID and b"small" in message, (out - arrays[name], message)
+
+
+def test_evict_lengths_beside_tables_of_any_stride(qk):
+    """Rows of a table that lie further apart than addresses reach overlap nothing before them."""
+    for stride in (1 << 40, (1 << 63) - 1):
+        b = batch(qk, sequences=65535, context=1 << 30, page_table=1 << 40, table_stride=stride)
+        for out, word in ((1 << 31, b"small"), ((1 << 40) + 8, b"own"), ((1 << 40) + (1 << 20), b"own")):
+            status = qk.load().qk_kv_evict(cache(qk), b, None, weights(qk), 1 << 29, 1 << 28, 100, out, P, 0, None)
+            assert status == INVALID and word in qk.load().qk_last_error(), (stride, out)
+
+
 def test_the_weights_structure_matches_the_header(qk, tmp_path):
     lines = [f"_Static_assert(sizeof(qk_kv_weights) == {ctypes.sizeof(qk.KVWeights)}, \"size\");"]
     for field, _ in qk.KVWeights._fields_:
