@@ -421,8 +421,12 @@ size_t qk_paged_attention_workspace_size(const qk_kv_cache *cache, const qk_kv_b
 
 /* What an eviction goes by, of every slot of a cache and key/value head: weight is
  * the attention weight that its token has gathered, position the token's own (both
- * device, [pages x kv_heads x page_size], a page's and head's slots side by side). No
- * value in them needs to be set before qk_kv_weigh has met the token. */
+ * device, [pages x kv_heads x page_size], a page's and head's slots side by side). The
+ * qk_kv_weigh call that has a token among its new ones begins its slots, whatever they
+ * held before. Those of a token that no call has among its new ones (where only the last
+ * rows of a prompt are weighed) the caller begins, before they are weighed or cut: by
+ * weight 0 and its position for every head, or by a call on all of the prompt's rows with
+ * -inf as the lse of those that are not to count. */
 typedef struct qk_kv_weights {
     float *weight;
     int32_t *position;

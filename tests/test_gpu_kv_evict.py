@@ -409,6 +409,42 @@ def test_sequences_that_cannot_be_cut_stay_and_are_reported(gpu):
     e.check((*want[:3], [40, 200, 40], want[4]))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_prompt_of_which_only_the_last_rows_count(gpu, kind):
+    """Slots begin with the call whose new tokens they hold: with -inf for the other rows' logs all of a prompt's
+    do, whatever they held, and an eviction goes by what its last rows looked at."""
+    for n, count in ((300, 20), (14, 3)):
+        print(f"[case] weigh last rows of {n} {kind}", flush=True)
+        p = make(kind, [n], [n], dim=64, page=24, seed=43)
+        w = Weigh(gpu, p, 4)
+        lse = w.lse.copy()
+        lse[:n - count] = -np.inf
+        w.lsed.upload(lse)
+        p.dev["weight"].upload(np.full(p.weight.shape, np.nan, np.float32))
+        p.dev["position"].upload(np.full(p.position.shape, 1 << 30, np.int32))
+        w.call()
+        gpu.synchronize()
+        weight, position = w.got()
+        pg, sl = slots(p, 0, n)
+        assert (position[pg, :, sl] == np.arange(n)[:, None]).all()
+        q, K = ref.decode(w.q, F32), ref.decode(p.rows(0, p.k), p.kind)
+        want, off = np.zeros((n, 2)), np.zeros((n, 2))
+        for h in range(4):
+            qh, l = q[n - count:, h * 64:(h + 1) * 64], lse[n - count:, h].astype(np.float64)[:, None]
+            reach = float(w.scale) * (np.abs(qh) @ np.abs(K[:, h // 2]).T)
+            g = np.where(np.arange(n) <= np.arange(n - count, n)[:, None], np.exp(float(w.scale) * (qh @ K[:, h // 2].T) - l), 0)
+            want[:, h // 2] += g.sum(0)
+            off[:, h // 2] += (g * ((64 / 4 + 8) * reach + 5 * np.abs(l) + 6) * U).sum(0) + (count + 41) * U * g.sum(0)
+        assert (np.abs(weight[pg, :, sl] - want) <= off).all()
+        e = Evict(gpu, p, [n // 2], [2])
+        e.p.weight, e.p.position = np.nan_to_num(weight), position
+        p.dev["weight"].upload(e.p.weight)
+        p.dev["position"].upload(e.p.position)
+        e.call()
+        gpu.synchronize()
+        e.check()
+
+
 def test_captured_weighing_and_eviction(gpu):
     """One captured pair of calls, replayed on changed lengths with eager work in between."""
     p = Paged4([1, 1], [150, 700], dim=128, seed=8)
