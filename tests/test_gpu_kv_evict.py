@@ -242,6 +242,79 @@ def test_weights_of_bad_pages_and_lengths(gpu):
     assert np.array_equal(w.got()[0], p.weight)
 
 
+@pytest.mark.parametrize("head_major", [False, True])
+@pytest.mark.parametrize("kind", ["q4_1", "f16"])
+def test_weights_of_many_contexts(gpu, kind, head_major):
+    """More (context, head) units than compute units, and parts of contexts that eight do not divide."""
+    print(f"[case] weigh many contexts {kind} head_major={head_major}", flush=True)
+    rng = np.random.default_rng(31)
+    new = [0 if i % 11 == 5 else 3 if i % 7 == 2 else 1 for i in range(35)]
+    contexts = [max(int(c), n) for c, n in zip(rng.integers(1, 701, 35), new)]
+    contexts[20] = 700
+    p = make(kind, new, contexts, kv_heads=9, dim=64, page=24, head_major=head_major, seed=32, gaps=(2, 1))
+    w = Weigh(gpu, p, 18, seen=[c + 5 * s for s, c in enumerate(contexts)])
+    w.call()
+    gpu.synchronize()
+    w.check()
+    assert p.fault() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_weights_of_a_chunk_beside_single_tokens(gpu, kind):
+    """A sequence of many rows among ones of few, in the kernel for few: its rows' tiles add to a weight one
+    after another, each with a rounding of its own (the others have one tile, as the class says of all)."""
+    print(f"[case] weigh chunk beside tokens {kind}", flush=True)
+    rng = np.random.default_rng(33)
+    new, chunk, G = [1] * 20, 170, 4
+    contexts = [int(c) for c in rng.integers(1, 300, 20)]
+    new.insert(7, chunk)
+    contexts.insert(7, 400)
+    p = make(kind, new, contexts, dim=128, seed=34)
+    w = Weigh(gpu, p, 2 * G)
+    pg, sl = slots(p, 7, 400)
+    w.off[pg, :, sl] += (chunk * G / 16) * U * np.abs(w.want[pg, :, sl])
+    w.call()
+    gpu.synchronize()
+    w.check()
+    assert p.fault() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_weights_of_contexts_shorter_than_their_new_tokens(gpu, kind):
+    """Reported, and no harm to other sequences or to slots past that context."""
+    for new, contexts, short in (([1, 5, 2], [40, 40, 30], 2), ([50, 50, 50], [60, 90, 75], 30)):
+        print(f"[case] weigh short context {new} {kind}", flush=True)
+        p = make(kind, new, contexts, page=8, dim=64, seed=35)
+        w = Weigh(gpu, p, 4)
+        lengths = np.asarray(contexts, np.int32)
+        lengths[1] = short
+        p.dev["context"].upload(lengths)
+        w.call()
+        gpu.synchronize()
+        assert p.fault() == gpu.KV_FAULT_LENGTH
+        weight, position = w.got()
+        pg, sl = slots(p, 1, contexts[1])
+        assert np.array_equal(weight[pg[short:], :, sl[short:]], p.weight[pg[short:], :, sl[short:]])
+        assert np.array_equal(position[pg[short:], :, sl[short:]], p.position[pg[short:], :, sl[short:]])
+        # new token i of n has position short - n + i: the slots before `short` are all of new tokens
+        assert (position[pg[:short], :, sl[:short]] == np.arange(short)[:, None]).all()
+        q, K = ref.decode(w.q, F32)[p.start[1]:p.start[2]], ref.decode(p.rows(1, p.k), p.kind)
+        got, want, off = (np.zeros((short, 2)) for _ in range(3))
+        got[:] = weight[pg[:short], :, sl[:short]]
+        at = np.arange(short - new[1], short)[:, None]
+        for h in range(4):
+            qh, k, lse = q[:, h * 64:(h + 1) * 64], K[:short, h // 2], w.lse[p.start[1]:p.start[2], h].astype(np.float64)[:, None]
+            x, reach = float(w.scale) * (qh @ k.T), float(w.scale) * (np.abs(qh) @ np.abs(k).T)
+            g = np.where(np.arange(short) <= at, np.exp(x - lse), 0)
+            want[:, h // 2] += g.sum(0)
+            off[:, h // 2] += (g * ((64 / 4 + 8) * reach + 5 * np.abs(lse) + 6) * U).sum(0) + (new[1] + 41) * U * g.sum(0)
+        assert (np.abs(got - want) <= off).all()
+        for x, y, e in ((weight, w.want, w.off), (position, w.want_position, 0)):
+            for s in (0, 2):
+                pg, sl = slots(p, s, contexts[s])
+                assert (np.abs(x[pg, :, sl] - y[pg, :, sl]) <= (e if np.isscalar(e) else e[pg, :, sl])).all()
+
+
 # ------------------------------------------------------------------- evict --
 
 def rank_key(weight):
@@ -407,6 +480,33 @@ def test_sequences_that_cannot_be_cut_stay_and_are_reported(gpu):
     gpu.synchronize()
     assert p.fault() == gpu.KV_FAULT_PAGE
     e.check((*want[:3], [40, 200, 40], want[4]))
+
+
+LONG = {"as-they-come": None, "all-alike": WEIGHTS["all-alike"], "ties": WEIGHTS["ties"]}
+
+
+@pytest.mark.parametrize("name", LONG)
+def test_evictions_of_long_contexts(gpu, name):
+    """Every loop over a head's slots takes several turns, and ties are counted on from one to the next."""
+    print(f"[case] evict long {name}", flush=True)
+    p = Paged([0, 0, 0], [40000, 16385, 70001], dim=64, page=256, kv_heads=2, seed=41)
+    e = Evict(gpu, p, [30000, 8000, 11], [500, 20, 3], weight=LONG[name])
+    e.call()
+    gpu.synchronize()
+    assert e.check() > 0
+    assert p.fault() == 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "q4_1"])
+def test_evictions_of_many_heads(gpu, kind):
+    """A few hundred (sequence, head) units, each of more moves than its workgroups take in a turn."""
+    print(f"[case] evict many heads {kind}", flush=True)
+    p = make(kind, [0] * 32, [1300 - 2 * s for s in range(32)], dim=64, page=64, kv_heads=8, seed=42)
+    e = Evict(gpu, p, [650] * 32, [40] * 32)
+    e.call()
+    gpu.synchronize()
+    assert e.check() > 32 * 8 * 256
+    assert p.fault() == 0
 
 
 @pytest.mark.parametrize("kind", KINDS)
