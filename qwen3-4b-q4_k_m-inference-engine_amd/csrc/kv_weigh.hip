@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64 * kWaves, KIND != QK_TYPE_Q4_1 && Q32 && D == 12
   constexpr int LPK = D / 8, KPL = 64 / LPK, NL = Q4 ? 2 : kBlock / KPL;  // lanes a key, keys a load, loads a block
   __shared__ __attribute__((aligned(16))) uint8_t k_lds[kWaves][Q4 ? 16 : kBlock * 2 * D];
   __shared__ int64_t place[kWaves][2][kBlock];
-  __shared__ float factors[kWaves][16], logs[kWaves][16];
+  __shared__ __attribute__((aligned(16))) float factors[kWaves][16], logs[kWaves][16];
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups go to the eight XCDs in turn. Where there are many, the first parts of all
