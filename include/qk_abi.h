@@ -443,7 +443,8 @@ typedef struct qk_kv_weights {
  * sums in an order that the arguments alone decide. A page may belong to one sequence
  * of the call only. Keys on a page that is none get nothing; a sequence longer than
  * max_context by as much as does not fit, or than its page table, is left alone (both
- * reported, see qk_kv_cache::fault).
+ * reported, see qk_kv_cache::fault). A chunk of a prompt among single tokens is right but
+ * slow: sequences of many new tokens and of few are better weighed in two calls.
  * workspace: qk_kv_weigh_workspace_size bytes, 256-byte aligned (NULL when that is 0),
  * whatever it holds; calls that may run concurrently need separate ones. Nothing is
  * allocated: the call can be captured. No counterpart in the reference. */
@@ -469,7 +470,7 @@ size_t qk_kv_weigh_workspace_size(const qk_kv_cache *cache, const qk_kv_batch *b
  * Later steps pass context_out as context and count `seen` on; attention sees kept
  * tokens as it did, as long as it has no window (which would count slots).
  * keep, recent, seen: device arrays of `sequences` (seen NULL: the contexts). The
- * batch's token_start and tokens are not looked at. A page may belong to one
+ * batch's token_start and tokens decide nothing, but are checked as in other calls. A page may belong to one
  * sequence of the call only. Sequences with a page that is none, or longer than
  * max_context or their page table, stay as they are and are reported (see
  * qk_kv_cache::fault).

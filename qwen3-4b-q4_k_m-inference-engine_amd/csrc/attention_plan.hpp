@@ -66,9 +66,11 @@ constexpr int64_t kOrderedKeys = 1024;
 // so the counters of every plan fit one fixed region at the workspace's start:
 // no call's parts lie where a call of another batch keeps its counters.
 constexpr int64_t kMostUnits = 2 * kUnits;
-// Over Q4_1 blocks contexts are cut into even shares of all keys, four workgroups a
-// compute unit, which hide one another's starts, and parts of 256 keys, two turns of
-// four waves, at least (us). Half as many workgroups: 32 sequences of up to 8192 keys 95
+// Over Q4_1 blocks the kernel cuts contexts into even shares of all keys, for two
+// workgroups a compute unit (its registers hold no more), parts of 256 keys, two turns of
+// four waves, at least. The plan's part is the grid, of four workgroups a compute unit: it
+// bounds into how many shares the longest contexts go; workgroups without one end at once
+// (us). A grid half as large: 32 sequences of up to 8192 keys 95
 // and 109, three of up to 131072 83 to 86 and 93, but 16 of up to 8192 54 and 50.
 // Parts of 512 keys: one sequence of 1000 16 and 17, of 2000 18.2 and 20.8, of 4096 15.6 and 17.6.
 constexpr int kLeastPartQ4 = 256, kSlotsQ4 = 1024;

@@ -18,9 +18,12 @@
 // values) a decode step: one token 2.7 us, 64 3.9.
 //
 // Q4_1 caches: a finished row goes through LDS, from where each lane takes four
-// values and the four 16 further on, the codes of one dword, four lanes a block. Norm and
-// rotation are formed in 64 bits there and rounded once, so that codes do not depend on
-// the order of a sum: 4096 tokens, 173 MB with the rotated q, 32 us (5.3 TB/s).
+// values and the four 16 further on, the codes of one dword, four lanes a block. The norm's
+// sum of squares and the sine and cosine are formed in 64 bits there and rounded once, so
+// that codes do not depend on the order of a sum; the inverse root, the scaling and the
+// rotation (products rounded each) are fp32. Of 4.2 million keys' codes two differ from
+// those of other fp32 steps, at borders between codes. 4096 tokens, 173 MB with the
+// rotated q: 32 us (5.3 TB/s).
 #include "q4_1.hpp"
 #include "qk_device.hpp"
 #include "qk_launch.hpp"

@@ -1,8 +1,10 @@
 // Cached rows of the new tokens out of their pages, as values: what a caller keeps
 // of a sequence elsewhere, hands to another cache, or compares. D/8 lanes a row, as in
 // the append; a workgroup takes one token and up to 16 (D = 128) or 32 (D = 64) of
-// its rows. Memory bounds it (8192 tokens of 2 x 8 heads of 128 out of Q4_1 blocks, 44 MB,
-// 13.7 us, 3.2 TB/s); a call of few tokens is the launch.
+// its rows. What bounds it is the way to a row, not memory: each workgroup searches its
+// token's sequence and looks up its page before the one load that a lane has in flight
+// (8192 tokens of 2 x 8 heads of 128 out of Q4_1 blocks, 44 MB, 13.7 us, 3.2 TB/s, where a
+// copy reaches 5.1). A call of few tokens is the launch.
 #include <type_traits>
 
 #include "q4_1.hpp"

@@ -9,15 +9,20 @@
 // a lane's registers and of four lanes. Q4_1 rows come straight from their codes, as in
 // paged_attention_few_q4.hip. One token over 1000 keys: 7.4 us, the call. 64 tokens
 // over up to 8192 in Q4_1: 74 us, 2.5 TB/s of keys and weights read and weights written;
-// unpacking and the exponentials bound it.
+// vector operations bound it, 270 a block of keys: unpacking, places (divisions by the
+// page's size), and eight exponentials, each behind a branch on its mask and taken for a
+// tile's rows that are none as well (12 of 16, with one token and four heads a group).
+// A workgroup takes its sequence's tiles of 16 rows one after another, keys anew for each:
+// a call lasts as long as that of a chunk among single tokens (weigh_plan.hpp).
 //
 // Many rows (a prompt's): each of four waves holds 64 keys in registers, as the
 // columns of 32x32x16 products, and all walk the same tiles of 32 rows, in LDS, split in
 // parts there and loaded a tile ahead. The exponentials and the conversion of F32 q, which
 // every workgroup does anew, bound it (105 of 245 vector operations a tile). Where keys are too few
 // to occupy the card the rows are shared out too, and a second launch adds up the parts.
-// 63 new tokens over 32768 keys in F16, F32 q: 49 to 57 us; two prompts of up to 2047 in BF16, 28
-// heads over 4: 43 to 49.
+// 63 new tokens over 32768 keys in F16, F32 q: 49 to 57 us. Two prompts of up to 2047 in BF16, 28
+// heads over 4: 43 to 49, of which exponentials and sums are 11 if spread over the card; there
+// each of 1856 workgroups gathers 256 keys for 14 tiles at most, uneven numbers of them.
 //
 // F32 q and 16-bit keys meet as in the attention: two fp16 parts of q (22 bits, after
 // scaling each row by a power of two) or three bf16 ones.

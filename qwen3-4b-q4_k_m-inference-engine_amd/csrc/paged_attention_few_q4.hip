@@ -28,8 +28,10 @@
 //
 // 64 tokens over up to 8192: 112 us, of that the F16 cache takes 175; codes unpacked
 // into LDS first took 190. Three over up to 131072 (F16 q): 83 to 87, and 156. The kernel then
-// reads 3 TB/s, 5 in the middle of long parts: 320 to 410 vector operations a block of 32
-// keys, the unpacking's among them, take as long as its 5 KB from HBM.
+// reads 3 TB/s, 5 in the middle of long parts. Its 320 to 410 vector operations a block of 32
+// keys, a third of them the unpacking, are 45 of the 112 us if spread over the whole card, its
+// bytes 65 at a copy's rate: with two waves a SIMD it reaches neither, with one of them alone
+// where a compute unit's shorter context has ended.
 #include <type_traits>
 
 #include "paged_attention_few.hpp"
@@ -241,7 +243,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_few_q4_kernel(const 
     }
     return v;
   };
-  // w: the weights of the block's group, and of others, that do not count
   // w: the weights of the block's group, and of others, that do not count. FINITE: all
   // values are; else those that are not go in as zeros (0 times them is none, and a
   // weight's parts may be of either sign).

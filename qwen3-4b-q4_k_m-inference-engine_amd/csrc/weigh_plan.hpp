@@ -34,6 +34,10 @@ inline WeighPlan plan_weigh(int64_t tokens, int64_t sequences, int64_t q_heads, 
   if (tokens == 0 || sequences == 0) return p;
   max_context = max_context < 1 ? 1 : max_context < kMostPositions ? max_context : int64_t{kMostPositions};
   const int64_t rows = tokens * (q_heads / kv_heads), units = sequences * kv_heads;
+  // By the mean, as lengths are on the device. One sequence of many rows among ones of
+  // few takes its tiles one after another then, and is better off in a call of its own (us,
+  // 64 single tokens over up to 8192 keys and a chunk over 8192, in one call and in two: a chunk
+  // of 64 tokens 234 and 89, of 128 424 and 101, of 512 1571 and 168, of 900 2743 and 240).
   p.few = rows <= 64 * sequences;
   p.row_parts = 1;
   if (p.few) {
