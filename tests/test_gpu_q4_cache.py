@@ -316,6 +316,33 @@ def test_nan_blocks_reach_only_the_rows_that_see_them(gpu, q_type):
 
 
 @pytest.mark.parametrize("q_type", Q_TYPES)
+def test_infinite_codes_reach_only_the_rows_that_see_them(gpu, q_type):
+    """Blocks whose code 15 stands for an infinity: infinities and NaN where the definition has them, beside finite columns."""
+    for new, contexts, bound in (([30], [30], 30), ([3], [60], 60), ([5, 1], [300, 90], 300), ([120, 80], [120, 333], 4000)):
+        for dim in (64, 128):
+            print(f"[case] attention q4_1 infinite codes {contexts} {q_type} dim={dim}", flush=True)
+            p = Paged4(new, contexts, dim=dim, seed=14)
+            first = contexts[0] - new[0]
+            for at, d, codes in ((first + 1, 6000, {3: 15, 20: 15}), (first + 2, -6000, {3: 15, 7: 10})):  # block 1 of two tokens
+                row = p.seen(p.v4)[p.table[0, at // p.page], at % p.page]
+                row[:, 20:40] = 0
+                row[:, 20:22] = np.array([d], np.float16).view(np.uint8)
+                for i, code in codes.items():
+                    row[:, 24 + i % 16] |= code << (4 if i >= 16 else 0)
+            p.settle()
+            a = Attend(gpu, p, 4, q_type=Q_TYPES[q_type], max_context=bound)
+            a.call()
+            gpu.synchronize()
+            out = ref.decode(a.results()[0], Q_TYPES[q_type])[p.start[0]:p.start[1]]
+            assert np.isfinite(out[:1]).all()
+            assert np.isposinf(out[1:, :, 52]).all() and np.isposinf(out[1, :, 35]).all() and np.isnan(out[2:, :, 35]).all()
+            others = np.delete(out, [35, 52], axis=-1)
+            assert np.isfinite(others).all()
+            V = ref.decode(p.rows(0, p.v), F16)[:, :, 39]
+            assert V[first + 2, 0] == -60000 and p.fault() == 0
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES)
 def test_weights_beside_much_larger_ones_keep_their_precision(gpu, q_type):
     """A first token of near-zero value that takes nearly all of the mass."""
     for new, contexts in (([1, 1], [1000, 333]), ([40], [700])):
